@@ -6,5 +6,7 @@ from .modeling_csm import CSMModel, CSMOutput, CSMKVCache, sample_topk  # noqa: 
 from .processor import CSMProcessor  # noqa: F401
 from .serving import ContinuousBatcher  # noqa: F401
 from .mimi import MimiDecoder, MimiDecodeConfig  # noqa: F401
+from .ops import paged_rope_append, paged_prefix_attention, sample_filtered  # noqa: F401
 
-__all__ = ["CSMConfig", "LlamaSubConfig", "CSMModel", "CSMOutput", "CSMKVCache", "sample_topk", "CSMProcessor", "ContinuousBatcher", "MimiDecoder", "MimiDecodeConfig"]
+__all__ = ["CSMConfig", "LlamaSubConfig", "CSMModel", "CSMOutput", "CSMKVCache", "sample_topk", "CSMProcessor", "ContinuousBatcher", "MimiDecoder", "MimiDecodeConfig", "paged_rope_append", "paged_prefix_attention",
+           "sample_filtered"]

@@ -21,6 +21,15 @@ UNIT_FLAGS = {"attn_prefill": ["-mllvm", "--amdgpu-mfma-vgpr-form"], "gemm16": [
 # being s_loaded by every wave at its first instruction (gemv.h GEMV_HOT_PARAMS; round 6)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Wno-pass-failed", "-mllvm", "-amdgpu-kernarg-preload-count=16"]
 
+# stand-alone operators (include/csm_ops.h) in a library of their own: they need no engine, and the engine library's measurement records are
+# stamped with ITS sources.  packed-fp32-ops off: no v_pk_*_f32 in these kernels
+OPS_SRC = os.path.join(CSRC, "ops")
+OPS_LIB = os.path.join(HERE, "libcsm_ops.so")
+OPS_UNITS = ["ops_api", "paged_append", "paged_attn", "sample_filtered"]
+OPS_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Wno-pass-failed",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+OPS_UNIT_FLAGS = {}
+
 
 def _hipcc() -> str:
     for c in (os.environ.get("HIPCC"), shutil.which("hipcc"), "/opt/rocm/bin/hipcc"):
@@ -56,6 +65,8 @@ def build_library(force: bool = False, verbose: bool = False, defines=(), out: s
     run time with the CSM_HIP_LIB environment variable."""
     global OBJ
     lib_out = out or LIB
+    if not defines and out is None:
+        build_ops_library(force, verbose)
     if not force and not defines and os.path.exists(LIB) and os.path.getmtime(LIB) >= _sources_mtime():
         return LIB
     hipcc = _hipcc()
@@ -77,6 +88,32 @@ def build_library(force: bool = False, verbose: bool = False, defines=(), out: s
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr[-4000:]}")
     return lib_out
+
+
+def build_ops_library(force: bool = False, verbose: bool = False) -> str:
+    """libcsm_ops.so from csrc/ops (include/csm_ops.h); reused when it is newer than its sources unless `force`."""
+    deps = [os.path.join(OPS_SRC, f) for f in os.listdir(OPS_SRC) if f.endswith((".hip", ".h"))]
+    deps += [os.path.join(CSRC, "common.h"), os.path.join(os.path.dirname(HERE), "include", "csm_ops.h")]
+    if not force and os.path.exists(OPS_LIB) and os.path.getmtime(OPS_LIB) >= max(os.path.getmtime(f) for f in deps):
+        return OPS_LIB
+    hipcc, obj_dir = _hipcc(), os.path.join(OPS_SRC, "build")
+    os.makedirs(obj_dir, exist_ok=True)
+
+    def compile_one(u):
+        cmd = [hipcc, *OPS_FLAGS, *OPS_UNIT_FLAGS.get(u, []), "-c", os.path.join(OPS_SRC, u + ".hip"), "-o", os.path.join(obj_dir, u + ".o")]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"hipcc failed for ops/{u}.hip:\n{r.stderr[-4000:]}")
+        if verbose:
+            print(f"[build] ops/{u}.o", file=sys.stderr)
+
+    with ThreadPoolExecutor(min(len(OPS_UNITS), os.cpu_count() or 4)) as ex:
+        list(ex.map(compile_one, OPS_UNITS))
+    cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *[os.path.join(obj_dir, u + ".o") for u in OPS_UNITS], "-o", OPS_LIB]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{r.stderr[-4000:]}")
+    return OPS_LIB
 
 
 if __name__ == "__main__":

@@ -1,0 +1,123 @@
+// Rotary embedding + append into a paged KV cache: raw q|k|v rows -> rotated q, rotated k and v in their cache slots, one launch.
+//   y[i] = x[i] cos - x[i + d/2] sin,   y[i + d/2] = x[i + d/2] cos + x[i] sin,   angle of position pos_offset + slot
+// Bound by memory: every input element is read once, every output written once, 1.5 flops per byte.  A thread owns 16 elements of one head:
+// 8 of the lower half and the 8 they rotate with (q, k), or 16 consecutive ones (v), so that both partners are in its registers and all
+// traffic is 16-byte vectors; consecutive threads take consecutive 8-element pieces of a row.
+#include "ops_common.h"
+
+struct AppendArgs {
+  Paged c;
+  const void* qkv;
+  void *k, *v, *q_out;
+  const float *cos_t, *sin_t;
+  int64_t qkv_stride, q_stride;
+  int n_q, hd, units, total, rope_positions, pos_offset;   // units: 16-element pieces of a row; total = rows * units
+};
+
+constexpr int APPEND_THREADS = 256, CU_LDS = 1024;
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  W8<T> w;
+  w.load(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = w.get(i);
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+  *reinterpret_cast<f32x4*>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+}
+__device__ __forceinline__ void store8(bf16_t* p, const float (&x)[8]) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)f32_to_bf16(x[2 * i]) | ((uint32_t)f32_to_bf16(x[2 * i + 1]) << 16);
+  *reinterpret_cast<u32x4*>(p) = w;
+}
+
+template <typename XT, typename CT>
+__global__ __launch_bounds__(APPEND_THREADS) void paged_append_kernel(AppendArgs a) {
+  __shared__ int32_t cu_s[CU_LDS];
+  const Paged& c = a.c;
+  const int32_t* cu = c.cu;
+  if (cu && c.n_seqs < CU_LDS) {   // the search is a chain of dependent reads: make them LDS reads
+    for (int i = threadIdx.x; i <= c.n_seqs; i += APPEND_THREADS) cu_s[i] = cu[i];
+    __syncthreads();
+    cu = cu_s;
+  }
+  const int idx = blockIdx.x * APPEND_THREADS + threadIdx.x;
+  if (idx >= a.total) return;
+  const int row = idx / a.units, unit = idx - row * a.units;
+  int seq = row, t = 0, n_new = 1;
+  if (c.cu) {
+    seq = ops_find_seq(cu, c.n_seqs, row);
+    if (seq < 0) return;
+    t = row - cu[seq];
+    n_new = cu[seq + 1] - cu[seq];
+  }
+  const int len = c.lens[seq];
+  const int64_t slot64 = (int64_t)len - n_new + t, pos = slot64 + a.pos_offset;
+  if (len < 0 || slot64 < 0 || slot64 > 0x7fffffff || pos >= a.rope_positions) return;
+  const int slot = (int)slot64;
+  const int page = ops_page(c.table + seq * c.table_stride, c.width, c.n_pages, c.shift, slot);
+  if (page < 0) return;
+  const int per_head = a.hd >> 4, head = unit / per_head, piece = unit - head * per_head, half = a.hd >> 1;
+  const int in_page = slot & ((1 << c.shift) - 1);
+  const bool is_v = head >= a.n_q + c.n_kv;
+  const int i0 = is_v ? 16 * piece : 8 * piece, i1 = is_v ? i0 + 8 : i0 + half;
+  const XT* x = reinterpret_cast<const XT*>(a.qkv) + row * a.qkv_stride + (int64_t)head * a.hd;
+  float lo[8], hi[8];
+  load8(x + i0, lo);
+  load8(x + i1, hi);
+  if (!is_v) {
+    float cs[8], sn[8];
+    load8(a.cos_t + pos * half + i0, cs);
+    load8(a.sin_t + pos * half + i0, sn);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float l = lo[i], h = hi[i];
+      lo[i] = l * cs[i] - h * sn[i];
+      hi[i] = h * cs[i] + l * sn[i];
+    }
+  }
+  if (head < a.n_q) {
+    XT* y = reinterpret_cast<XT*>(a.q_out) + row * a.q_stride + (int64_t)head * a.hd;
+    store8(y + i0, lo);
+    store8(y + i1, hi);
+  } else {
+    const int h = is_v ? head - a.n_q - c.n_kv : head - a.n_q;
+    CT* y = is_v ? reinterpret_cast<CT*>(a.v) + page * c.vp + h * c.vh + in_page * c.vs : reinterpret_cast<CT*>(a.k) + page * c.kp + h * c.kh + in_page * c.ks;
+    store8(y + i0, lo);
+    store8(y + i1, hi);
+  }
+}
+
+extern "C" int csm_ops_paged_rope_append(const csm_ops_rope_append_t* p, void* stream) {
+  if (!p) return ops_fail(CSM_OPS_ERR_ARG, "null argument");
+  const csm_ops_paged_t& c = p->c;
+  if (const int r = ops_check_paged(c)) return r;
+  if (p->x_dtype != CSM_OPS_F32 && p->x_dtype != CSM_OPS_BF16) return ops_fail(CSM_OPS_ERR_ARG, "unknown dtype %d", p->x_dtype);
+  if (p->n_q < 1) return ops_fail(CSM_OPS_ERR_ARG, "n_q must be positive");
+  if (c.head_dim % 16 || c.head_dim > 256) return ops_fail(CSM_OPS_ERR_ARG, "head_dim %d is not a multiple of 16 up to 256", c.head_dim);
+  if (p->pos_offset < 0 || p->rope_positions < 0) return ops_fail(CSM_OPS_ERR_ARG, "negative position");
+  if (!c.rows) return 0;
+  if (!p->qkv || !p->q_out || !p->cos || !p->sin) return ops_fail(CSM_OPS_ERR_ARG, "null pointer");
+  if (!ops_aligned(p->qkv) || !ops_aligned(p->q_out) || !ops_aligned(p->cos) || !ops_aligned(p->sin) || !ops_stride16(p->qkv_stride, p->x_dtype) ||
+      !ops_stride16(p->q_out_stride, p->x_dtype))
+    return ops_fail(CSM_OPS_ERR_ARG, "qkv, q_out, cos and sin must start on 16 bytes and have rows of multiples of 16 bytes");
+  const int64_t units = (int64_t)(p->n_q + 2 * (int64_t)c.n_kv) * (c.head_dim / 16), total = units * c.rows;
+  if (total > 0x7fffff00) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
+  AppendArgs a;
+  a.c = ops_paged(c);
+  a.qkv = p->qkv; a.k = c.k; a.v = c.v; a.q_out = p->q_out; a.cos_t = p->cos; a.sin_t = p->sin;
+  a.qkv_stride = p->qkv_stride; a.q_stride = p->q_out_stride; a.n_q = p->n_q; a.hd = c.head_dim;
+  a.units = (int)units; a.total = (int)total; a.rope_positions = p->rope_positions; a.pos_offset = p->pos_offset;
+  const dim3 grid((unsigned)((total + APPEND_THREADS - 1) / APPEND_THREADS));
+  hipStream_t st = (hipStream_t)stream;
+  const bool xb = p->x_dtype == CSM_OPS_BF16, cb = c.dtype == CSM_OPS_BF16;
+  if (xb && cb) hipLaunchKernelGGL((paged_append_kernel<bf16_t, bf16_t>), grid, dim3(APPEND_THREADS), 0, st, a);
+  else if (xb) hipLaunchKernelGGL((paged_append_kernel<bf16_t, float>), grid, dim3(APPEND_THREADS), 0, st, a);
+  else if (cb) hipLaunchKernelGGL((paged_append_kernel<float, bf16_t>), grid, dim3(APPEND_THREADS), 0, st, a);
+  else hipLaunchKernelGGL((paged_append_kernel<float, float>), grid, dim3(APPEND_THREADS), 0, st, a);
+  OPS_HIP(hipGetLastError());
+  return 0;
+}
