@@ -28,7 +28,7 @@ OPS_LIB = os.path.join(HERE, "libcsm_ops.so")
 OPS_UNITS = ["ops_api", "paged_append", "paged_attn", "sample_filtered"]
 OPS_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Wno-pass-failed",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-OPS_UNIT_FLAGS = {}
+OPS_UNIT_FLAGS = {"paged_attn": ["-mllvm", "--amdgpu-mfma-vgpr-form"]}   # accumulators in VGPRs: the softmax reads every score at once
 
 
 def _hipcc() -> str:

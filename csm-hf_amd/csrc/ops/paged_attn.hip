@@ -1,8 +1,26 @@
 // Attention of a batch over a shared prefix and each sequence's own pages (include/csm_ops.h).
 //   out[r, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q.k_j - m),   j over the prefix's slots and own slots 0 .. slot(r)
-// First form: one wave per (row, head); the head's elements are spread over the lanes, one key at a time with a running maximum and sum.
+//
+// The keys of a row form one axis: prefix slots 0 .. P-1, then own slots.  Query rows of one kv-head are FLATTENED to (token row, head of the
+// group): f = row * rep + h.  A workgroup takes up to 64 such rows and a range of the axis:
+//   prefix item : rows of the WHOLE batch, range inside the prefix -- a prefix slot is fetched once per 64 rows, not once per sequence;
+//   own item    : rows of one sequence, range inside its own slots (its prefix too, where every sequence brings rows enough of its own);
+// and leaves (max, sum, unnormalised output) per row, which a second small launch joins.  Up to 16 live rows: the four waves split the keys and
+// join through LDS.  More: the waves split the rows.
+//
+// One pass per wave, 16 query rows at a time, both products transposed so that a lane owns one query row from score to result:
+//   S^T[key][row] = K Q^T   lane (row = lane % 16, g = lane / 16) ends with the scores of keys 4g .. 4g+3 of each 16-key group
+//   O^T[d][row]  += V^T P^T contracted over keys in exactly that order, so P never leaves its lane
+// K goes from memory straight into the A operand (a lane's 16 bytes are 8 elements of one key); V passes through a wave-private LDS tile and
+// ds_read_b64_tr_b16, which hands out the columns.  The running reference m moves only when a score exceeds it by 2^8 (p <= 256 is harmless in
+// fp32 sums), so no cross-lane maximum and no rescaling happen in most tiles.
 #include "ops_common.h"
 #include <math.h>
+
+typedef __attribute__((ext_vector_type(8))) short b16x8;
+typedef __attribute__((ext_vector_type(4))) short b16x4;
+typedef __attribute__((ext_vector_type(2))) float f2;
+typedef __attribute__((ext_vector_type(2))) __bf16 b2;
 
 struct AttnOpArgs {
   Paged c;
@@ -10,51 +28,465 @@ struct AttnOpArgs {
   void* out;
   const int32_t* prefix;
   int64_t q_stride, out_stride;
-  int n_q, prefix_pages, prefix_len;
-  float scale;
+  int n_q, rep, prefix_len;
+  float c2;               // |scale| log2(e); the sign of scale is folded into q
+  uint32_t q_flip;
+  int np_tiles, nsp, no_tiles, nso, per_seq_tiles, with_prefix, nsplit;   // nsplit = partial results per row
+  float* part;            // [rows * n_q][nsplit][hd]
+  float2* ml;             // [rows * n_q][nsplit] (reference in log2 units, sum)
+};
+
+constexpr int AT = 256, MAX_SPLIT = 64, ROWS = 64;
+constexpr float SLACK = 8.f;
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {   // round to nearest even
+  const f2 v = {lo, hi};
+  const b2 r = __builtin_convertvector(v, b2);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_trunc(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
+__device__ __forceinline__ float trunc_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ float xor16_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// 8 floats as N bf16 pieces: one rounded piece, or an exact sum of truncated ones (2: 16 bits, 3: all 24)
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], b16x8 (&out)[N]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = n == N - 1 ? pack_bf16(r[2 * i], r[2 * i + 1]) : pack_trunc(r[2 * i], r[2 * i + 1]);
+    if (n < N - 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] -= trunc_bf16(r[i]);
+    }
+    out[n] = *reinterpret_cast<const b16x8*>(&w);
+  }
+}
+
+// ---- products of one wave, by type.  NG = 16-key groups per tile -------------------------------
+template <typename XT, typename CT, int HD>
+struct Prod;
+
+// bf16 cache: v_mfma_f32_16x16x32_bf16.  bf16 queries: one piece of q; p in two bf16 pieces (16 bits), so that rounding p adds nothing to the one
+// rounding of the result -- the launch waits for memory, the second product is free.  fp32 queries: q and p as three pieces each, exactly.
+template <typename XT, int HD>
+struct Prod<XT, bf16_t, HD> {
+  static constexpr int NG = 2, NQ = sizeof(XT) == 2 ? 1 : 3, NP = sizeof(XT) == 2 ? 2 : 3, T = HD / 32, LPK = HD / 8, KPP = 64 / LPK, NV = 32 / KPP;
+  static constexpr int LDS_BYTES = 32 * HD * 2;
+  b16x8 q[NQ][T];
+  struct Tile { u32x4 k[NG][T], v[NV]; };
+
+  __device__ __forceinline__ void load_q(const XT* p, int g, uint32_t flip) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      float x[8];
+      W8<XT> w;
+      if (p) w.load(p + 32 * t + 8 * g); else w.zero();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(__float_as_uint(w.get(i)) ^ flip);
+      b16x8 f[NQ];
+      split8<NQ>(x, f);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) q[n][t] = f[n];
+    }
+  }
+  // pg[kt], sl[kt]: page (0 where there is none) and slot in it of key 16 kt + lane % 16
+  static __device__ __forceinline__ void load(Tile& t, const bf16_t* kb, const bf16_t* vb, const Paged& c, const int (&pg)[NG], const int (&sl)[NG], int lane) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int kt = 0; kt < NG; ++kt) {
+      const bf16_t* p = kb + pg[kt] * c.kp + sl[kt] * c.ks + 8 * g;
+#pragma unroll
+      for (int s = 0; s < T; ++s) t.k[kt][s] = *reinterpret_cast<const u32x4*>(p + 32 * s);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int kk = i * KPP, from = (kk & 15) + lane / LPK;   // key kk + lane / LPK of the tile
+      const int page = __shfl(pg[kk >> 4], from), slot = __shfl(sl[kk >> 4], from);
+      t.v[i] = *reinterpret_cast<const u32x4*>(vb + page * c.vp + slot * c.vs + (lane % LPK) * 8);
+    }
+  }
+  __device__ __forceinline__ void scores(const Tile& t, f32x4 (&s)[NG]) const {
+#pragma unroll
+    for (int kt = 0; kt < NG; ++kt) {
+      s[kt] = (f32x4)(0.f);
+#pragma unroll
+      for (int n = NQ - 1; n >= 0; --n)
+#pragma unroll
+        for (int x = 0; x < T; ++x) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const b16x8*>(&t.k[kt][x]), q[n][x], s[kt], 0, 0, 0);
+    }
+  }
+  // 16-byte chunk ch of key kk lies at chunk ch ^ (kk & 7): the rows of a transposing read then cover all banks
+  static __device__ __forceinline__ void stage_v(const Tile& t, char* lds, int lane, uint32_t valid) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int kk = i * KPP + lane / LPK, ch = lane % LPK;
+      u32x4 x = t.v[i];
+      if (valid != 0xffffffffu && !((valid >> kk) & 1)) x = (u32x4)(0u);   // 0 * (what an unused slot holds) must be 0
+      *reinterpret_cast<u32x4*>(lds + kk * HD * 2 + ((ch ^ (kk & 7)) << 4)) = x;
+    }
+  }
+  static __device__ __forceinline__ void accumulate(const f32x4 (&p)[NG], char* lds, f32x4 (&o)[HD / 16], int lane) {
+    const int g = lane >> 4, li = lane & 15;
+    const float x[8] = {p[0][0], p[0][1], p[0][2], p[0][3], p[1][0], p[1][1], p[1][2], p[1][3]};
+    b16x8 f[NP];
+    split8<NP>(x, f);
+    const int k0 = 4 * g + (li >> 2), k1 = 16 + k0;   // k0 & 7 == k1 & 7
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) {
+      const int at = (((2 * dt + ((li & 3) >> 1)) ^ (k0 & 7)) << 4) + (li & 1) * 8;
+      typedef __attribute__((address_space(3))) b16x4* lp;
+      const b16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + k0 * HD * 2 + at));
+      const b16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + k1 * HD * 2 + at));
+      const b16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+      for (int n = NP - 1; n >= 0; --n) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, f[n], o[dt], 0, 0, 0);
+    }
+  }
+};
+
+// fp32 cache and queries: v_mfma_f32_16x16x4_f32, fp32 throughout.  Contraction step (u, e) of the scores takes d = 16 u + 4 g + e from lane
+// group g, so that a lane's 16-byte loads of K and Q are operands as they are.
+template <int HD>
+struct Prod<float, float, HD> {
+  static constexpr int NG = 1, U = HD / 16, LPK = HD / 4, KPP = 64 / LPK, NV = 16 / KPP, LD = HD + 4;   // LDS rows 4 floats longer: groups of rows on different banks
+  static constexpr int LDS_BYTES = 16 * LD * 4;
+  f32x4 q[U];
+  struct Tile { f32x4 k[NG][U], v[NV]; };
+
+  __device__ __forceinline__ void load_q(const float* p, int g, uint32_t flip) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      f32x4 x = (f32x4)(0.f);
+      if (p) x = *reinterpret_cast<const f32x4*>(p + 16 * u + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[u][e] = __uint_as_float(__float_as_uint(x[e]) ^ flip);
+    }
+  }
+  static __device__ __forceinline__ void load(Tile& t, const float* kb, const float* vb, const Paged& c, const int (&pg)[NG], const int (&sl)[NG], int lane) {
+    const float* p = kb + pg[0] * c.kp + sl[0] * c.ks + 4 * (lane >> 4);
+#pragma unroll
+    for (int u = 0; u < U; ++u) t.k[0][u] = *reinterpret_cast<const f32x4*>(p + 16 * u);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int from = i * KPP + lane / LPK;
+      const int page = __shfl(pg[0], from), slot = __shfl(sl[0], from);
+      t.v[i] = *reinterpret_cast<const f32x4*>(vb + page * c.vp + slot * c.vs + (lane % LPK) * 4);
+    }
+  }
+  __device__ __forceinline__ void scores(const Tile& t, f32x4 (&s)[NG]) const {
+    f32x4 a = (f32x4)(0.f);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[0][u][e], q[u][e], a, 0, 0, 0);
+    s[0] = a;
+  }
+  static __device__ __forceinline__ void stage_v(const Tile& t, char* lds, int lane, uint32_t valid) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int kk = i * KPP + lane / LPK;
+      f32x4 x = t.v[i];
+      if ((valid & 0xffffu) != 0xffffu && !((valid >> kk) & 1)) x = (f32x4)(0.f);
+      *reinterpret_cast<f32x4*>(lds + (kk * LD + (lane % LPK) * 4) * 4) = x;
+    }
+  }
+  static __device__ __forceinline__ void accumulate(const f32x4 (&p)[NG], char* lds, f32x4 (&o)[HD / 16], int lane) {
+    const float* v = reinterpret_cast<const float*>(lds) + 4 * (lane >> 4) * LD + (lane & 15);
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e * LD + 16 * dt], p[0][e], o[dt], 0, 0, 0);
+  }
+};
+
+// ---- one wave over keys [k0, k1) of the axis, tiles first, first + step, ... -------------------------------------------------------------
+struct KeyAxis {
+  const int32_t *prefix, *own;
+  int prefix_len;
+  __device__ __forceinline__ int page(int j, const Paged& c) const {   // of axis position j, -1 where it does not exist
+    const int s = j < prefix_len ? j : j - prefix_len;
+    const int p = (j < prefix_len ? prefix : own)[s >> c.shift];
+    return (unsigned)p < (unsigned)c.n_pages ? p : -1;
+  }
+  __device__ __forceinline__ int slot(int j, const Paged& c) const { return (j < prefix_len ? j : j - prefix_len) & ((1 << c.shift) - 1); }
 };
 
 template <typename XT, typename CT, int HD>
-__global__ __launch_bounds__(64) void paged_attn_simple_kernel(AttnOpArgs a) {
-  constexpr int N = HD / 64;
-  const Paged& c = a.c;
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kvh = h / (a.n_q / c.n_kv);
-  int seq = row, t = 0, n_new = 1;
-  if (c.cu) {
-    seq = ops_find_seq(c.cu, c.n_seqs, row);
-    if (seq < 0) return;
-    t = row - c.cu[seq];
-    n_new = c.cu[seq + 1] - c.cu[seq];
+__device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const Prod<XT, CT, HD>& pr, const KeyAxis& ax, int kvh, int k0, int k1, int first, int step,
+                                            int lim, int lim_min, char* lds, f32x4 (&o)[HD / 16], float& m, float& l) {
+  using P = Prod<XT, CT, HD>;
+  constexpr int NG = P::NG, KT = 16 * NG;
+  const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const CT* kb = reinterpret_cast<const CT*>(a.k) + kvh * a.c.kh;
+  const CT* vb = reinterpret_cast<const CT*>(a.v) + kvh * a.c.vh;
+  m = -INFINITY; l = 0.f;
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i) o[i] = (f32x4)(0.f);
+
+  auto look = [&](int j0, int (&pg)[NG], int (&sl)[NG]) {
+#pragma unroll
+    for (int kt = 0; kt < NG; ++kt) {
+      const int j = j0 + 16 * kt + li;
+      pg[kt] = j < k1 ? ax.page(j, a.c) : -1;
+      sl[kt] = j < k1 ? ax.slot(j, a.c) : 0;
+    }
+  };
+  auto fetch = [&](typename P::Tile& t, const int (&pg)[NG], const int (&sl)[NG], uint32_t& valid) {
+    int safe[NG];
+    valid = 0;
+#pragma unroll
+    for (int kt = 0; kt < NG; ++kt) {
+      valid |= ((uint32_t)__ballot(pg[kt] >= 0) & 0xffffu) << (16 * kt);
+      safe[kt] = pg[kt] < 0 ? 0 : pg[kt];   // page 0 exists: n_pages >= 1 here
+    }
+    P::load(t, kb, vb, a.c, safe, sl, lane);
+  };
+  int j = k0 + first * KT;
+  const int hop = step * KT;
+  if (j >= k1) return;
+  typename P::Tile t;
+  uint32_t valid;
+  int pg[NG], sl[NG];
+  look(j, pg, sl);
+  fetch(t, pg, sl, valid);
+  look(j + hop, pg, sl);
+  for (; j < k1; j += hop) {
+    constexpr uint32_t ALL = NG == 2 ? 0xffffffffu : 0xffffu;
+    f32x4 s[NG];
+    P::stage_v(t, lds, lane, valid);
+    pr.scores(t, s);
+    if (valid != ALL || j + KT > lim_min) {
+#pragma unroll
+      for (int kt = 0; kt < NG; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int kk = 16 * kt + 4 * g + e;
+          s[kt][e] = ((valid >> kk) & 1) && j + kk < lim ? s[kt][e] : -INFINITY;
+        }
+    }
+    if (j + hop < k1) {   // the tile's registers are free: the next one is in flight behind the softmax and the second product
+      fetch(t, pg, sl, valid);
+      look(j + 2 * hop, pg, sl);
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int kt = 0; kt < NG; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kt][e]);
+    top *= a.c2;
+    if (__any(top > m + SLACK)) {   // (-inf + 8 = -inf: the first tile with a key always comes here)
+      top = xor32_max(xor16_max(top));
+      const float m_new = fmaxf(m, top), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) o[i] *= alpha;
+      m = m_new;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int kt = 0; kt < NG; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[kt][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[kt][e], a.c2, -ref));
+        l += s[kt][e];
+      }
+    P::accumulate(s, lds, o, lane);
   }
-  const int len = c.lens[seq];
-  if (len < 0) return;
-  const int64_t seen64 = (int64_t)len - n_new + t + 1, cap = (int64_t)c.width << c.shift;
-  const int own = (int)(seen64 < 0 ? 0 : seen64 > cap ? cap : seen64);
-  float q[N], o[N] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) q[i] = to_f32(reinterpret_cast<const XT*>(a.q)[row * a.q_stride + (int64_t)h * HD + i * 64 + lane]) * a.scale;
-  for (int j = 0; j < a.prefix_len + own; ++j) {
-    const bool in_prefix = j < a.prefix_len;
-    const int slot = in_prefix ? j : j - a.prefix_len;
-    const int page = in_prefix ? ops_page(a.prefix, a.prefix_pages, c.n_pages, c.shift, slot) : ops_page(c.table + seq * c.table_stride, c.width, c.n_pages, c.shift, slot);
-    if (page < 0) continue;
-    const int at = slot & ((1 << c.shift) - 1);
-    const CT* kp = reinterpret_cast<const CT*>(a.k) + page * c.kp + kvh * c.kh + at * c.ks;
-    const CT* vp = reinterpret_cast<const CT*>(a.v) + page * c.vp + kvh * c.vh + at * c.vs;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) s += q[i] * to_f32(kp[i * 64 + lane]);
-    s = wave_sum(s);
-    const float m_new = fmaxf(m, s), ref = m_new == -INFINITY ? 0.f : m_new, alpha = __expf(m - ref), p = __expf(s - ref);
-    l = l * alpha + p;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * alpha + p * to_f32(vp[i * 64 + lane]);
-    m = m_new;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) store_kv(reinterpret_cast<XT*>(a.out) + row * a.out_stride + (int64_t)h * HD + i * 64 + lane, l == 0.f ? 0.f : o[i] / l);
+  l = xor32_sum(xor16_sum(l));
 }
 
+// ---- results ------------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
+__device__ __forceinline__ void store4(bf16_t* p, const f32x4& v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])); }
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }   // a row without a key: zeros
+
+// sequence and tile of own item `tile` when rows are ragged: tiles are counted per sequence in order
+__device__ __forceinline__ bool find_tile(const AttnOpArgs& a, int tile, int& seq, int& first, int& n_rows, int& in_seq) {
+  const Paged& c = a.c;
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int b0 = 0; b0 < c.n_seqs; b0 += 64) {
+    const int b = b0 + lane;
+    int lo = 0, n = 0;
+    if (b < c.n_seqs) {
+      lo = min(max(c.cu[b], 0), c.rows);
+      n = min(max(c.cu[b + 1], lo), c.rows) - lo;
+    }
+    const int tiles = (n * a.rep + ROWS - 1) / ROWS;
+    int upto = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(upto, d);
+      if (lane >= d) upto += y;
+    }
+    const uint64_t past = __ballot(before + upto > tile);
+    if (past) {
+      const int w = __ffsll((unsigned long long)past) - 1;
+      seq = b0 + w;
+      first = __builtin_amdgcn_readlane(lo, w);
+      n_rows = __builtin_amdgcn_readlane(n, w);
+      in_seq = tile - before - __builtin_amdgcn_readlane(upto - tiles, w);
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+template <typename XT, typename CT, int HD>
+__global__ __launch_bounds__(AT, 2) void paged_attn_kernel(AttnOpArgs a) {
+  using P = Prod<XT, CT, HD>;
+  constexpr int WAVE_LDS = P::LDS_BYTES > 16 * (HD + 4) * 4 ? P::LDS_BYTES : 16 * (HD + 4) * 4;   // V tile; at the end 16 rows of fp32 results
+  __shared__ __attribute__((aligned(16))) char lds[4 * WAVE_LDS];
+  __shared__ float ml_s[4][16][2];
+  const Paged& c = a.c;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.x % c.n_kv;   // fastest: with 8 kv-heads the items of one head share an XCD's L2
+  int it = blockIdx.x / c.n_kv;
+
+  int row0, f0, live, slot_bias, k0, k1, split, axis_end;
+  KeyAxis ax{a.prefix, nullptr, a.prefix_len};
+  const bool own = it >= a.np_tiles * a.nsp;
+  int len = 0, n_rows = 1;
+  // keys that token row t of an own item sees, the prefix among them: its own slots are 0 .. slot_bias + t - 1, as far as the table goes
+  const int cap = c.width << c.shift;
+  auto sees = [&](int t) { return a.prefix_len + min(max(slot_bias + t, 0), cap); };
+  if (!own) {
+    split = it % a.nsp;
+    f0 = (it / a.nsp) * ROWS;
+    row0 = 0;
+    live = min(ROWS, c.rows * a.rep - f0);
+    slot_bias = 0;
+    k0 = 0; axis_end = a.prefix_len;
+  } else {
+    it -= a.np_tiles * a.nsp;
+    split = it % a.nso;
+    const int tile = it / a.nso;
+    int seq, in_seq;
+    if (c.cu) {
+      if (!find_tile(a, tile, seq, row0, n_rows, in_seq)) return;
+    } else {
+      seq = tile / a.per_seq_tiles;
+      in_seq = tile - seq * a.per_seq_tiles;
+      row0 = seq;
+    }
+    len = c.lens[seq];
+    if (len < 0) return;
+    f0 = in_seq * ROWS;
+    live = min(ROWS, n_rows * a.rep - f0);
+    ax.own = c.table + seq * c.table_stride;
+    slot_bias = len - n_rows + 1;
+    k0 = a.with_prefix ? 0 : a.prefix_len;
+    axis_end = sees((f0 + live - 1) / a.rep);
+  }
+  const int nsplit = own ? a.nso : a.nsp, slot0 = own ? a.nsplit - a.nso : 0;
+  {
+    constexpr int KT = 16 * P::NG;
+    const int span = max(axis_end - k0, 0), chunk = ((span + nsplit - 1) / nsplit + KT - 1) / KT * KT;
+    k0 = min(k0 + split * chunk, axis_end);
+    k1 = min(k0 + chunk, axis_end);
+    if (c.n_pages == 0) k1 = k0;
+  }
+  // rows of this wave: all waves the same 16 (keys split over the waves), or 16 each
+  const bool by_keys = live <= 16;
+  const int mine = by_keys ? 0 : 16 * wave, n_mine = min(16, live - mine);
+  char* my_lds = lds + wave * WAVE_LDS;
+  f32x4 o[HD / 16];
+  float m = -INFINITY, l = 0.f;
+  const int f = f0 + mine + li, row = row0 + f / a.rep, head = kvh * a.rep + f % a.rep;
+  const bool row_live = li < n_mine;
+  if (n_mine > 0) {
+    P pr;
+    pr.load_q(row_live ? reinterpret_cast<const XT*>(a.q) + row * a.q_stride + (int64_t)head * HD : nullptr, g, a.q_flip);
+    const int lim = own ? sees(f / a.rep) : a.prefix_len, lim_min = own ? sees((f0 + mine) / a.rep) : a.prefix_len;   // rows ascend: the first sees least
+    wave_attend<XT, CT, HD>(a, pr, ax, kvh, k0, k1, by_keys ? wave : 0, by_keys ? 4 : 1, lim, lim_min, my_lds, o, m, l);
+  }
+  if (by_keys) {   // join the four waves: every one rescales to the common reference and leaves its rows in LDS
+    if (g == 0) { ml_s[wave][li][0] = m; ml_s[wave][li][1] = l; }
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml_s[w][li][0]);
+    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    float* mine_o = reinterpret_cast<float*>(my_lds) + li * (HD + 4);
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) store4(mine_o + 16 * dt + 4 * g, o[dt] * alpha);
+    __syncthreads();
+    for (int i = threadIdx.x; i < live * (HD / 4); i += AT) {
+      const int r = i / (HD / 4), d = (i % (HD / 4)) * 4, ff = f0 + r;
+      const int rr = row0 + ff / a.rep, hh = kvh * a.rep + ff % a.rep;
+      f32x4 sum = (f32x4)(0.f);
+      float top_r = -INFINITY, l_r = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top_r = fmaxf(top_r, ml_s[w][r][0]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * WAVE_LDS) + r * (HD + 4) + d);
+        const float mw = ml_s[w][r][0];
+        l_r += mw == -INFINITY ? ml_s[w][r][1] : ml_s[w][r][1] * __builtin_amdgcn_exp2f(mw - top_r);
+      }
+      const int64_t at = (int64_t)rr * a.n_q + hh;
+      if (a.nsplit == 1) {
+        store4(reinterpret_cast<XT*>(a.out) + rr * a.out_stride + (int64_t)hh * HD + d, sum * inverse(l_r));
+      } else {
+        store4(a.part + (at * a.nsplit + slot0 + split) * HD + d, sum);
+        if (d == 0) a.ml[at * a.nsplit + slot0 + split] = make_float2(top_r, l_r);
+      }
+    }
+    return;
+  }
+  if (!row_live) return;
+  const int64_t at = (int64_t)row * a.n_q + head;
+  if (a.nsplit == 1) {
+    const float inv = inverse(l);
+    XT* y = reinterpret_cast<XT*>(a.out) + row * a.out_stride + (int64_t)head * HD + 4 * g;
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) store4(y + 16 * dt, o[dt] * inv);
+  } else {
+    float* y = a.part + (at * a.nsplit + slot0 + split) * HD + 4 * g;
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) store4(y + 16 * dt, o[dt]);
+    if (g == 0) a.ml[at * a.nsplit + slot0 + split] = make_float2(m, l);
+  }
+}
+
+// join the partial results of a (row, head): one wave each
+template <typename XT, int HD>
+__global__ __launch_bounds__(AT) void paged_attn_join_kernel(AttnOpArgs a) {
+  const Paged& c = a.c;
+  const int lane = threadIdx.x & 63;
+  const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (at >= (int64_t)c.rows * a.n_q) return;
+  const int row = (int)(at / a.n_q), head = (int)(at - (int64_t)row * a.n_q);
+  const int seq = c.cu ? ops_find_seq(c.cu, c.n_seqs, row) : row;
+  if (seq < 0 || c.lens[seq] < 0) return;
+  const float2 x = lane < a.nsplit ? a.ml[at * a.nsplit + lane] : make_float2(-INFINITY, 0.f);
+  const float top = wave_max(x.x);
+  const float w = lane < a.nsplit ? (x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x.x - top)) : 0.f;
+  const float inv = inverse(wave_sum(w * x.y));
+  constexpr int N = HD / 64;
+  float o[N] = {};
+  const float* p = a.part + at * a.nsplit * HD + lane * N;
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
+    if (ws != 0.f) {   // (0: a split without a key)
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] += ws * p[(int64_t)s * HD + i];
+    }
+  }
+  XT* y = reinterpret_cast<XT*>(a.out) + row * a.out_stride + (int64_t)head * HD + lane * N;
+#pragma unroll
+  for (int i = 0; i < N; ++i) store_kv(y + i, o[i] * inv);
+}
+
+// ---- entry points -----------------------------------------------------------------------------------------------------------------------
 static int check(const csm_ops_attention_t* p) {
   if (!p) return ops_fail(CSM_OPS_ERR_ARG, "null argument");
   const csm_ops_paged_t& c = p->c;
@@ -65,7 +497,8 @@ static int check(const csm_ops_attention_t* p) {
   if (p->n_q < 1 || p->n_q % c.n_kv) return ops_fail(CSM_OPS_ERR_ARG, "n_q %d is not a multiple of n_kv %d", p->n_q, c.n_kv);
   if (p->prefix_len < 0 || p->prefix_pages < 0) return ops_fail(CSM_OPS_ERR_ARG, "negative size");
   if ((int64_t)p->prefix_pages * c.page_size < p->prefix_len) return ops_fail(CSM_OPS_ERR_ARG, "%d pages of %d slots do not hold a prefix of %d", p->prefix_pages, c.page_size, p->prefix_len);
-  if ((int64_t)c.table_width * c.page_size + p->prefix_len > 0x7fffff00) return ops_fail(CSM_OPS_ERR_CAPACITY, "more than 2^31 slots");
+  if ((int64_t)c.table_width * c.page_size + p->prefix_len > 0x7fff0000) return ops_fail(CSM_OPS_ERR_CAPACITY, "more than 2^31 slots");
+  if ((int64_t)c.rows * p->n_q > (1 << 28) || c.n_seqs > (1 << 28)) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
   if (!isfinite(p->scale)) return ops_fail(CSM_OPS_ERR_ARG, "scale must be finite");
   if (!c.rows) return 0;
   if (!p->q || !p->out || (p->prefix_len && !p->prefix_table)) return ops_fail(CSM_OPS_ERR_ARG, "null pointer");
@@ -74,10 +507,56 @@ static int check(const csm_ops_attention_t* p) {
   return 0;
 }
 
+// How the work is cut.  Items should fill 256 CUs a few times over (a CU holds two workgroups), but an item shorter than 128 keys is mostly
+// start-up, and every split costs a partial result per row.
+static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
+  const csm_ops_paged_t& c = p->c;
+  a.c = ops_paged(c);
+  a.n_q = p->n_q; a.rep = p->n_q / c.n_kv; a.prefix_len = p->prefix_len;
+  const int64_t flat = (int64_t)c.rows * a.rep;
+  a.per_seq_tiles = (a.rep + ROWS - 1) / ROWS;
+  const int64_t own_tiles = c.cu_rows ? flat / ROWS + c.n_seqs : (int64_t)c.n_seqs * a.per_seq_tiles;
+  // sequences that bring half a tile of rows of their own read the prefix with them: nothing to share, nothing to join
+  a.with_prefix = p->prefix_len > 0 && c.cu_rows && c.n_seqs > 0 && flat / c.n_seqs >= ROWS / 2;
+  const int64_t np = p->prefix_len && !a.with_prefix ? (flat + ROWS - 1) / ROWS : 0;
+  const int64_t own_keys = (int64_t)c.table_width * c.page_size + (a.with_prefix ? p->prefix_len : 0);
+  auto splits = [&](int64_t tiles, int64_t keys) {
+    const int64_t want = 1024 / (tiles * c.n_kv < 1 ? 1 : tiles * c.n_kv), most = (keys + 127) / 128;
+    int64_t n = want < most ? want : most;
+    return (int)(n < 1 ? 1 : n > MAX_SPLIT / 2 ? MAX_SPLIT / 2 : n);
+  };
+  a.nsp = np ? splits(np, p->prefix_len) : 0;
+  a.nso = splits(own_tiles, own_keys);
+  a.np_tiles = (int)np; a.no_tiles = (int)own_tiles; a.nsplit = a.nsp + a.nso;
+  if (((int64_t)a.np_tiles * a.nsp + (int64_t)a.no_tiles * a.nso) * c.n_kv > 0x7fffffff) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
+  return 0;
+}
+static size_t workspace(const csm_ops_attention_t* p, const AttnOpArgs& a) {
+  if (a.nsplit <= 1) return 0;
+  return (size_t)p->c.rows * p->n_q * a.nsplit * (p->c.head_dim * sizeof(float) + sizeof(float2));
+}
+
 extern "C" int csm_ops_paged_attention_workspace(const csm_ops_attention_t* p, size_t* bytes) {
   if (!bytes) return ops_fail(CSM_OPS_ERR_ARG, "null argument");
   if (const int r = check(p)) return r;
+  AttnOpArgs a;
   *bytes = 0;
+  if (!p->c.rows) return 0;
+  if (const int r = plan(p, a)) return r;
+  *bytes = workspace(p, a);
+  return 0;
+}
+
+template <typename XT, typename CT, int HD>
+static int launch(const AttnOpArgs& a, hipStream_t st) {
+  const unsigned items = (unsigned)(((int64_t)a.np_tiles * a.nsp + (int64_t)a.no_tiles * a.nso) * a.c.n_kv);
+  hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD>), dim3(items), dim3(AT), 0, st, a);
+  OPS_HIP(hipGetLastError());
+  if (a.nsplit > 1) {
+    const unsigned n = (unsigned)(((int64_t)a.c.rows * a.n_q + 3) / 4);
+    hipLaunchKernelGGL((paged_attn_join_kernel<XT, HD>), dim3(n), dim3(AT), 0, st, a);
+    OPS_HIP(hipGetLastError());
+  }
   return 0;
 }
 
@@ -86,21 +565,18 @@ extern "C" int csm_ops_paged_prefix_attention(const csm_ops_attention_t* p, void
   const csm_ops_paged_t& c = p->c;
   if (!c.rows) return 0;
   AttnOpArgs a;
-  a.c = ops_paged(c);
+  if (const int r = plan(p, a)) return r;
+  const size_t need = workspace(p, a);
+  if (need && (!p->workspace || p->workspace_bytes < need || !ops_aligned(p->workspace)))
+    return ops_fail(CSM_OPS_ERR_CAPACITY, "workspace of %zu bytes: %zu on 16 bytes are needed", p->workspace_bytes, need);
   a.q = p->q; a.k = c.k; a.v = c.v; a.out = p->out; a.prefix = p->prefix_table; a.q_stride = p->q_stride; a.out_stride = p->out_stride;
-  a.n_q = p->n_q; a.prefix_pages = p->prefix_pages; a.prefix_len = p->prefix_len; a.scale = p->scale;
-  const dim3 grid(c.rows, p->n_q);
+  a.part = reinterpret_cast<float*>(p->workspace);
+  a.ml = need ? reinterpret_cast<float2*>(a.part + (size_t)c.rows * p->n_q * a.nsplit * c.head_dim) : nullptr;
+  a.q_flip = p->scale < 0.f ? 0x80000000u : 0u;
+  // a scale of 0 becomes one that no finite score can raise above 0: -inf times it is still -inf
+  a.c2 = fmaxf(fabsf(p->scale) * 1.4426950408889634f, 1e-37f);
   hipStream_t st = (hipStream_t)stream;
   const bool xb = p->x_dtype == CSM_OPS_BF16, cb = c.dtype == CSM_OPS_BF16;
-#define GO(HD)                                                                                                          \
-  do {                                                                                                                  \
-    if (xb) hipLaunchKernelGGL((paged_attn_simple_kernel<bf16_t, bf16_t, HD>), grid, dim3(64), 0, st, a);               \
-    else if (cb) hipLaunchKernelGGL((paged_attn_simple_kernel<float, bf16_t, HD>), grid, dim3(64), 0, st, a);           \
-    else hipLaunchKernelGGL((paged_attn_simple_kernel<float, float, HD>), grid, dim3(64), 0, st, a);                    \
-  } while (0)
-  if (c.head_dim == 64) GO(64);
-  else GO(128);
-#undef GO
-  OPS_HIP(hipGetLastError());
-  return 0;
+  if (c.head_dim == 64) return xb ? launch<bf16_t, bf16_t, 64>(a, st) : cb ? launch<float, bf16_t, 64>(a, st) : launch<float, float, 64>(a, st);
+  return xb ? launch<bf16_t, bf16_t, 128>(a, st) : cb ? launch<float, bf16_t, 128>(a, st) : launch<float, float, 128>(a, st);
 }
