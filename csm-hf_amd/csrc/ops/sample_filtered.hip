@@ -4,13 +4,14 @@
 // Sums are uint64 fixed point (w scaled by 2^min(62 - ceil log2 V, 51)) of weights computed in fp64: exact integer additions, so neither the
 // split over threads nor any order of arrival changes a result, and what is rounded away per weight is below 2^-45 of the largest.
 //
-// One workgroup per row.  No sort: a cut is found by narrowing an interval of order keys (count and mass at or above a probe, one block sum per
-// step; the probe alternates between the middle VALUE, which a smooth row needs few of, and the middle KEY, which bounds any row) until at most
-// 64 entries or one single key are left, which a wave then ranks exactly.
-//   V <= 16 384: the row lives in registers (up to 16 consecutive entries per thread), read once.
-//   larger V:    one pass for the maximum, one for the mass (only where top-p needs the whole row's) and for the entries above a threshold that 4 096
-//                samples put near the 12 288th largest; these are compacted in index order and treated like a short row.  Where that list
-//                is not enough (a flat row whose nucleus is larger), the same search streams over the row.
+// No sort: a cut is found by narrowing an interval of order keys (count and mass at or above a probe, one block sum per step; the probe
+// alternates between the middle VALUE, which a smooth row needs few of, and the middle KEY, which bounds any row) until at most 32 entries or
+// one single key are left, which a wave then ranks exactly.
+//   V <= 16 384: one workgroup, the row in registers (4 or 16 consecutive entries per thread), read once.  Such a launch is a chain of dependent
+//                steps over code that runs once, so its loops carry no branches and its sums stay on the DPP path.
+//   larger V:    three launches, so that few rows still use many CUs: a threshold near the 12 288th largest from 4 096 samples; per chunk of
+//                8 192 entries its maximum, its mass and the entries above the threshold; per row the cuts and the draw on those entries.
+//                Where they are not enough (a flat row whose nucleus is larger), the same search streams over the row.
 #include "ops_common.h"
 #include <math.h>
 
@@ -23,11 +24,18 @@ struct SampleOpArgs {
   float temperature, top_p, min_p;
   int topk;
   int32_t* out;
+  // long rows: workspace
+  int chunks;
+  uint32_t* thr;           // [rows]
+  struct ChunkHead* heads; // [rows][chunks]
+  uint2* lists;            // [rows][chunks][CHUNK_CAP] (key, index)
 };
-constexpr int E = 16;                     // entries per thread
-constexpr int LIST = 1024 * E;            // entries of a compacted list
+constexpr int NT = 1024;                  // threads per row
+constexpr int LIST = NT * 16;             // entries that fit the registers of a workgroup
 constexpr int SAMPLES = 4096, AIM = LIST * 3 / 4;   // the list's threshold is a sample's order statistic that aims at this many entries: at V = 131 072
                                                     // their number scatters by 613, LIST is 6.7 of that away
+constexpr int CHUNK = 8192, CHUNK_CAP = 2048, MAX_V = 1 << 21, MAX_CHUNKS = MAX_V / CHUNK;
+struct ChunkHead { double mass; float mx; int32_t at; uint32_t count, pad; };   // mass relative to the chunk's own maximum, `at` its first place
 
 __device__ __forceinline__ uint32_t order_key(float x) {   // larger float = larger key
   const uint32_t u = __float_as_uint(x);
@@ -41,90 +49,89 @@ __device__ __forceinline__ float logit(const T* x, int i) {   // NaN counts as -
 }
 constexpr uint32_t NEG_INF_KEY = 0x007fffffu;   // order_key(-inf); keys at or below it are no entries
 
-// w * 2^shift as an integer.  2^t = 2^n 2^f with f in [-1/2, 1/2] from its power series (12 terms: below 2^-52); adding 2^52 leaves the rounded
+// w * 2^shift as an integer.  2^t = 2^n 2^f with f in [-1/2, 1/2] from its power series (up to f^11: below 2^-47); adding 2^52 leaves the rounded
 // integer in the mantissa (shift <= 51).
 struct Weigh {
   float mx;
   double k2;   // log2(e) / T
   int shift;
-  __device__ __forceinline__ uint64_t operator()(float x) const {
-    if (x == mx) return 1ull << shift;
-    if (x == -INFINITY || mx == INFINITY) return 0;
+  __device__ __forceinline__ uint64_t operator()(float x) const {   // (no branches: lanes differ)
     const double t = fmax(((double)x - (double)mx) * k2, -1200.0), n = rint(t), f = (t - n) * 0.69314718055994530942;
-    double p = 1.0 / 479001600.0;
-    p = __fma_rn(p, f, 1.0 / 39916800.0); p = __fma_rn(p, f, 1.0 / 3628800.0); p = __fma_rn(p, f, 1.0 / 362880.0);
-    p = __fma_rn(p, f, 1.0 / 40320.0); p = __fma_rn(p, f, 1.0 / 5040.0); p = __fma_rn(p, f, 1.0 / 720.0); p = __fma_rn(p, f, 1.0 / 120.0);
-    p = __fma_rn(p, f, 1.0 / 24.0); p = __fma_rn(p, f, 1.0 / 6.0); p = __fma_rn(p, f, 0.5); p = __fma_rn(p, f, 1.0); p = __fma_rn(p, f, 1.0);
-    return (uint64_t)__double_as_longlong(ldexp(p, (int)n + shift) + 4503599627370496.0) & 0xfffffffffffffull;
+    double p = 1.0 / 39916800.0;
+    p = __fma_rn(p, f, 1.0 / 3628800.0); p = __fma_rn(p, f, 1.0 / 362880.0); p = __fma_rn(p, f, 1.0 / 40320.0);
+    p = __fma_rn(p, f, 1.0 / 5040.0); p = __fma_rn(p, f, 1.0 / 720.0); p = __fma_rn(p, f, 1.0 / 120.0); p = __fma_rn(p, f, 1.0 / 24.0);
+    p = __fma_rn(p, f, 1.0 / 6.0); p = __fma_rn(p, f, 0.5); p = __fma_rn(p, f, 1.0); p = __fma_rn(p, f, 1.0);
+    const uint64_t w = (uint64_t)__double_as_longlong(ldexp(p, (int)n + shift) + 4503599627370496.0) & 0xfffffffffffffull;
+    return x == mx ? 1ull << shift : x == -INFINITY || mx == INFINITY ? 0ull : w;
   }
 };
 
 // ---- block sums -------------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor((unsigned long long)v, d);
+// running sum over the lanes on the DPP path (row shifts, then the two row broadcasts): no trip through the LDS crossbar
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp0(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp0(uint64_t v) { return (uint64_t)dpp0<CTRL, ROWS>((uint32_t)v) | ((uint64_t)dpp0<CTRL, ROWS>((uint32_t)(v >> 32)) << 32); }
+template <typename T>
+__device__ __forceinline__ T row_upto(T v) {   // within 16 lanes
+  v += dpp0<0x111, 0xf>(v); v += dpp0<0x112, 0xf>(v); v += dpp0<0x114, 0xf>(v); v += dpp0<0x118, 0xf>(v);
   return v;
 }
-__device__ __forceinline__ uint32_t wave_sum32(uint32_t v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+template <typename T>
+__device__ __forceinline__ T wave_upto(T v) {
+  v = row_upto(v);
+  v += dpp0<0x142, 0xa>(v); v += dpp0<0x143, 0xc>(v);
   return v;
 }
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) { return (uint64_t)lane_value((uint32_t)v, lane) | ((uint64_t)lane_value((uint32_t)(v >> 32), lane) << 32); }
+template <typename T>
+__device__ __forceinline__ T wave_total(T v) { return lane_value(wave_upto(v), 63); }
 struct Red { uint64_t m[2][16]; uint32_t c[2][16]; };   // two generations: one barrier per sum
 
-template <int NT>
 struct Block {
   Red* r;
   int gen = 0;
-  __device__ __forceinline__ void sum(uint32_t& cnt, uint64_t& mass, bool want_mass) {
-    cnt = wave_sum32(cnt);
-    if (want_mass) mass = wave_sum64(mass);
-    const int g = gen ^= 1;
-    if ((threadIdx.x & 63) == 0) { r->c[g][threadIdx.x >> 6] = cnt; r->m[g][threadIdx.x >> 6] = mass; }
+  // totals over the 16 waves: cnt is already the wave's, mass is per lane
+  template <bool MASS>
+  __device__ __forceinline__ void sum(uint32_t& cnt, uint64_t& mass) {
+    if (MASS) mass = wave_total(mass);
+    const int g = gen ^= 1, lane = threadIdx.x & 63;
+    if (lane == 0) { r->c[g][threadIdx.x >> 6] = cnt; if (MASS) r->m[g][threadIdx.x >> 6] = mass; }
     __syncthreads();
-    cnt = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i) cnt += r->c[g][i];
-    if (want_mass) {
-      mass = 0;
-#pragma unroll
-      for (int i = 0; i < NT / 64; ++i) mass += r->m[g][i];
-    }
+    cnt = lane_value(row_upto(r->c[g][lane & 15]), 15);
+    if (MASS) mass = lane_value(row_upto(r->m[g][lane & 15]), 15);
+  }
+  __device__ __forceinline__ uint32_t count(uint32_t wave_cnt) {
+    uint64_t none = 0;
+    sum<false>(wave_cnt, none);
+    return wave_cnt;
   }
   // sum over the threads before this one, and over all
   __device__ __forceinline__ uint64_t before(uint64_t v, uint64_t& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint64_t y = __shfl_up((unsigned long long)x, d);
-      if (lane >= d) x += y;
-    }
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint64_t x = wave_upto(v);
     const int g = gen ^= 1;
     if (lane == 63) r->m[g][wave] = x;
     __syncthreads();
-    uint64_t b = 0;
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i) {
-      if (i < wave) b += r->m[g][i];
-      total += r->m[g][i];
-    }
-    return b + x - v;
+    const uint64_t w = row_upto(r->m[g][lane & 15]);
+    total = lane_value(w, 15);
+    return (wave ? lane_value(w, wave - 1) : 0) + x - v;
   }
 };
 
 // ---- the search ---------------------------------------------------------------------------------------------------------------------------
 struct Cut { uint32_t key; uint32_t ties; };   // kept: keys above `key`, and the first `ties` entries equal to it
-struct Few { uint64_t w[64]; uint32_t key[64]; int n; };
+struct Few { uint32_t key[64]; int n; };
+constexpr uint32_t FEW = 32;   // a search ends with at most so many entries: ranking one costs a wave about as much as a third of a step
 
 // Largest interval end `lo` whose entries at or above it reach the target -- a count (MASS false) or a mass -- narrowed to the exact entry.
 // At entry: everything in [lo, ...) reaches it, nothing at or above hi does (cnt_hi / mass_hi are what lies there).
-template <int NT, bool MASS, typename Src>
-__device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, const Weigh& weigh, uint32_t lo, uint32_t cnt_lo, uint32_t hi, uint32_t want_n, double want_m) {
+template <bool MASS, typename Src>
+__device__ __forceinline__ Cut find_cut(Src& src, Block& blk, Few* few, const Weigh& weigh, uint32_t lo, uint32_t cnt_lo, uint32_t hi, uint32_t want_n, double want_m) {
   uint32_t cnt_hi = 0;
   uint64_t mass_hi = 0;
-  for (int step = 0; cnt_lo - cnt_hi > 64 && hi - lo > 1; ++step) {
+  for (int step = 0; cnt_lo - cnt_hi > FEW && hi - lo > 1; ++step) {
     uint32_t mid = lo + (hi - lo) / 2;
     if (!(step & 1)) {
       const float v = 0.5f * key_value(lo) + 0.5f * key_value(hi - 1);
@@ -134,7 +141,7 @@ __device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, cons
     uint32_t cnt;
     uint64_t mass = 0;
     src.template stat<MASS>(mid, cnt, mass);
-    blk.sum(cnt, mass, MASS);
+    blk.sum<MASS>(cnt, mass);
     if (MASS ? (double)mass >= want_m : cnt >= want_n) { lo = mid; cnt_lo = cnt; }
     else { hi = mid; cnt_hi = cnt; mass_hi = mass; }
   }
@@ -149,20 +156,18 @@ __device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, cons
   __syncthreads();
   src.gather(lo, hi, few);
   __syncthreads();
-  // every wave ranks the (at most 64) entries itself
-  const int lane = threadIdx.x & 63, n = min(few->n, 64);
+  // every wave ranks the entries itself
+  const int lane = threadIdx.x & 63, n = __builtin_amdgcn_readfirstlane(min(few->n, 64));
   const uint32_t key = lane < n ? few->key[lane] : 0;
   const uint64_t w = lane < n && MASS ? weigh(key_value(key)) : 0;
-  if (MASS && threadIdx.x < 64) few->w[lane] = w;
-  if (MASS) __syncthreads();
   uint32_t rank = 0, above = 0;
   uint64_t before = mass_hi;
   for (int j = 0; j < n; ++j) {
-    const uint32_t kj = few->key[j];
+    const uint32_t kj = lane_value(key, j);
     const bool first = kj > key || (kj == key && j < lane);
     rank += first;
     above += kj > key;
-    if (MASS && first) before += few->w[j];
+    if (MASS) before += first ? lane_value(w, j) : 0ull;
   }
   const bool here = lane < n && (MASS ? (double)before < want_m && (double)(before + w) >= want_m : cnt_hi + rank == want_n - 1);
   const uint64_t at = __ballot(here);
@@ -174,26 +179,26 @@ __device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, cons
   return r;
 }
 
-// a row (or list) in registers: thread t holds entries t * per .. t * per + per - 1; key 0 = not (or no longer) an entry
+// a row (or list) in registers: thread t holds entries t * per .. t * per + per - 1; key 0, w 0 = not (or no longer) an entry
+template <int E>
 struct RegRow {
   uint32_t key[E];
   uint64_t w[E];
   int per;
   template <bool MASS>
-  __device__ __forceinline__ void stat(uint32_t c, uint32_t& cnt, uint64_t& mass) const {
+  __device__ __forceinline__ void stat(uint32_t c, uint32_t& cnt, uint64_t& mass) const {   // cnt: of the wave
     cnt = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (e < per) {
-        const bool in = key[e] >= c;
-        cnt += in;
-        if (MASS) mass += in ? w[e] : 0;
-      }
+    for (int e = 0; e < E; ++e) {
+      const bool in = key[e] >= c;
+      cnt += __popcll(__ballot(in));
+      if (MASS) mass += in ? w[e] : 0;
+    }
   }
   __device__ __forceinline__ void gather(uint32_t lo, uint32_t hi, Few* few) const {
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (e < per && key[e] >= lo && key[e] < hi) {
+      if (key[e] - lo < hi - lo) {
         const int at = atomicAdd(&few->n, 1);
         if (at < 64) few->key[at] = key[e];
       }
@@ -201,24 +206,25 @@ struct RegRow {
 };
 
 // drop what a cut does not keep
-template <int NT>
-__device__ __forceinline__ void apply(RegRow& r, Block<NT>& blk, const Cut& c) {
-  uint32_t mine = 0;
+template <int E>
+__device__ __forceinline__ void apply(RegRow<E>& r, Block& blk, const Cut& c) {
+  uint32_t mine = 0, wave_all = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e < r.per) mine += r.key[e] == c.key;
-  uint32_t all = mine;
-  uint64_t unused = 0;
-  blk.sum(all, unused, false);
-  uint64_t rank = 0, total;
-  if (all > c.ties) rank = blk.before(mine, total);
+  for (int e = 0; e < E; ++e) {
+    const bool eq = r.key[e] == c.key;
+    mine += eq;
+    wave_all += __popcll(__ballot(eq));
+  }
+  uint32_t rank = 0;
+  uint64_t total;
+  if (blk.count(wave_all) > c.ties) rank = (uint32_t)blk.before(mine, total);
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e < r.per) {
-      bool keep = r.key[e] >= c.key;
-      if (r.key[e] == c.key) keep = rank++ < c.ties;
-      if (!keep) { r.key[e] = 0; r.w[e] = 0; }
-    }
+  for (int e = 0; e < E; ++e) {
+    const bool eq = r.key[e] == c.key, keep = r.key[e] > c.key || (eq && rank < c.ties);
+    rank += eq;
+    r.key[e] = keep ? r.key[e] : 0;
+    r.w[e] = keep ? r.w[e] : 0;
+  }
 }
 
 struct Setting {
@@ -241,86 +247,81 @@ __device__ __forceinline__ Setting setting(const SampleOpArgs& a, int row) {
   if (s.u >= 1.f) s.u = 0.99999994f;
   return s;
 }
-__device__ __forceinline__ double target(float top_p, uint64_t base) { return fmax((double)top_p * (double)base, 1.0); }   // at least one entry
+__device__ __forceinline__ double target(float top_p, double base) { return fmax((double)top_p * base, 1.0); }   // at least one entry
 
 // filters and draw on entries in registers; returns the place (e, in the thread that owns it) or -1.  `base`: the mass that top_p refers to when
-// top-k is off (0: that of these entries).  `enough` comes back false when these entries cannot hold the nucleus.
-template <int NT>
-__device__ __forceinline__ int filter_and_draw(RegRow& r, Block<NT>& blk, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, uint64_t base, bool& enough) {
+// it is not that of these entries (< 0: it is).  `enough` comes back false when these entries cannot hold the nucleus.
+template <int E>
+__device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block& blk, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, double base, bool& enough) {
   enough = true;
   if (s.k && (uint32_t)s.k < n) {
-    apply(r, blk, find_cut<NT, false>(r, blk, few, weigh, key_min, n, key_max + 1, (uint32_t)s.k, 0.0));
+    apply(r, blk, find_cut<false>(r, blk, few, weigh, key_min, n, key_max + 1, (uint32_t)s.k, 0.0));
     n = (uint32_t)s.k;
   }
   if (s.top_p < 1.f) {
     uint32_t cnt = 0;
     uint64_t mass = 0;
-    r.stat<true>(1u, cnt, mass);
-    blk.sum(cnt, mass, true);
-    const double want = target(s.top_p, base ? base : mass);
+    r.template stat<true>(1u, cnt, mass);
+    blk.sum<true>(cnt, mass);
+    const double want = target(s.top_p, base < 0.0 ? (double)mass : base);
     if ((double)mass < want) { enough = false; return -1; }
-    apply(r, blk, find_cut<NT, true>(r, blk, few, weigh, key_min, n, key_max + 1, 0u, want));
+    apply(r, blk, find_cut<true>(r, blk, few, weigh, key_min, n, key_max + 1, 0u, want));
   }
   uint64_t mine = 0, total;
   const double least = (double)s.min_p * (double)(1ull << weigh.shift);
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e < r.per) {
-      if ((double)r.w[e] < least) r.w[e] = 0;
-      mine += r.w[e];
-    }
+  for (int e = 0; e < E; ++e) {
+    r.w[e] = (double)r.w[e] < least ? 0 : r.w[e];
+    mine += r.w[e];
+  }
   const uint64_t before = blk.before(mine, total);
   const double want = (double)s.u * (double)total;
-  if (!((double)before > want) && (double)(before + mine) > want) {
-    uint64_t run = before;
+  if ((double)before > want || !((double)(before + mine) > want)) return -1;
+  uint64_t run = before + mine;
+  int found = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (e < r.per) {
-        run += r.w[e];
-        if ((double)run > want) return e;
-      }
+  for (int e = E - 1; e >= 0; --e) {   // the first place whose running sum is past the target
+    found = (double)run > want && r.w[e] ? e : found;
+    run -= r.w[e];
   }
-  return -1;
+  return found;
 }
 
-template <int NT>
 __device__ __forceinline__ float block_max(float v, float* s) {
   v = wave_max(v);
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
-  float m = s[0];
-#pragma unroll
-  for (int i = 1; i < NT / 64; ++i) m = fmaxf(m, s[i]);
-  return m;
+  float m = s[threadIdx.x & 15];
+  m = fmaxf(m, dpp_all<0xB1>(m)); m = fmaxf(m, dpp_all<0x4E>(m)); m = fmaxf(m, dpp_all<0x141>(m)); m = fmaxf(m, dpp_all<0x140>(m));
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(m)));
 }
 
 // rows of at most NT * E entries
-template <int NT, typename XT>
+template <int E, typename XT>
 __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
   __shared__ Red red;
   __shared__ Few few;
-  __shared__ float mx_s[2][NT / 64];
+  __shared__ float mx_s[2][16];
   __shared__ int best;
   const int row = blockIdx.x, tid = threadIdx.x;
   const XT* x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
   const Setting s = setting(a, row);
-  Block<NT> blk{&red};
-  RegRow r;
+  Block blk{&red};
+  RegRow<E> r;
   r.per = (a.V + NT - 1) / NT;
-  const int first = tid * r.per;
+  const int first = tid * r.per, mine = min(r.per, a.V - first);   // (mine <= 0 behind the row's end)
   float v[E], mx = -INFINITY, mn = INFINITY;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e < r.per) v[e] = logit(x, min(first + e, a.V - 1));
+  for (int e = 0; e < E; ++e) v[e] = logit(x, min(first + e, a.V - 1));
   uint32_t n = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e < r.per) {
-      if (first + e >= a.V) v[e] = -INFINITY;
-      mx = fmaxf(mx, v[e]);
-      if (v[e] > -INFINITY) { mn = fminf(mn, v[e]); ++n; }
-    }
-  mx = block_max<NT>(mx, mx_s[0]);
+  for (int e = 0; e < E; ++e) {
+    v[e] = e < mine ? v[e] : -INFINITY;
+    mx = fmaxf(mx, v[e]);
+    mn = v[e] > -INFINITY ? fminf(mn, v[e]) : mn;
+    n += __popcll(__ballot(v[e] > -INFINITY));
+  }
+  mx = block_max(mx, mx_s[0]);
   if (mx == -INFINITY) {
     if (tid == 0) a.out[row] = -1;
     return;
@@ -328,29 +329,47 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
   if (s.k == 1) {   // the first entry of the order
     if (tid == 0) best = a.V;
     __syncthreads();
+    int at = a.V;
 #pragma unroll
-    for (int e = E - 1; e >= 0; --e)
-      if (e < r.per && v[e] == mx) atomicMin(&best, first + e);
+    for (int e = E - 1; e >= 0; --e) at = v[e] == mx ? first + e : at;
+    if (at < a.V) atomicMin(&best, at);
     __syncthreads();
     if (tid == 0) a.out[row] = best;
     return;
   }
-  mn = -block_max<NT>(-mn, mx_s[1]);
+  mn = -block_max(-mn, mx_s[1]);
   const Weigh weigh{mx, 1.4426950408889634074 / (double)s.T, a.shift};
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    r.key[e] = 0; r.w[e] = 0;
-    if (e < r.per && v[e] > -INFINITY) { r.key[e] = order_key(v[e]); r.w[e] = weigh(v[e]); }
+    r.key[e] = v[e] > -INFINITY ? order_key(v[e]) : 0;
+    r.w[e] = weigh(v[e]);
   }
-  uint64_t none = 0;
-  blk.sum(n, none, false);
+  n = blk.count(n);
   bool enough;
-  const int e = filter_and_draw<NT>(r, blk, &few, weigh, s, n, order_key(mn), order_key(mx), 0, enough);
+  const int e = filter_and_draw(r, blk, &few, weigh, s, n, order_key(mn), order_key(mx), -1.0, enough);
   if (e >= 0) a.out[row] = first + e;
 }
 
 // ---- long rows ------------------------------------------------------------------------------------------------------------------------------
-// A wave owns a run of consecutive entries (a multiple of 64 * VEC); lanes take VEC consecutive ones at a time, 16-byte loads where the row allows.
+template <typename XT>
+__device__ __forceinline__ void gather8(W8<XT>& r, const XT* x, int i, int V);   // x[i .. i + 7] one by one, -inf past the row's end
+template <>
+__device__ __forceinline__ void gather8<float>(W8<float>& r, const float* x, int i, int V) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = i + e < V ? x[min(i + e, V - 1)] : -INFINITY;
+    if (e < 4) r.a[e] = v; else r.b[e - 4] = v;
+  }
+}
+template <>
+__device__ __forceinline__ void gather8<bf16_t>(W8<bf16_t>& r, const bf16_t* x, int i, int V) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t lo = i + 2 * e < V ? x[min(i + 2 * e, V - 1)] : 0xff80u, hi = i + 2 * e + 1 < V ? x[min(i + 2 * e + 1, V - 1)] : 0xff80u;
+    r.r[e] = lo | (hi << 16);
+  }
+}
+// The row as it lies in memory, for the search that streams.  A wave owns a run of consecutive entries (a multiple of 64 * VEC).
 template <typename XT, bool ALIGNED>
 struct LongRow {
   static constexpr int VEC = 8;
@@ -359,21 +378,15 @@ struct LongRow {
   const Weigh* weigh;
   uint32_t floor_key;   // entries below are not counted
   template <typename F>
-  __device__ __forceinline__ void each(int from, int to, F f) const {   // f(index of the first, values): every lane of the wave takes part
+  __device__ __forceinline__ void each(int from, int to, F f) const {   // f(index, value, whether the index is in the run): every lane takes part
     const int lane = threadIdx.x & 63;
     for (int i0 = from; i0 < to; i0 += 64 * VEC) {
       const int i = i0 + lane * VEC;
-      float v[VEC];
-      if (ALIGNED && i + VEC <= V) {
-        W8<XT> w;
-        w.load(x + i);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) { const float y = w.get(e) + 0.f; v[e] = y != y ? -INFINITY : y; }
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = i + e < V ? logit(x, i + e) : -INFINITY;
-      }
-      f(i, v);
+      W8<XT> w;
+      if (ALIGNED && i + VEC <= V) w.load(x + i);
+      else gather8(w, x, i, V);
+#pragma unroll 2
+      for (int e = 0; e < VEC; ++e) { const float y = w.get(e) + 0.f; f(i + e, y != y ? -INFINITY : y, i + e < to); }
     }
   }
   __device__ __forceinline__ int begin() const { return min((int)(threadIdx.x >> 6) * seg, V); }
@@ -382,175 +395,300 @@ struct LongRow {
   __device__ __forceinline__ void stat(uint32_t c, uint32_t& cnt, uint64_t& mass) const {
     uint32_t n = 0;
     uint64_t m = 0;
-    each(begin(), end(), [&](int, const float (&v)[VEC]) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const uint32_t key = order_key(v[e]);
-        if (key >= c && key >= floor_key) { ++n; if (MASS) m += (*weigh)(v[e]); }
-      }
+    each(begin(), end(), [&](int, float v, bool) {
+      const uint32_t key = order_key(v);
+      const bool in = key >= c && key >= floor_key;
+      n += __popcll(__ballot(in));
+      if (MASS) { const uint64_t w = (*weigh)(v); m += in ? w : 0; }
     });
     cnt = n;
     mass = m;
   }
   __device__ __forceinline__ void gather(uint32_t lo, uint32_t hi, Few* few) const {
-    each(begin(), end(), [&](int, const float (&v)[VEC]) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const uint32_t key = order_key(v[e]);
-        if (key >= lo && key < hi && key >= floor_key) {
-          const int at = atomicAdd(&few->n, 1);
-          if (at < 64) few->key[at] = key;
-        }
+    each(begin(), end(), [&](int, float v, bool) {
+      const uint32_t key = order_key(v);
+      if (key >= lo && key < hi && key >= floor_key) {
+        const int at = atomicAdd(&few->n, 1);
+        if (at < 64) few->key[at] = key;
       }
     });
   }
 };
-struct ListLds { float x[LIST]; int32_t i[LIST]; };
 
-template <typename XT, bool ALIGNED>
-__global__ __launch_bounds__(1024) void sample_long_kernel(SampleOpArgs a) {
-  constexpr int NT = 1024;
-  extern __shared__ __attribute__((aligned(16))) char dyn[];
-  ListLds* list = reinterpret_cast<ListLds*>(dyn);
+// ---- launch 1 of a long row: the list's threshold, from samples spread over the row.  ~0 = no list
+template <typename XT>
+__global__ __launch_bounds__(NT) void sample_threshold_kernel(SampleOpArgs a) {
   __shared__ Red red;
   __shared__ Few few;
-  __shared__ float mx_s[2][NT / 64];
+  __shared__ float mx_s[2][16];
+  const int row = blockIdx.x, tid = threadIdx.x;
+  const XT* x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
+  const Setting s = setting(a, row);
+  uint32_t thr = ~0u;
+  if (s.k != 1 && (s.k || s.top_p < 1.f || s.min_p > 0.f)) {
+    constexpr int E = SAMPLES / NT;
+    Block blk{&red};
+    RegRow<E> r;
+    uint32_t n = 0;
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = logit(x, (int)((int64_t)(tid * E + e) * a.V / SAMPLES));
+    float mx = -INFINITY, mn = INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      r.key[e] = v[e] > -INFINITY ? order_key(v[e]) : 0;
+      n += __popcll(__ballot(v[e] > -INFINITY));
+      mx = fmaxf(mx, v[e]);
+      mn = v[e] > -INFINITY ? fminf(mn, v[e]) : mn;
+    }
+    mx = block_max(mx, mx_s[0]);
+    mn = -block_max(-mn, mx_s[1]);
+    n = blk.count(n);
+    const int aim = s.k && s.k < AIM / 4 - 512 ? 4 * s.k + 2048 : AIM;   // a short top-k needs a short list
+    const uint32_t rank = max(1u, (uint32_t)((int64_t)aim * SAMPLES / a.V));
+    thr = NEG_INF_KEY + 1;
+    if (n > rank) thr = find_cut<false>(r, blk, &few, Weigh{}, order_key(mn), n, order_key(mx) + 1, rank, 0.0).key;
+  }
+  if (tid == 0) a.thr[row] = thr;
+}
+
+// ---- launch 2: a workgroup per chunk.  A thread owns 32 consecutive entries.
+template <typename XT, bool ALIGNED>
+__global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
+  constexpr int PER = CHUNK / 256;
+  __shared__ float mx_s[4];
+  __shared__ double mass_s[4];
+  __shared__ uint32_t cnt_s[4];
+  __shared__ int at_s;
+  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const XT* x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
+  const Setting s = setting(a, row);
+  const int i0 = chunk * CHUNK + tid * PER;
+  W8<XT> raw[PER / 8];
+  if (ALIGNED && i0 + PER <= a.V) {
+#pragma unroll
+    for (int j = 0; j < PER / 8; ++j) raw[j].load(x + i0 + 8 * j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER / 8; ++j) gather8(raw[j], x, i0 + 8 * j, a.V);
+  }
+  if (tid == 0) at_s = a.V;
+  auto value = [&](int j, int e) { const float v = raw[j].get(e) + 0.f; return v != v ? -INFINITY : v; };
+  float mx = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < PER / 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, value(j, e));
+  const float my_mx = mx;
+  mx = wave_max(mx);
+  if (lane == 0) mx_s[wave] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(mx_s[0], mx_s[1]), fmaxf(mx_s[2], mx_s[3]));
+  if (my_mx == mx) {
+    int at = a.V;
+#pragma unroll
+    for (int j = PER / 8 - 1; j >= 0; --j)
+#pragma unroll
+      for (int e = 7; e >= 0; --e) at = value(j, e) == mx ? i0 + 8 * j + e : at;
+    atomicMin(&at_s, at);
+  }
+  const uint32_t thr = a.thr[row];
+  uint32_t mine = 0;
+#pragma unroll
+  for (int j = 0; j < PER / 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mine += order_key(value(j, e)) >= thr;
+  const uint32_t upto = wave_upto(mine);
+  // the chunk's mass where it counts: no top-k, and a nucleus or nothing at all to cut
+  double mass = 0.0;
+  if (!s.k && (s.top_p < 1.f || s.min_p == 0.f) && mx > -INFINITY) {
+    const Weigh weigh{mx, 1.4426950408889634074 / (double)s.T, 51};
+    uint64_t m = 0;
+    W8<XT> left[PER / 8];
+#pragma unroll
+    for (int j = 0; j < PER / 8; ++j) left[j] = raw[j];
+#pragma unroll 1
+    for (int turn = 0; turn < PER / 8; ++turn) {   // (rolled: code that runs once is paid for by its size)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { const float v = left[0].get(e) + 0.f; m += weigh(v != v ? -INFINITY : v); }
+#pragma unroll
+      for (int j = 0; j + 1 < PER / 8; ++j) left[j] = left[j + 1];
+    }
+    m = wave_total(m);      // 64 * 32 weights of at most 2^51
+    mass = (double)m * 0x1p-51;
+  }
+  if (lane == 63) { cnt_s[wave] = upto; mass_s[wave] = mass; }
+  __syncthreads();
+  uint32_t before = 0;
+  for (int w = 0; w < wave; ++w) before += cnt_s[w];
+  if (tid == 0) {
+    ChunkHead h;
+    h.mass = (mass_s[0] + mass_s[1]) + (mass_s[2] + mass_s[3]);
+    h.mx = mx; h.at = at_s; h.count = cnt_s[0] + cnt_s[1] + cnt_s[2] + cnt_s[3]; h.pad = 0;
+    a.heads[(int64_t)row * a.chunks + chunk] = h;
+  }
+  if (mine) {
+    uint32_t p = before + upto - mine;
+    uint2* list = a.lists + ((int64_t)row * a.chunks + chunk) * CHUNK_CAP;
+#pragma unroll
+    for (int j = 0; j < PER / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t key = order_key(value(j, e));
+        if (key >= thr) { if (p < CHUNK_CAP) list[p] = make_uint2(key, (uint32_t)(i0 + 8 * j + e)); ++p; }
+      }
+  }
+}
+
+// ---- launch 3: a workgroup per row
+template <typename XT, bool ALIGNED>
+__global__ __launch_bounds__(NT) void sample_list_kernel(SampleOpArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t keys[];   // [LIST]
+  __shared__ Red red;
+  __shared__ Few few;
+  __shared__ float mx_s[16];
   __shared__ int best;
-  __shared__ uint32_t cnt_s[NT / 64], tie_s[NT / 64];
-  __shared__ uint64_t mass_s[NT / 64];
+  __shared__ uint32_t start_s[MAX_CHUNKS], tie_s[16];
+  __shared__ uint64_t mass_s[16];
+  __shared__ double cum_s[MAX_CHUNKS];
+  constexpr int E = LIST / NT;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Setting s = setting(a, row);
-  Block<NT> blk{&red};
-  LongRow<XT, ALIGNED> src;
-  constexpr int VEC = LongRow<XT, ALIGNED>::VEC;
-  src.x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
-  src.V = a.V;
-  src.seg = (a.V + NT * VEC - 1) / (NT * VEC) * (64 * VEC);
-  src.floor_key = NEG_INF_KEY + 1;
-  const int from = src.begin(), to = src.end();
-
-  float mx = -INFINITY, mn = INFINITY;
-  src.each(from, to, [&](int, const float (&v)[VEC]) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) { mx = fmaxf(mx, v[e]); mn = v[e] > -INFINITY ? fminf(mn, v[e]) : mn; }
-  });
-  mx = block_max<NT>(mx, mx_s[0]);
+  const uint32_t thr = a.thr[row];
+  Block blk{&red};
+  const ChunkHead* heads = a.heads + (int64_t)row * a.chunks;
+  ChunkHead h{0.0, -INFINITY, a.V, 0u, 0u};
+  if (tid < a.chunks) h = heads[tid];
+  if (tid == 0) best = a.V;
+  const float mx = block_max(h.mx, mx_s);
   if (mx == -INFINITY) {
     if (tid == 0) a.out[row] = -1;
     return;
   }
   if (s.k == 1) {
-    if (tid == 0) best = a.V;
-    __syncthreads();
-    src.each(from, to, [&](int i, const float (&v)[VEC]) {
-#pragma unroll
-      for (int e = VEC - 1; e >= 0; --e)
-        if (v[e] == mx) atomicMin(&best, i + e);
-    });
+    if (tid < a.chunks && h.mx == mx) atomicMin(&best, h.at);
     __syncthreads();
     if (tid == 0) a.out[row] = best;
     return;
   }
-  mn = -block_max<NT>(-mn, mx_s[1]);
-  const Weigh weigh{mx, 1.4426950408889634074 / (double)s.T, a.shift};
+  const double k2 = 1.4426950408889634074 / (double)s.T;
+  const Weigh weigh{mx, k2, a.shift};
+  // masses of the chunks in one scale, summed in their order by one thread: the same bits every time
+  if (tid < a.chunks) cum_s[tid] = h.mx == mx ? h.mass : h.mx == -INFINITY || mx == INFINITY ? 0.0 : h.mass * exp2(fmax(((double)h.mx - (double)mx) * k2, -1200.0));
+  uint64_t n_list;
+  const uint64_t start = blk.before(tid < a.chunks ? h.count : 0, n_list);
+  if (tid < a.chunks) start_s[tid] = (uint32_t)start;
+  const uint32_t crowded = blk.count(__popcll(__ballot(h.count > CHUNK_CAP)));
+  if (tid == 0) {
+    double c = 0.0;
+    for (int i = 0; i < a.chunks; ++i) { c += cum_s[i]; cum_s[i] = c; }
+  }
+  __syncthreads();
+  const double all = cum_s[a.chunks - 1];
+  const uint32_t key_max = order_key(mx);
+
+  LongRow<XT, ALIGNED> src;
+  constexpr int VEC = LongRow<XT, ALIGNED>::VEC;
+  src.x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
+  src.V = a.V;
+  src.seg = (a.V + NT * VEC - 1) / (NT * VEC) * (64 * VEC);
   src.weigh = &weigh;
-  const uint32_t key_min = order_key(mn), key_max = order_key(mx);
-  const bool filtered = s.k || s.top_p < 1.f;
-  Cut cut{0u, 0u};      // what the streaming draw keeps
-  uint32_t n = 0;
-  if (filtered) {
-    // threshold of the list, from samples spread over the row
-    RegRow r;
-    uint32_t ns = 0;
-    r.per = SAMPLES / NT;
+  src.floor_key = NEG_INF_KEY + 1;
+
+  if (!s.k && s.top_p >= 1.f && s.min_p == 0.f) {   // nothing is cut: the chunk that holds u * total, then its entries
+    const double want = (double)s.u * all;
+    int c = 0;
+    while (c < a.chunks - 1 && !(cum_s[c] > want)) ++c;
+    const double rest = (want - (c ? cum_s[c - 1] : 0.0)) * (double)(1ull << a.shift);
+    constexpr int PER = CHUNK / NT;
+    const int i0 = c * CHUNK + tid * PER;
+    uint64_t w[PER], mine = 0, total;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      w[e] = i0 + e < a.V ? weigh(logit(src.x, min(i0 + e, a.V - 1))) : 0;
+      mine += w[e];
+    }
+    const uint64_t before = blk.before(mine, total);
+    uint64_t run = before;
+    int at = a.V, last = -1;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      run += w[e];
+      if (w[e] && (double)run > rest && at == a.V) at = i0 + e;
+      if (w[e]) last = i0 + e;
+    }
+    if (at < a.V) atomicMin(&best, at);
+    __syncthreads();
+    const bool none = best == a.V;      // (rounding left the target past the chunk's last entry)
+    __syncthreads();
+    if (none) {
+      if (tid == 0) best = -1;
+      __syncthreads();
+      atomicMax(&best, last >= 0 ? last : -1);
+      __syncthreads();
+      if (tid == 0 && best < 0) best = heads[c].at;
+      __syncthreads();
+    }
+    if (tid == 0) a.out[row] = best;
+    return;
+  }
+
+  bool ok = !crowded && n_list > 0 && n_list <= LIST;
+  if (ok && s.k) ok = n_list >= (uint64_t)s.k || thr <= NEG_INF_KEY + 1;
+  if (ok && !s.k && s.top_p >= 1.f) ok = thr <= NEG_INF_KEY + 1 || (double)weigh(key_value(thr)) < (double)s.min_p * (double)(1ull << a.shift);   // min-p alone: all it keeps is listed
+  if (ok) {
+    const uint2* lists = a.lists + (int64_t)row * a.chunks * CHUNK_CAP;
+    for (int c = wave; c < a.chunks; c += 16) {
+      const uint32_t at = start_s[c], cnt = (c + 1 < a.chunks ? start_s[c + 1] : (uint32_t)n_list) - at;
+      for (uint32_t i = lane; i < cnt; i += 64) keys[at + i] = lists[(int64_t)c * CHUNK_CAP + i].x;
+    }
+    __syncthreads();
+    RegRow<E> r;
+    const uint32_t n = (uint32_t)n_list;
+    r.per = (int)((n + NT - 1) / NT);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      r.key[e] = 0; r.w[e] = 0;
-      if (e < SAMPLES / NT) {
-        const float v = logit(src.x, (int)((int64_t)(tid * (SAMPLES / NT) + e) * a.V / SAMPLES));
-        if (v > -INFINITY) { r.key[e] = order_key(v); ++ns; }
-      }
+      const uint32_t p = tid * r.per + e;
+      r.key[e] = e < r.per && p < n ? keys[min(p, (uint32_t)LIST - 1)] : 0;
+      r.w[e] = 0;
     }
-    uint64_t none = 0;
-    blk.sum(ns, none, false);
-    uint32_t thr = key_min;
-    const uint32_t rank = max(1u, (uint32_t)((int64_t)AIM * SAMPLES / a.V));
-    if (ns > rank) thr = find_cut<NT, false>(r, blk, &few, weigh, NEG_INF_KEY + 1, ns, key_max + 1, rank, 0.0).key;
-    // count what the list would take; the whole row's mass where top-p refers to it
-    const bool want_mass = s.top_p < 1.f && !s.k;
-    uint32_t take = 0, more = 0, all = 0;
-    uint64_t base = 0;
-    src.each(from, to, [&](int, const float (&v)[VEC]) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const uint32_t key = order_key(v[e]);
-        take += key >= thr && key > NEG_INF_KEY;
-        more += key > thr;
-        all += key > NEG_INF_KEY;
-        if (want_mass) base += weigh(v[e]);
-      }
-    });
-    uint32_t total_take = take, total_more = more;
-    n = all;
-    blk.sum(n, base, want_mass);
-    blk.sum(total_take, none, false);
-    blk.sum(total_more, none, false);
-    if (total_take > LIST) { ++thr; take = more; total_take = total_more; }   // (a crowd of equals at the threshold stays out)
-    const bool list_ok = total_take <= LIST && (s.k == 0 || (uint32_t)s.k <= total_take || total_take == n);
-    bool enough = false;
-    if (list_ok && total_take) {
-      const uint32_t wave_take = wave_sum32(take);
-      if (lane == 0) cnt_s[wave] = wave_take;
-      __syncthreads();
-      uint32_t at = 0;
-      for (int w = 0; w < wave; ++w) at += cnt_s[w];
-      src.each(from, to, [&](int i, const float (&v)[VEC]) {
-        uint32_t mine = 0;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) { const uint32_t key = order_key(v[e]); mine += key >= thr && key > NEG_INF_KEY; }
-        uint32_t upto = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const uint32_t y = __shfl_up(upto, d);
-          if (lane >= d) upto += y;
-        }
-        uint32_t p = at + upto - mine;
-        at += __builtin_amdgcn_readlane(upto, 63);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const uint32_t key = order_key(v[e]);
-          if (key >= thr && key > NEG_INF_KEY) { list->x[p] = v[e]; list->i[p] = i + e; ++p; }
-        }
-      });
-      __syncthreads();
-      r.per = (int)((total_take + NT - 1) / NT);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        r.key[e] = 0; r.w[e] = 0;
-        const uint32_t p = tid * r.per + e;
-        if (e < r.per && p < total_take) { const float v = list->x[p]; r.key[e] = order_key(v); r.w[e] = weigh(v); }
-      }
-      const int e = filter_and_draw<NT>(r, blk, &few, weigh, s, total_take, thr > key_min ? thr : key_min, key_max, s.k ? 0 : base, enough);
-      if (e >= 0) a.out[row] = list->i[tid * r.per + e];
+    for (int e = 0; e < E; ++e)
+      if (e < r.per) r.w[e] = r.key[e] ? weigh(key_value(r.key[e])) : 0;
+    bool enough;
+    const int e = filter_and_draw(r, blk, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << a.shift), enough);
+    if (e >= 0) {
+      const uint32_t p = tid * r.per + e;
+      int c = 0;
+      while (c + 1 < a.chunks && start_s[c + 1] <= p) ++c;
+      a.out[row] = (int)lists[(int64_t)c * CHUNK_CAP + (p - start_s[c])].y;
     }
     if (enough) return;
-    // the list does not hold the answer: the same search over the row itself
-    if (s.k && (uint32_t)s.k < n) cut = find_cut<NT, false>(src, blk, &few, weigh, key_min, n, key_max + 1, (uint32_t)s.k, 0.0);
-    if (s.top_p < 1.f) {
-      uint32_t cnt;
-      uint64_t above;
-      src.template stat<true>(cut.key + 1, cnt, above);
-      blk.sum(cnt, above, true);
-      const uint64_t each = cut.ties ? weigh(key_value(cut.key)) : 0;
-      const double want = target(s.top_p, above + each * cut.ties);
-      if ((double)above >= want) {
-        src.floor_key = max(src.floor_key, cut.key + 1);
-        cut = find_cut<NT, true>(src, blk, &few, weigh, max(key_min, src.floor_key), cnt, key_max + 1, 0u, want);
-        src.floor_key = NEG_INF_KEY + 1;
-      } else {
-        const double q = each ? ceil((want - (double)above) / (double)each) : 1.0;
-        if (q < (double)cut.ties) cut.ties = q < 1.0 ? 1u : (uint32_t)q;
-      }
+  }
+
+  // the list does not hold the answer: the same search over the row itself
+  Cut cut{0u, 0u};
+  {
+    uint32_t n;
+    uint64_t none = 0;
+    src.template stat<false>(NEG_INF_KEY + 1, n, none);
+    n = blk.count(n);
+    if (s.k && (uint32_t)s.k < n) cut = find_cut<false>(src, blk, &few, weigh, NEG_INF_KEY + 1, n, key_max + 1, (uint32_t)s.k, 0.0);
+  }
+  if (s.top_p < 1.f) {
+    uint32_t cnt;
+    uint64_t above = 0;
+    src.template stat<true>(cut.key + 1, cnt, above);
+    blk.sum<true>(cnt, above);
+    const uint64_t each = cut.ties ? weigh(key_value(cut.key)) : 0;
+    const double want = target(s.top_p, (double)(above + each * cut.ties));
+    if ((double)above >= want) {
+      src.floor_key = max(src.floor_key, cut.key + 1);
+      cut = find_cut<true>(src, blk, &few, weigh, src.floor_key, cnt, key_max + 1, 0u, want);
+      src.floor_key = NEG_INF_KEY + 1;
+    } else {
+      const double q = each ? ceil((want - (double)above) / (double)each) : 1.0;
+      if (q < (double)cut.ties) cut.ties = q < 1.0 ? 1u : (uint32_t)q;
     }
   }
   // draw by streaming: mass and ties of every wave's run, then the one run that holds the target
@@ -558,22 +696,20 @@ __global__ __launch_bounds__(1024) void sample_long_kernel(SampleOpArgs a) {
   auto value = [&](float v) { const uint64_t w = weigh(v); return (double)w < least ? 0ull : w; };
   uint64_t mass = 0;
   uint32_t ties = 0;
-  src.each(from, to, [&](int, const float (&v)[VEC]) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const uint32_t key = order_key(v[e]);
-      if (key > cut.key && key > NEG_INF_KEY) mass += value(v[e]);
-      ties += key == cut.key;
-    }
+  src.each(src.begin(), src.end(), [&](int, float v, bool) {
+    const uint32_t key = order_key(v);
+    const uint64_t w = value(v);
+    mass += key > cut.key && key > NEG_INF_KEY ? w : 0;
+    ties += key == cut.key;
   });
-  mass = wave_sum64(mass);
-  ties = wave_sum32(ties);
+  mass = wave_total(mass);
+  ties = wave_total(ties);
   const uint64_t each = cut.ties ? value(key_value(cut.key)) : 0;
   if (lane == 0) { mass_s[wave] = mass; tie_s[wave] = ties; }
   __syncthreads();
   uint64_t total = 0, run_before = 0;
   uint32_t tie_before = 0;
-  for (int w = 0; w < NT / 64; ++w) {
+  for (int w = 0; w < 16; ++w) {
     const uint32_t t = min(tie_s[w], cut.ties - min(cut.ties, tie_before));
     total += mass_s[w] + t * each;
     tie_before += tie_s[w];
@@ -581,7 +717,7 @@ __global__ __launch_bounds__(1024) void sample_long_kernel(SampleOpArgs a) {
   const double want = (double)s.u * (double)total;
   int at = 0;
   tie_before = 0;
-  for (int w = 0; w < NT / 64; ++w) {
+  for (int w = 0; w < 16; ++w) {
     const uint32_t t = min(tie_s[w], cut.ties - min(cut.ties, tie_before));
     const uint64_t m = mass_s[w] + t * each;
     at = w;
@@ -614,18 +750,56 @@ __global__ __launch_bounds__(1024) void sample_long_kernel(SampleOpArgs a) {
   }
 }
 
-extern "C" int csm_ops_sample_filtered(const csm_ops_sample_t* p, void* stream) {
+static int check(const csm_ops_sample_t* p) {
   if (!p) return ops_fail(CSM_OPS_ERR_ARG, "null argument");
   if (p->x_dtype != CSM_OPS_F32 && p->x_dtype != CSM_OPS_BF16) return ops_fail(CSM_OPS_ERR_ARG, "unknown dtype %d", p->x_dtype);
   if (p->rows < 0 || p->V < 1) return ops_fail(CSM_OPS_ERR_ARG, "rows must not be negative and V must be positive");
-  if (p->V > (1 << 24)) return ops_fail(CSM_OPS_ERR_CAPACITY, "V = %d: at most 2^24", p->V);
+  if (p->V > MAX_V) return ops_fail(CSM_OPS_ERR_CAPACITY, "V = %d: at most 2^21", p->V);
+  if ((int64_t)p->rows * ((p->V + CHUNK - 1) / CHUNK) > 0x7fffffff) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
   if (!p->temperatures && !(p->temperature >= 0.f && p->temperature < INFINITY)) return ops_fail(CSM_OPS_ERR_ARG, "temperature must be finite and not negative");
   if (!p->topks && (p->topk < 0 || p->topk > p->V)) return ops_fail(CSM_OPS_ERR_ARG, "selected index k out of range");
   if (!p->top_ps && !(p->top_p > 0.f && p->top_p <= 1.f)) return ops_fail(CSM_OPS_ERR_ARG, "top_p must lie in (0, 1]");
   if (!p->min_ps && !(p->min_p >= 0.f && p->min_p <= 1.f)) return ops_fail(CSM_OPS_ERR_ARG, "min_p must lie in [0, 1]");
+  return 0;
+}
+static size_t workspace(const csm_ops_sample_t* p, SampleOpArgs& a) {   // heads | lists | thresholds
+  a.chunks = (p->V + CHUNK - 1) / CHUNK;
+  if (p->V <= LIST) return 0;
+  const size_t n = (size_t)p->rows * a.chunks;
+  char* base = reinterpret_cast<char*>(p->workspace);
+  a.heads = reinterpret_cast<ChunkHead*>(base);
+  a.lists = reinterpret_cast<uint2*>(base + n * sizeof(ChunkHead));
+  a.thr = reinterpret_cast<uint32_t*>(base + n * (sizeof(ChunkHead) + CHUNK_CAP * sizeof(uint2)));
+  return n * (sizeof(ChunkHead) + CHUNK_CAP * sizeof(uint2)) + (size_t)p->rows * 4;
+}
+
+extern "C" int csm_ops_sample_workspace(const csm_ops_sample_t* p, size_t* bytes) {
+  if (!bytes) return ops_fail(CSM_OPS_ERR_ARG, "null argument");
+  if (const int r = check(p)) return r;
+  SampleOpArgs a;
+  *bytes = workspace(p, a);
+  return 0;
+}
+
+template <typename XT, bool ALIGNED>
+static int launch_long(const SampleOpArgs& a, int rows, hipStream_t st) {
+  // the keys of a list and what stands beside them: 69 KB of the CU's 160
+  OPS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(sample_list_kernel<XT, ALIGNED>), hipFuncAttributeMaxDynamicSharedMemorySize, LIST * sizeof(uint32_t)));
+  hipLaunchKernelGGL((sample_threshold_kernel<XT>), dim3(rows), dim3(NT), 0, st, a);
+  hipLaunchKernelGGL((sample_chunk_kernel<XT, ALIGNED>), dim3((unsigned)rows * a.chunks), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((sample_list_kernel<XT, ALIGNED>), dim3(rows), dim3(NT), LIST * sizeof(uint32_t), st, a);
+  OPS_HIP(hipGetLastError());
+  return 0;
+}
+
+extern "C" int csm_ops_sample_filtered(const csm_ops_sample_t* p, void* stream) {
+  if (const int r = check(p)) return r;
   if (!p->rows) return 0;
   if (!p->logits || !p->uniform || !p->out) return ops_fail(CSM_OPS_ERR_ARG, "null pointer");
   SampleOpArgs a;
+  const size_t need = workspace(p, a);
+  if (need && (!p->workspace || p->workspace_bytes < need || !ops_aligned(p->workspace)))
+    return ops_fail(CSM_OPS_ERR_CAPACITY, "workspace of %zu bytes: %zu on 16 bytes are needed", p->workspace_bytes, need);
   a.logits = p->logits; a.stride = p->logits_stride; a.V = p->V; a.uniform = p->uniform; a.temperatures = p->temperatures;
   a.top_ps = p->top_ps; a.min_ps = p->min_ps; a.topks = p->topks; a.temperature = p->temperature; a.top_p = p->top_p; a.min_p = p->min_p;
   a.topk = p->topk; a.out = p->out;
@@ -635,19 +809,16 @@ extern "C" int csm_ops_sample_filtered(const csm_ops_sample_t* p, void* stream) 
   hipStream_t st = (hipStream_t)stream;
   const bool b = p->x_dtype == CSM_OPS_BF16;
   const dim3 grid(p->rows);
-  if (p->V <= 256 * E) {
-    if (b) hipLaunchKernelGGL((sample_short_kernel<256, bf16_t>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((sample_short_kernel<256, float>), grid, dim3(256), 0, st, a);
-  } else if (p->V <= 1024 * E) {
-    if (b) hipLaunchKernelGGL((sample_short_kernel<1024, bf16_t>), grid, dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((sample_short_kernel<1024, float>), grid, dim3(1024), 0, st, a);
+  if (p->V <= 4 * NT) {
+    if (b) hipLaunchKernelGGL((sample_short_kernel<4, bf16_t>), grid, dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((sample_short_kernel<4, float>), grid, dim3(NT), 0, st, a);
+  } else if (p->V <= LIST) {
+    if (b) hipLaunchKernelGGL((sample_short_kernel<16, bf16_t>), grid, dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((sample_short_kernel<16, float>), grid, dim3(NT), 0, st, a);
   } else {
     const bool al = ops_aligned(p->logits) && (p->rows == 1 || ops_stride16(p->logits_stride, p->x_dtype));
-    const void* f = b ? (al ? (const void*)sample_long_kernel<bf16_t, true> : (const void*)sample_long_kernel<bf16_t, false>)
-                      : (al ? (const void*)sample_long_kernel<float, true> : (const void*)sample_long_kernel<float, false>);
-    OPS_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, sizeof(ListLds)));
-    void* args[] = {&a};
-    OPS_HIP(hipLaunchKernel(f, grid, dim3(1024), args, sizeof(ListLds), st));
+    return b ? (al ? launch_long<bf16_t, true>(a, p->rows, st) : launch_long<bf16_t, false>(a, p->rows, st))
+             : (al ? launch_long<float, true>(a, p->rows, st) : launch_long<float, false>(a, p->rows, st));
   }
   OPS_HIP(hipGetLastError());
   return 0;

@@ -19,8 +19,8 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 OPS_LIB_PATH = os.path.join(_HERE, "libcsm_ops.so")
 OPS_ABI_VERSION = 1
-OPS_EXPORTS = ["csm_ops_paged_rope_append", "csm_ops_paged_attention_workspace", "csm_ops_paged_prefix_attention", "csm_ops_sample_filtered",
-               "csm_ops_last_error", "csm_ops_abi_version"]
+OPS_EXPORTS = ["csm_ops_paged_rope_append", "csm_ops_paged_attention_workspace", "csm_ops_paged_prefix_attention", "csm_ops_sample_workspace",
+               "csm_ops_sample_filtered", "csm_ops_last_error", "csm_ops_abi_version"]
 _DT = {torch.float32: 0, torch.bfloat16: 1}
 
 
@@ -48,7 +48,8 @@ class AttentionArgs(C.Structure):
 class SampleArgs(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("logits_stride", C.c_int64), ("x_dtype", C.c_int32), ("rows", C.c_int32), ("V", C.c_int32),
                 ("uniform", C.c_void_p), ("temperatures", C.c_void_p), ("top_ps", C.c_void_p), ("min_ps", C.c_void_p), ("topks", C.c_void_p),
-                ("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float), ("topk", C.c_int32), ("out", C.c_void_p)]
+                ("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float), ("topk", C.c_int32), ("out", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 _lib = None
@@ -69,6 +70,7 @@ def load_ops_library():
         lib.csm_ops_paged_rope_append.argtypes = [C.POINTER(RopeAppendArgs), C.c_void_p]
         lib.csm_ops_paged_attention_workspace.argtypes = [C.POINTER(AttentionArgs), C.POINTER(C.c_size_t)]
         lib.csm_ops_paged_prefix_attention.argtypes = [C.POINTER(AttentionArgs), C.c_void_p]
+        lib.csm_ops_sample_workspace.argtypes = [C.POINTER(SampleArgs), C.POINTER(C.c_size_t)]
         lib.csm_ops_sample_filtered.argtypes = [C.POINTER(SampleArgs), C.c_void_p]
         _lib = lib
     return _lib
@@ -229,7 +231,7 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, *, temperature:
     the fewest that reach `top_p` of their mass, of these the ones with at least `min_p` times the largest probability; the token is the first
     index at which the running sum of kept probability passes `uniform` times its total.  `temperature = 0` is the arg-max, the lowest index
     of equals, like `sample_topk`; exactly `topk` entries stay, so `topk = 1` is the arg-max too (`sample_topk` keeps every entry that ties with
-    the k-th).  Any V; a NaN logit counts as -inf; a row with nothing but -inf gives -1."""
+    the k-th).  V up to 2^21; a NaN logit counts as -inf; a row with nothing but -inf gives -1."""
     _on_device(logits, ("logits", logits), ("uniform", uniform))
     _need(logits.dim() >= 1 and logits.dtype in _DT, "logits must be a float32 or bfloat16 tensor [..., V]")
     V, lead = logits.shape[-1], logits.shape[:-1]
@@ -254,5 +256,11 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, *, temperature:
             setattr(a, one, int(value) if dtype is torch.int32 else float(value))
     out = torch.empty(rows, dtype=torch.int32, device=logits.device)
     a.logits, a.logits_stride, a.x_dtype, a.rows, a.V, a.out = lg.data_ptr(), lg.stride(0), _DT[lg.dtype], rows, V, out.data_ptr()
-    _call(load_ops_library().csm_ops_sample_filtered, a, logits.device)
+    lib = load_ops_library()
+    need = C.c_size_t()
+    _ck(lib, lib.csm_ops_sample_workspace(C.byref(a), C.byref(need)))
+    if need.value:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=logits.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
+    _call(lib.csm_ops_sample_filtered, a, logits.device)
     return out.view(*lead, 1)

@@ -99,8 +99,8 @@ int csm_ops_paged_prefix_attention(const csm_ops_attention_t* a, void* stream);
  * lowest index of equals.  NaN logits count as -inf; several +inf share the row equally; a row of nothing but -inf gives -1.  u outside
  * [0, 1) is clamped to it.  topk <= 0 or >= V, top_p >= 1, min_p <= 0 switch that filter off; the first entry is always kept.  The pointers
  * give one value per row and win over the scalars; NULL = the scalar for all rows.  Per-row values the kernel cannot use are read as the
- * nearest that it can (temperature < 0 or NaN: 0; top_p < 0 or NaN: 0; min_p > 1: 1, NaN: 0).  Sums run in 64-bit fixed point over weights
- * computed in fp64, so a result does not depend on the order of any addition. */
+ * nearest that it can (temperature < 0 or NaN: 0; top_p < 0 or NaN: 0; min_p > 1: 1, NaN: 0).  V up to 2^21.  Weights are
+ * computed in fp64 and summed in 64-bit fixed point, chunks of a long row in fp64 in their order: the same input gives the same token. */
 typedef struct {
   const void* logits;                 /* [rows][V] at logits_stride, any alignment */
   int64_t logits_stride;
@@ -111,7 +111,10 @@ typedef struct {
   float temperature, top_p, min_p;
   int32_t topk;
   int32_t* out;                       /* [rows] */
+  void* workspace;                    /* csm_ops_sample_workspace bytes (16 B; 0 up to V = 16 384), undefined before and after, one per call in flight */
+  size_t workspace_bytes;
 } csm_ops_sample_t;
+int csm_ops_sample_workspace(const csm_ops_sample_t* a, size_t* bytes_host);
 int csm_ops_sample_filtered(const csm_ops_sample_t* a, void* stream);
 
 const char* csm_ops_last_error(void);

@@ -89,7 +89,7 @@ def test_attention_refusals(over):
 
 
 @pytest.mark.parametrize("over", [
-    dict(x_dtype=2), dict(rows=-1), dict(V=0), dict(V=(1 << 24) + 1), dict(temperature=-0.5), dict(temperature=float("inf")), dict(temperature=float("nan")), dict(topk=-1), dict(topk=101),
+    dict(x_dtype=2), dict(rows=-1), dict(V=0), dict(V=(1 << 21) + 1), dict(temperature=-0.5), dict(temperature=float("inf")), dict(temperature=float("nan")), dict(topk=-1), dict(topk=101),
     dict(top_p=0.0), dict(top_p=1.5), dict(top_p=float("nan")), dict(min_p=-0.1), dict(min_p=1.01), dict(logits=None), dict(uniform=None), dict(out=None)])
 def test_sample_refusals(over):
     lib = ops.load_ops_library()
