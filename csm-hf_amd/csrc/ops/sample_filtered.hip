@@ -8,7 +8,8 @@
 // alternates between the middle VALUE, which a smooth row needs few of, and the middle KEY, which bounds any row) until at most 32 entries or
 // one single key are left, which a wave then ranks exactly.
 //   V <= 16 384: one workgroup, the row in registers (4 or 16 consecutive entries per thread), read once.  Such a launch is a chain of dependent
-//                steps over code that runs once, so its loops carry no branches and its sums stay on the DPP path.
+//                steps over code that runs once, so its loops carry no branches and its sums stay on the DPP path.  A top-k of at most 64 narrows
+//                the row to 64 entries at once, and one wave does the rest without a barrier.
 //   larger V:    three launches, so that few rows still use many CUs: a threshold near the 12 288th largest from 4 096 samples; per chunk of
 //                8 192 entries its maximum, its mass and the entries above the threshold; per row the cuts and the draw on those entries.
 //                Where they are not enough (a flat row whose nucleus is larger), the same search streams over the row.
@@ -30,8 +31,7 @@ struct SampleOpArgs {
   struct ChunkHead* heads; // [rows][chunks]
   uint2* lists;            // [rows][chunks][CHUNK_CAP] (key, index)
 };
-constexpr int NT = 1024;                  // threads per row
-constexpr int LIST = NT * 16;             // entries that fit the registers of a workgroup
+constexpr int LIST = 1024 * 16;           // entries that fit the registers of a workgroup
 constexpr int SAMPLES = 4096, AIM = LIST * 3 / 4;   // the list's threshold is a sample's order statistic that aims at this many entries: at V = 131 072
                                                     // their number scatters by 613, LIST is 6.7 of that away
 constexpr int CHUNK = 8192, CHUNK_CAP = 2048, MAX_V = 1 << 21, MAX_CHUNKS = MAX_V / CHUNK;
@@ -72,6 +72,10 @@ template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t dpp0(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint64_t dpp0(uint64_t v) { return (uint64_t)dpp0<CTRL, ROWS>((uint32_t)v) | ((uint64_t)dpp0<CTRL, ROWS>((uint32_t)(v >> 32)) << 32); }
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_any(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_any(uint64_t v) { return (uint64_t)dpp_any<CTRL>((uint32_t)v) | ((uint64_t)dpp_any<CTRL>((uint32_t)(v >> 32)) << 32); }
 template <typename T>
 __device__ __forceinline__ T row_upto(T v) {   // within 16 lanes
   v += dpp0<0x111, 0xf>(v); v += dpp0<0x112, 0xf>(v); v += dpp0<0x114, 0xf>(v); v += dpp0<0x118, 0xf>(v);
@@ -89,18 +93,29 @@ template <typename T>
 __device__ __forceinline__ T wave_total(T v) { return lane_value(wave_upto(v), 63); }
 struct Red { uint64_t m[2][16]; uint32_t c[2][16]; };   // two generations: one barrier per sum
 
+// sum over the W (4 or 16) entries that the waves left in LDS, in every lane
+template <int W, typename T>
+__device__ __forceinline__ T over_waves(T v) {
+  v += dpp_any<0xB1>(v); v += dpp_any<0x4E>(v);
+  if (W > 4) { v += dpp_any<0x141>(v); v += dpp_any<0x140>(v); }
+  return v;
+}
+
+template <int NT>
 struct Block {
+  static constexpr int W = NT / 64;
+  static_assert(W == 4 || W == 16, "");
   Red* r;
   int gen = 0;
-  // totals over the 16 waves: cnt is already the wave's, mass is per lane
+  // totals over the waves: cnt is already the wave's, mass is per lane
   template <bool MASS>
   __device__ __forceinline__ void sum(uint32_t& cnt, uint64_t& mass) {
     if (MASS) mass = wave_total(mass);
     const int g = gen ^= 1, lane = threadIdx.x & 63;
     if (lane == 0) { r->c[g][threadIdx.x >> 6] = cnt; if (MASS) r->m[g][threadIdx.x >> 6] = mass; }
     __syncthreads();
-    cnt = lane_value(row_upto(r->c[g][lane & 15]), 15);
-    if (MASS) mass = lane_value(row_upto(r->m[g][lane & 15]), 15);
+    cnt = lane_value(over_waves<W>(r->c[g][lane % W]), 0);
+    if (MASS) mass = lane_value(over_waves<W>(r->m[g][lane % W]), 0);
   }
   __device__ __forceinline__ uint32_t count(uint32_t wave_cnt) {
     uint64_t none = 0;
@@ -108,15 +123,16 @@ struct Block {
     return wave_cnt;
   }
   // sum over the threads before this one, and over all
-  __device__ __forceinline__ uint64_t before(uint64_t v, uint64_t& total) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const uint64_t x = wave_upto(v);
+  template <typename T>
+  __device__ __forceinline__ T before(T v, T& total) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const T x = wave_upto(v);
     const int g = gen ^= 1;
     if (lane == 63) r->m[g][wave] = x;
     __syncthreads();
-    const uint64_t w = row_upto(r->m[g][lane & 15]);
-    total = lane_value(w, 15);
-    return (wave ? lane_value(w, wave - 1) : 0) + x - v;
+    const T w = (T)r->m[g][lane % W];
+    total = lane_value(over_waves<W>(w), 0);
+    return lane_value(over_waves<W>(lane % W < wave ? w : (T)0), 0) + x - v;
   }
 };
 
@@ -125,23 +141,24 @@ struct Cut { uint32_t key; uint32_t ties; };   // kept: keys above `key`, and th
 struct Few { uint32_t key[64]; int n; };
 constexpr uint32_t FEW = 32;   // a search ends with at most so many entries: ranking one costs a wave about as much as a third of a step
 
+__device__ __forceinline__ uint32_t probe(uint32_t lo, uint32_t hi, int step) {   // lo < probe < hi: the middle value and the middle key in turn
+  const float v = 0.5f * key_value(lo) + 0.5f * key_value(hi - 1);
+  const uint32_t kv = order_key(v + 0.f);
+  return !(step & 1) && v == v && kv > lo && kv < hi ? kv : lo + (hi - lo) / 2;
+}
+
 // Largest interval end `lo` whose entries at or above it reach the target -- a count (MASS false) or a mass -- narrowed to the exact entry.
 // At entry: everything in [lo, ...) reaches it, nothing at or above hi does (cnt_hi / mass_hi are what lies there).
-template <bool MASS, typename Src>
-__device__ __forceinline__ Cut find_cut(Src& src, Block& blk, Few* few, const Weigh& weigh, uint32_t lo, uint32_t cnt_lo, uint32_t hi, uint32_t want_n, double want_m) {
+template <bool MASS, int NT, typename Src>
+__device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, const Weigh& weigh, uint32_t lo, uint32_t cnt_lo, uint32_t hi, uint32_t want_n, double want_m) {
   uint32_t cnt_hi = 0;
   uint64_t mass_hi = 0;
   for (int step = 0; cnt_lo - cnt_hi > FEW && hi - lo > 1; ++step) {
-    uint32_t mid = lo + (hi - lo) / 2;
-    if (!(step & 1)) {
-      const float v = 0.5f * key_value(lo) + 0.5f * key_value(hi - 1);
-      const uint32_t kv = order_key(v + 0.f);
-      if (v == v && kv > lo && kv < hi) mid = kv;
-    }
+    const uint32_t mid = probe(lo, hi, step);
     uint32_t cnt;
     uint64_t mass = 0;
     src.template stat<MASS>(mid, cnt, mass);
-    blk.sum<MASS>(cnt, mass);
+    blk.template sum<MASS>(cnt, mass);
     if (MASS ? (double)mass >= want_m : cnt >= want_n) { lo = mid; cnt_lo = cnt; }
     else { hi = mid; cnt_hi = cnt; mass_hi = mass; }
   }
@@ -167,7 +184,7 @@ __device__ __forceinline__ Cut find_cut(Src& src, Block& blk, Few* few, const We
     const bool first = kj > key || (kj == key && j < lane);
     rank += first;
     above += kj > key;
-    if (MASS) before += first ? lane_value(w, j) : 0ull;
+    if (MASS) before += first ? lane_value(w, j) : (uint64_t)0;
   }
   const bool here = lane < n && (MASS ? (double)before < want_m && (double)(before + w) >= want_m : cnt_hi + rank == want_n - 1);
   const uint64_t at = __ballot(here);
@@ -206,8 +223,8 @@ struct RegRow {
 };
 
 // drop what a cut does not keep
-template <int E>
-__device__ __forceinline__ void apply(RegRow<E>& r, Block& blk, const Cut& c) {
+template <int E, int NT>
+__device__ __forceinline__ void apply(RegRow<E>& r, Block<NT>& blk, const Cut& c) {
   uint32_t mine = 0, wave_all = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -215,9 +232,8 @@ __device__ __forceinline__ void apply(RegRow<E>& r, Block& blk, const Cut& c) {
     mine += eq;
     wave_all += __popcll(__ballot(eq));
   }
-  uint32_t rank = 0;
-  uint64_t total;
-  if (blk.count(wave_all) > c.ties) rank = (uint32_t)blk.before(mine, total);
+  uint32_t rank = 0, total;
+  if (blk.count(wave_all) > c.ties) rank = blk.before(mine, total);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const bool eq = r.key[e] == c.key, keep = r.key[e] > c.key || (eq && rank < c.ties);
@@ -249,10 +265,75 @@ __device__ __forceinline__ Setting setting(const SampleOpArgs& a, int row) {
 }
 __device__ __forceinline__ double target(float top_p, double base) { return fmax((double)top_p * base, 1.0); }   // at least one entry
 
+// All filters and the draw on at most 64 entries in index order, by one wave: lane i holds entry i (key 0: none), the first `k` of the order
+// count.  Every lane adds up what precedes it in the order; the result is the entry's lane.
+__device__ __forceinline__ int draw_few(uint32_t key, int n, uint32_t k, const Weigh& weigh, const Setting& s) {
+  const int lane = threadIdx.x & 63;
+  const uint64_t w = key ? weigh(key_value(key)) : 0;
+  uint32_t rank = 0;
+  uint64_t before = 0;
+  for (int j = 0; j < n; ++j) {
+    const uint32_t kj = lane_value(key, j);
+    const bool first = kj > key || (kj == key && j < lane);
+    rank += first;
+    before += first ? lane_value(w, j) : (uint64_t)0;
+  }
+  bool keep = key && rank < k;
+  const double reach = target(s.top_p, (double)wave_total(keep ? w : (uint64_t)0));   // (every lane takes part)
+  keep = keep && (s.top_p >= 1.f || (double)before < reach);
+  keep = keep && (double)w >= (double)s.min_p * (double)(1ull << weigh.shift);
+  const uint64_t upto = wave_upto(keep ? w : (uint64_t)0);
+  const double want = (double)s.u * (double)lane_value(upto, 63);
+  return __ffsll((unsigned long long)__ballot(keep && (double)upto > want)) - 1;
+}
+
+// The short way for a small top-k: a threshold that leaves between k and 64 entries, these in index order to one wave.  -2: a crowd of equals
+// allows no such threshold.  Otherwise the place (e, in the thread that owns it) or -1.  Needs keys only.
+struct FewOrder { uint32_t key[64]; int hit; };
+template <int E, int NT>
+__device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, FewOrder* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t k, uint32_t key_min, uint32_t key_max) {
+  uint32_t lo = key_min, hi = key_max + 1, cnt_lo = n;
+  for (int step = 0; cnt_lo > 64 && hi - lo > 1; ++step) {
+    const uint32_t mid = probe(lo, hi, step);
+    uint32_t cnt;
+    uint64_t none = 0;
+    r.template stat<false>(mid, cnt, none);
+    cnt = blk.count(cnt);
+    if (cnt >= k) { lo = mid; cnt_lo = cnt; }
+    else hi = mid;
+  }
+  if (cnt_lo > 64) return -2;
+  uint32_t mine = 0, total;
+#pragma unroll
+  for (int e = 0; e < E; ++e) mine += r.key[e] >= lo;
+  const uint32_t first = blk.before(mine, total);
+  uint32_t p = first;
+  if (mine) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (r.key[e] >= lo) few->key[p++] = r.key[e];
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    const int hit = draw_few(lane < (int)cnt_lo ? few->key[lane] : 0u, (int)cnt_lo, k, weigh, s);
+    if (lane == 0) few->hit = hit;
+  }
+  __syncthreads();
+  const uint32_t hit = (uint32_t)few->hit;
+  if (hit - first >= mine) return -1;
+  int found = 0;
+  p = first + mine;
+#pragma unroll
+  for (int e = E - 1; e >= 0; --e)
+    if (r.key[e] >= lo) found = --p == hit ? e : found;
+  return found;
+}
+
 // filters and draw on entries in registers; returns the place (e, in the thread that owns it) or -1.  `base`: the mass that top_p refers to when
 // it is not that of these entries (< 0: it is).  `enough` comes back false when these entries cannot hold the nucleus.
-template <int E>
-__device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block& blk, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, double base, bool& enough) {
+template <int E, int NT>
+__device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block<NT>& blk, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, double base, bool& enough) {
   enough = true;
   if (s.k && (uint32_t)s.k < n) {
     apply(r, blk, find_cut<false>(r, blk, few, weigh, key_min, n, key_max + 1, (uint32_t)s.k, 0.0));
@@ -262,7 +343,7 @@ __device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block& blk, Few* fe
     uint32_t cnt = 0;
     uint64_t mass = 0;
     r.template stat<true>(1u, cnt, mass);
-    blk.sum<true>(cnt, mass);
+    blk.template sum<true>(cnt, mass);
     const double want = target(s.top_p, base < 0.0 ? (double)mass : base);
     if ((double)mass < want) { enough = false; return -1; }
     apply(r, blk, find_cut<true>(r, blk, few, weigh, key_min, n, key_max + 1, 0u, want));
@@ -287,26 +368,28 @@ __device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block& blk, Few* fe
   return found;
 }
 
+template <int NT>
 __device__ __forceinline__ float block_max(float v, float* s) {
   v = wave_max(v);
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
-  float m = s[threadIdx.x & 15];
+  float m = s[(threadIdx.x & 63) % (NT / 64)];
   m = fmaxf(m, dpp_all<0xB1>(m)); m = fmaxf(m, dpp_all<0x4E>(m)); m = fmaxf(m, dpp_all<0x141>(m)); m = fmaxf(m, dpp_all<0x140>(m));
   return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(m)));
 }
 
 // rows of at most NT * E entries
-template <int E, typename XT>
+template <int NT, int E, typename XT>
 __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
   __shared__ Red red;
   __shared__ Few few;
+  __shared__ FewOrder order;
   __shared__ float mx_s[2][16];
   __shared__ int best;
   const int row = blockIdx.x, tid = threadIdx.x;
   const XT* x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
   const Setting s = setting(a, row);
-  Block blk{&red};
+  Block<NT> blk{&red};
   RegRow<E> r;
   r.per = (a.V + NT - 1) / NT;
   const int first = tid * r.per, mine = min(r.per, a.V - first);   // (mine <= 0 behind the row's end)
@@ -321,7 +404,7 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
     mn = v[e] > -INFINITY ? fminf(mn, v[e]) : mn;
     n += __popcll(__ballot(v[e] > -INFINITY));
   }
-  mx = block_max(mx, mx_s[0]);
+  mx = block_max<NT>(mx, mx_s[0]);
   if (mx == -INFINITY) {
     if (tid == 0) a.out[row] = -1;
     return;
@@ -337,16 +420,20 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
     if (tid == 0) a.out[row] = best;
     return;
   }
-  mn = -block_max(-mn, mx_s[1]);
-  const Weigh weigh{mx, 1.4426950408889634074 / (double)s.T, a.shift};
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    r.key[e] = v[e] > -INFINITY ? order_key(v[e]) : 0;
-    r.w[e] = weigh(v[e]);
-  }
+  mn = -block_max<NT>(-mn, mx_s[1]);
   n = blk.count(n);
-  bool enough;
-  const int e = filter_and_draw(r, blk, &few, weigh, s, n, order_key(mn), order_key(mx), -1.0, enough);
+  const Weigh weigh{mx, 1.4426950408889634074 / (double)s.T, a.shift};
+  const uint32_t key_min = order_key(mn), key_max = order_key(mx), k = s.k && (uint32_t)s.k < n ? (uint32_t)s.k : n;
+#pragma unroll
+  for (int e = 0; e < E; ++e) r.key[e] = v[e] > -INFINITY ? order_key(v[e]) : 0;
+  int e = -2;
+  if (k <= 64) e = draw_small(r, blk, &order, weigh, s, n, k, key_min, key_max);
+  if (e == -2) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) r.w[i] = weigh(v[i]);
+    bool enough;
+    e = filter_and_draw(r, blk, &few, weigh, s, n, key_min, key_max, -1.0, enough);
+  }
   if (e >= 0) a.out[row] = first + e;
 }
 
@@ -417,7 +504,8 @@ struct LongRow {
 
 // ---- launch 1 of a long row: the list's threshold, from samples spread over the row.  ~0 = no list
 template <typename XT>
-__global__ __launch_bounds__(NT) void sample_threshold_kernel(SampleOpArgs a) {
+__global__ __launch_bounds__(256) void sample_threshold_kernel(SampleOpArgs a) {
+  constexpr int NT = 256;
   __shared__ Red red;
   __shared__ Few few;
   __shared__ float mx_s[2][16];
@@ -427,7 +515,7 @@ __global__ __launch_bounds__(NT) void sample_threshold_kernel(SampleOpArgs a) {
   uint32_t thr = ~0u;
   if (s.k != 1 && (s.k || s.top_p < 1.f || s.min_p > 0.f)) {
     constexpr int E = SAMPLES / NT;
-    Block blk{&red};
+    Block<NT> blk{&red};
     RegRow<E> r;
     uint32_t n = 0;
     float v[E];
@@ -441,8 +529,8 @@ __global__ __launch_bounds__(NT) void sample_threshold_kernel(SampleOpArgs a) {
       mx = fmaxf(mx, v[e]);
       mn = v[e] > -INFINITY ? fminf(mn, v[e]) : mn;
     }
-    mx = block_max(mx, mx_s[0]);
-    mn = -block_max(-mn, mx_s[1]);
+    mx = block_max<NT>(mx, mx_s[0]);
+    mn = -block_max<NT>(-mn, mx_s[1]);
     n = blk.count(n);
     const int aim = s.k && s.k < AIM / 4 - 512 ? 4 * s.k + 2048 : AIM;   // a short top-k needs a short list
     const uint32_t rank = max(1u, (uint32_t)((int64_t)aim * SAMPLES / a.V));
@@ -542,10 +630,12 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
 
 // ---- launch 3: a workgroup per row
 template <typename XT, bool ALIGNED>
-__global__ __launch_bounds__(NT) void sample_list_kernel(SampleOpArgs a) {
+__global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
+  constexpr int NT = 1024;
   extern __shared__ __attribute__((aligned(16))) uint32_t keys[];   // [LIST]
   __shared__ Red red;
   __shared__ Few few;
+  __shared__ FewOrder order;
   __shared__ float mx_s[16];
   __shared__ int best;
   __shared__ uint32_t start_s[MAX_CHUNKS], tie_s[16];
@@ -555,12 +645,12 @@ __global__ __launch_bounds__(NT) void sample_list_kernel(SampleOpArgs a) {
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Setting s = setting(a, row);
   const uint32_t thr = a.thr[row];
-  Block blk{&red};
+  Block<NT> blk{&red};
   const ChunkHead* heads = a.heads + (int64_t)row * a.chunks;
   ChunkHead h{0.0, -INFINITY, a.V, 0u, 0u};
   if (tid < a.chunks) h = heads[tid];
   if (tid == 0) best = a.V;
-  const float mx = block_max(h.mx, mx_s);
+  const float mx = block_max<NT>(h.mx, mx_s);
   if (mx == -INFINITY) {
     if (tid == 0) a.out[row] = -1;
     return;
@@ -576,7 +666,7 @@ __global__ __launch_bounds__(NT) void sample_list_kernel(SampleOpArgs a) {
   // masses of the chunks in one scale, summed in their order by one thread: the same bits every time
   if (tid < a.chunks) cum_s[tid] = h.mx == mx ? h.mass : h.mx == -INFINITY || mx == INFINITY ? 0.0 : h.mass * exp2(fmax(((double)h.mx - (double)mx) * k2, -1200.0));
   uint64_t n_list;
-  const uint64_t start = blk.before(tid < a.chunks ? h.count : 0, n_list);
+  const uint64_t start = blk.before((uint64_t)(tid < a.chunks ? h.count : 0), n_list);
   if (tid < a.chunks) start_s[tid] = (uint32_t)start;
   const uint32_t crowded = blk.count(__popcll(__ballot(h.count > CHUNK_CAP)));
   if (tid == 0) {
@@ -650,13 +740,15 @@ __global__ __launch_bounds__(NT) void sample_list_kernel(SampleOpArgs a) {
     for (int e = 0; e < E; ++e) {
       const uint32_t p = tid * r.per + e;
       r.key[e] = e < r.per && p < n ? keys[min(p, (uint32_t)LIST - 1)] : 0;
-      r.w[e] = 0;
     }
+    bool enough = true;
+    int e = -2;
+    if (s.k && s.k <= 64) e = draw_small(r, blk, &order, weigh, s, n, min((uint32_t)s.k, n), thr, key_max);
+    if (e == -2) {
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (e < r.per) r.w[e] = r.key[e] ? weigh(key_value(r.key[e])) : 0;
-    bool enough;
-    const int e = filter_and_draw(r, blk, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << a.shift), enough);
+      for (int i = 0; i < E; ++i) r.w[i] = r.key[i] ? weigh(key_value(r.key[i])) : 0;
+      e = filter_and_draw(r, blk, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << a.shift), enough);
+    }
     if (e >= 0) {
       const uint32_t p = tid * r.per + e;
       int c = 0;
@@ -679,7 +771,7 @@ __global__ __launch_bounds__(NT) void sample_list_kernel(SampleOpArgs a) {
     uint32_t cnt;
     uint64_t above = 0;
     src.template stat<true>(cut.key + 1, cnt, above);
-    blk.sum<true>(cnt, above);
+    blk.template sum<true>(cnt, above);
     const uint64_t each = cut.ties ? weigh(key_value(cut.key)) : 0;
     const double want = target(s.top_p, (double)(above + each * cut.ties));
     if ((double)above >= want) {
@@ -785,9 +877,9 @@ template <typename XT, bool ALIGNED>
 static int launch_long(const SampleOpArgs& a, int rows, hipStream_t st) {
   // the keys of a list and what stands beside them: 69 KB of the CU's 160
   OPS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(sample_list_kernel<XT, ALIGNED>), hipFuncAttributeMaxDynamicSharedMemorySize, LIST * sizeof(uint32_t)));
-  hipLaunchKernelGGL((sample_threshold_kernel<XT>), dim3(rows), dim3(NT), 0, st, a);
+  hipLaunchKernelGGL((sample_threshold_kernel<XT>), dim3(rows), dim3(256), 0, st, a);
   hipLaunchKernelGGL((sample_chunk_kernel<XT, ALIGNED>), dim3((unsigned)rows * a.chunks), dim3(256), 0, st, a);
-  hipLaunchKernelGGL((sample_list_kernel<XT, ALIGNED>), dim3(rows), dim3(NT), LIST * sizeof(uint32_t), st, a);
+  hipLaunchKernelGGL((sample_list_kernel<XT, ALIGNED>), dim3(rows), dim3(1024), LIST * sizeof(uint32_t), st, a);
   OPS_HIP(hipGetLastError());
   return 0;
 }
@@ -809,12 +901,16 @@ extern "C" int csm_ops_sample_filtered(const csm_ops_sample_t* p, void* stream) 
   hipStream_t st = (hipStream_t)stream;
   const bool b = p->x_dtype == CSM_OPS_BF16;
   const dim3 grid(p->rows);
-  if (p->V <= 4 * NT) {
-    if (b) hipLaunchKernelGGL((sample_short_kernel<4, bf16_t>), grid, dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((sample_short_kernel<4, float>), grid, dim3(NT), 0, st, a);
+  // few waves: each repeats the scalar part of every step, on 4 waves per SIMD it would take four times as long
+  if (p->V <= 256 * 4) {
+    if (b) hipLaunchKernelGGL((sample_short_kernel<256, 4, bf16_t>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((sample_short_kernel<256, 4, float>), grid, dim3(256), 0, st, a);
+  } else if (p->V <= 256 * 16) {
+    if (b) hipLaunchKernelGGL((sample_short_kernel<256, 16, bf16_t>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((sample_short_kernel<256, 16, float>), grid, dim3(256), 0, st, a);
   } else if (p->V <= LIST) {
-    if (b) hipLaunchKernelGGL((sample_short_kernel<16, bf16_t>), grid, dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((sample_short_kernel<16, float>), grid, dim3(NT), 0, st, a);
+    if (b) hipLaunchKernelGGL((sample_short_kernel<1024, 16, bf16_t>), grid, dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((sample_short_kernel<1024, 16, float>), grid, dim3(1024), 0, st, a);
   } else {
     const bool al = ops_aligned(p->logits) && (p->rows == 1 || ops_stride16(p->logits_stride, p->x_dtype));
     return b ? (al ? launch_long<bf16_t, true>(a, p->rows, st) : launch_long<bf16_t, false>(a, p->rows, st))
