@@ -50,19 +50,20 @@ __device__ __forceinline__ float logit(const T* x, int i) {   // NaN counts as -
 constexpr uint32_t NEG_INF_KEY = 0x007fffffu;   // order_key(-inf); keys at or below it are no entries
 
 // w * 2^shift as an integer.  2^t = 2^n 2^f with f in [-1/2, 1/2] from its power series (up to f^11: below 2^-47); adding 2^52 leaves the rounded
-// integer in the mantissa (shift <= 51).
+// integer in the mantissa (shift <= 51).  -inf ends as 0 without a test (the maximum also drops the NaN of 0 * -inf).
 struct Weigh {
   float mx;
   double k2;   // log2(e) / T
   int shift;
-  __device__ __forceinline__ uint64_t operator()(float x) const {   // (no branches: lanes differ)
-    const double t = fmax(((double)x - (double)mx) * k2, -1200.0), n = rint(t), f = (t - n) * 0.69314718055994530942;
-    double p = 1.0 / 39916800.0;
-    p = __fma_rn(p, f, 1.0 / 3628800.0); p = __fma_rn(p, f, 1.0 / 362880.0); p = __fma_rn(p, f, 1.0 / 40320.0);
-    p = __fma_rn(p, f, 1.0 / 5040.0); p = __fma_rn(p, f, 1.0 / 720.0); p = __fma_rn(p, f, 1.0 / 120.0); p = __fma_rn(p, f, 1.0 / 24.0);
-    p = __fma_rn(p, f, 1.0 / 6.0); p = __fma_rn(p, f, 0.5); p = __fma_rn(p, f, 1.0); p = __fma_rn(p, f, 1.0);
-    const uint64_t w = (uint64_t)__double_as_longlong(ldexp(p, (int)n + shift) + 4503599627370496.0) & 0xfffffffffffffull;
-    return x == mx ? 1ull << shift : x == -INFINITY || mx == INFINITY ? 0ull : w;
+  __device__ __forceinline__ uint64_t operator()(float x) const {
+    if (mx == INFINITY) return x == INFINITY ? 1ull << shift : 0ull;
+    const double t = fmax(((double)x - (double)mx) * k2, -1200.0), n = rint(t), f = t - n;
+    double p = 4.4455382718708116e-10;   // ln(2)^i / i!, i = 11 .. 0
+    p = __fma_rn(p, f, 7.0549116208011233e-09); p = __fma_rn(p, f, 1.0178086009239700e-07); p = __fma_rn(p, f, 1.3215486790144309e-06);
+    p = __fma_rn(p, f, 1.5252733804059840e-05); p = __fma_rn(p, f, 1.5403530393381610e-04); p = __fma_rn(p, f, 1.3333558146428443e-03);
+    p = __fma_rn(p, f, 9.6181291076284772e-03); p = __fma_rn(p, f, 5.5504108664821580e-02); p = __fma_rn(p, f, 2.4022650695910071e-01);
+    p = __fma_rn(p, f, 6.9314718055994531e-01); p = __fma_rn(p, f, 1.0);
+    return (uint64_t)__double_as_longlong(ldexp(p, (int)n + shift) + 4503599627370496.0) & 0xfffffffffffffull;
   }
 };
 
@@ -136,62 +137,108 @@ struct Block {
   }
 };
 
-// ---- the search ---------------------------------------------------------------------------------------------------------------------------
-struct Cut { uint32_t key; uint32_t ties; };   // kept: keys above `key`, and the first `ties` entries equal to it
-struct Few { uint32_t key[64]; int n; };
-constexpr uint32_t FEW = 32;   // a search ends with at most so many entries: ranking one costs a wave about as much as a third of a step
-
-__device__ __forceinline__ uint32_t probe(uint32_t lo, uint32_t hi, int step) {   // lo < probe < hi: the middle value and the middle key in turn
-  const float v = 0.5f * key_value(lo) + 0.5f * key_value(hi - 1);
-  const uint32_t kv = order_key(v + 0.f);
-  return !(step & 1) && v == v && kv > lo && kv < hi ? kv : lo + (hi - lo) / 2;
+// ---- one wave's sort of 64 values, descending by lane: a bitonic network whose exchanges are DPP moves and row swaps ----------------------------
+template <int D>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  if constexpr (D == 1) return dpp_any<0xB1>(v);
+  if constexpr (D == 2) return dpp_any<0x4E>(v);
+  if constexpr (D == 4) {   // banks 1 and 3 of a row from 4 lanes below, 0 and 2 from 4 lanes above
+    const int up = __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xa, false);
+    return (uint32_t)__builtin_amdgcn_update_dpp(up, (int)v, 0x104, 0xf, 0x5, false);
+  }
+  if constexpr (D == 8) return dpp_any<0x128>(v);
+  if constexpr (D == 16) { const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false); return threadIdx.x & 16 ? r[0] : r[1]; }
+  if constexpr (D == 32) { const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false); return threadIdx.x & 32 ? r[0] : r[1]; }
+}
+template <int D>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) { return (uint64_t)lane_xor<D>((uint32_t)v) | ((uint64_t)lane_xor<D>((uint32_t)(v >> 32)) << 32); }
+template <int SIZE, int D, typename T>
+__device__ __forceinline__ void sort_merge(T& v) {
+  const T o = lane_xor<D>(v);
+  const int lane = threadIdx.x & 63;
+  const bool big = ((lane & D) == 0) == ((lane & SIZE) == 0);   // this lane keeps the larger of the two (SIZE 64: descending throughout)
+  v = (v > o) == big ? v : o;
+  if constexpr (D > 1) sort_merge<SIZE, D / 2>(v);
+}
+template <typename T>
+__device__ __forceinline__ void wave_sort(T& v) {
+  sort_merge<2, 1>(v); sort_merge<4, 2>(v); sort_merge<8, 4>(v); sort_merge<16, 8>(v); sort_merge<32, 16>(v); sort_merge<64, 32>(v);
 }
 
+// ---- the search ---------------------------------------------------------------------------------------------------------------------------
+struct Cut { uint32_t key; uint32_t ties, same; };   // kept: keys above `key`, and the first `ties` of the `same` entries equal to it
+struct Few { uint32_t key[64]; int n; };
+
+// The interval of a search and where to look next: a false-position step over the values (with the Illinois rule: an end that stays twice has its
+// residual halved), every fourth time the middle key -- few steps on a smooth row, a bound on any.  y: the measure's distance from its target
+// in a scale that is straight enough (counts: their logarithm, a tail falls fast; masses: themselves).
+struct Interval {
+  uint32_t lo, hi;      // the target is reached at lo, not at hi
+  float y_lo, y_hi;
+  int step = 0, side = 0;
+  __device__ __forceinline__ uint32_t probe() const {   // lo < probe < hi
+    const float a = key_value(lo), b = key_value(hi - 1);
+    const float part = fminf(fmaxf(y_lo / (y_lo - y_hi), 0.03f), 0.97f);
+    const uint32_t kv = order_key((1.f - part) * a + part * b + 0.f);
+    return (step & 3) != 3 && kv > lo && kv < hi ? kv : lo + (hi - lo) / 2;   // (a NaN's key is above any hi)
+  }
+  __device__ __forceinline__ void take(uint32_t mid, float y, bool reached) {
+    ++step;
+    if (reached) { lo = mid; y_lo = y; if (side == 1) y_hi *= 0.5f; side = 1; }
+    else { hi = mid; y_hi = y; if (side == -1) y_lo *= 0.5f; side = -1; }
+  }
+};
+__device__ __forceinline__ float log_count(uint32_t n) { return __log2f(fmaxf((float)n, 0.5f)); }
+
 // Largest interval end `lo` whose entries at or above it reach the target -- a count (MASS false) or a mass -- narrowed to the exact entry.
-// At entry: everything in [lo, ...) reaches it, nothing at or above hi does (cnt_hi / mass_hi are what lies there).
+// At entry: everything in [lo, ...) reaches it (cnt_lo entries, mass_lo), nothing at or above hi does.
 template <bool MASS, int NT, typename Src>
-__device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, const Weigh& weigh, uint32_t lo, uint32_t cnt_lo, uint32_t hi, uint32_t want_n, double want_m) {
+__device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, const Weigh& weigh, uint32_t lo, uint32_t cnt_lo, uint64_t mass_lo, uint32_t hi, uint32_t want_n, double want_m) {
   uint32_t cnt_hi = 0;
   uint64_t mass_hi = 0;
-  for (int step = 0; cnt_lo - cnt_hi > FEW && hi - lo > 1; ++step) {
-    const uint32_t mid = probe(lo, hi, step);
+  const float goal = MASS ? 0.f : log_count(want_n);
+  Interval in{lo, hi, MASS ? (float)((double)mass_lo - want_m) : log_count(cnt_lo) - goal, MASS ? -(float)want_m : -1.f - goal};
+  while (cnt_lo - cnt_hi > 64 && in.hi - in.lo > 1) {
+    const uint32_t mid = in.probe();
     uint32_t cnt;
     uint64_t mass = 0;
     src.template stat<MASS>(mid, cnt, mass);
     blk.template sum<MASS>(cnt, mass);
-    if (MASS ? (double)mass >= want_m : cnt >= want_n) { lo = mid; cnt_lo = cnt; }
-    else { hi = mid; cnt_hi = cnt; mass_hi = mass; }
+    const bool reached = MASS ? (double)mass >= want_m : cnt >= want_n;
+    in.take(mid, MASS ? (float)((double)mass - want_m) : log_count(cnt) - goal, reached);
+    if (reached) cnt_lo = cnt;
+    else { cnt_hi = cnt; mass_hi = mass; }
   }
+  lo = in.lo; hi = in.hi;
   if (hi - lo <= 1) {   // one key: equal entries, equal weights
-    if (!MASS) return {lo, want_n - cnt_hi};
+    const uint32_t same = cnt_lo - cnt_hi;
+    if (!MASS) return {lo, want_n - cnt_hi, same};
     const uint64_t each = weigh(key_value(lo));
     const double q = each ? ceil((want_m - (double)mass_hi) / (double)each) : 1.0;
-    const uint32_t n = cnt_lo - cnt_hi;
-    return {lo, q < 1.0 ? 1u : q > (double)n ? n : (uint32_t)q};
+    return {lo, q < 1.0 ? 1u : q > (double)same ? same : (uint32_t)q, same};
   }
   if (threadIdx.x == 0) few->n = 0;
   __syncthreads();
   src.gather(lo, hi, few);
   __syncthreads();
-  // every wave ranks the entries itself
-  const int lane = threadIdx.x & 63, n = __builtin_amdgcn_readfirstlane(min(few->n, 64));
-  const uint32_t key = lane < n ? few->key[lane] : 0;
-  const uint64_t w = lane < n && MASS ? weigh(key_value(key)) : 0;
-  uint32_t rank = 0, above = 0;
-  uint64_t before = mass_hi;
-  for (int j = 0; j < n; ++j) {
-    const uint32_t kj = lane_value(key, j);
-    const bool first = kj > key || (kj == key && j < lane);
-    rank += first;
-    above += kj > key;
-    if (MASS) before += first ? lane_value(w, j) : (uint64_t)0;
+  // every wave sorts the entries itself
+  const int lane = threadIdx.x & 63, n = min(few->n, 64);
+  uint32_t key = lane < n ? few->key[lane] : 0;
+  wave_sort(key);
+  bool here = lane < n;
+  if (MASS) {
+    const uint64_t upto = wave_upto(here ? weigh(key_value(key)) : (uint64_t)0);
+    here = here && (double)(mass_hi + upto) >= want_m;
+  } else {
+    here = here && cnt_hi + lane + 1 >= want_n;
   }
-  const bool here = lane < n && (MASS ? (double)before < want_m && (double)(before + w) >= want_m : cnt_hi + rank == want_n - 1);
   const uint64_t at = __ballot(here);
-  const int src_lane = at ? __ffsll((unsigned long long)at) - 1 : 0;
+  const int first = at ? __ffsll((unsigned long long)at) - 1 : 0;
   Cut r;
-  r.key = __builtin_amdgcn_readlane(key, src_lane);
-  r.ties = __builtin_amdgcn_readlane(rank - above, src_lane) + 1;
+  r.key = lane_value(key, first);
+  const uint64_t equal = __ballot(key == r.key);
+  r.same = __popcll(equal);
+  r.ties = __popcll(equal & ((2ull << first) - 1));
   __syncthreads();   // `few` may be filled again
   return r;
 }
@@ -213,33 +260,40 @@ struct RegRow {
     }
   }
   __device__ __forceinline__ void gather(uint32_t lo, uint32_t hi, Few* few) const {
+    uint64_t in[E];
+    uint32_t n = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (key[e] - lo < hi - lo) {
-        const int at = atomicAdd(&few->n, 1);
-        if (at < 64) few->key[at] = key[e];
-      }
+    for (int e = 0; e < E; ++e) {
+      in[e] = __ballot(key[e] - lo < hi - lo);
+      n += __popcll(in[e]);
+    }
+    if (!n) return;
+    uint32_t at = 0;
+    if ((threadIdx.x & 63) == 0) at = atomicAdd(&few->n, (int)n);   // one reservation per wave; the order does not matter, they are sorted
+    at = lane_value(at, 0);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t p = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(in[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[e], 0));
+      if (key[e] - lo < hi - lo && p < 64) few->key[p] = key[e];
+      at += __popcll(in[e]);
+    }
   }
 };
 
-// drop what a cut does not keep
+// of the entries equal to a cut, drop those that it does not keep (entries below it are left: they lie under every later probe)
 template <int E, int NT>
-__device__ __forceinline__ void apply(RegRow<E>& r, Block<NT>& blk, const Cut& c) {
-  uint32_t mine = 0, wave_all = 0;
+__device__ __forceinline__ void drop_ties(RegRow<E>& r, Block<NT>& blk, const Cut& c) {
+  if (c.ties >= c.same) return;
+  uint32_t mine = 0, total;
+#pragma unroll
+  for (int e = 0; e < E; ++e) mine += r.key[e] == c.key;
+  uint32_t rank = blk.before(mine, total);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const bool eq = r.key[e] == c.key;
-    mine += eq;
-    wave_all += __popcll(__ballot(eq));
-  }
-  uint32_t rank = 0, total;
-  if (blk.count(wave_all) > c.ties) rank = blk.before(mine, total);
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const bool eq = r.key[e] == c.key, keep = r.key[e] > c.key || (eq && rank < c.ties);
+    const bool eq = r.key[e] == c.key, drop = eq && rank >= c.ties;
     rank += eq;
-    r.key[e] = keep ? r.key[e] : 0;
-    r.w[e] = keep ? r.w[e] : 0;
+    r.key[e] = drop ? 0 : r.key[e];
+    r.w[e] = drop ? 0 : r.w[e];
   }
 }
 
@@ -266,25 +320,21 @@ __device__ __forceinline__ Setting setting(const SampleOpArgs& a, int row) {
 __device__ __forceinline__ double target(float top_p, double base) { return fmax((double)top_p * base, 1.0); }   // at least one entry
 
 // All filters and the draw on at most 64 entries in index order, by one wave: lane i holds entry i (key 0: none), the first `k` of the order
-// count.  Every lane adds up what precedes it in the order; the result is the entry's lane.
-__device__ __forceinline__ int draw_few(uint32_t key, int n, uint32_t k, const Weigh& weigh, const Setting& s) {
+// count.  The entries are sorted with their places, cut, and their weights sent back to their places for the draw; the result is a place.
+__device__ __forceinline__ int draw_few(uint32_t key, uint32_t k, const Weigh& weigh, const Setting& s) {
   const int lane = threadIdx.x & 63;
-  const uint64_t w = key ? weigh(key_value(key)) : 0;
-  uint32_t rank = 0;
-  uint64_t before = 0;
-  for (int j = 0; j < n; ++j) {
-    const uint32_t kj = lane_value(key, j);
-    const bool first = kj > key || (kj == key && j < lane);
-    rank += first;
-    before += first ? lane_value(w, j) : (uint64_t)0;
-  }
-  bool keep = key && rank < k;
-  const double reach = target(s.top_p, (double)wave_total(keep ? w : (uint64_t)0));   // (every lane takes part)
-  keep = keep && (s.top_p >= 1.f || (double)before < reach);
-  keep = keep && (double)w >= (double)s.min_p * (double)(1ull << weigh.shift);
-  const uint64_t upto = wave_upto(keep ? w : (uint64_t)0);
-  const double want = (double)s.u * (double)lane_value(upto, 63);
-  return __ffsll((unsigned long long)__ballot(keep && (double)upto > want)) - 1;
+  uint64_t c = (uint64_t)key << 32 | (uint32_t)(63 - lane);
+  wave_sort(c);
+  const uint32_t sorted = (uint32_t)(c >> 32);
+  const uint64_t w = sorted && (uint32_t)lane < k ? weigh(key_value(sorted)) : 0, upto = wave_upto(w);
+  const double reach = target(s.top_p, (double)lane_value(upto, 63));
+  const bool keep = w && (s.top_p >= 1.f || (double)(upto - w) < reach) && (double)w >= (double)s.min_p * (double)(1ull << weigh.shift);
+  const int place = 63 - (int)(uint32_t)c;
+  const uint64_t v = keep ? w : 0;
+  const uint64_t back = (uint64_t)(uint32_t)__builtin_amdgcn_ds_permute(place * 4, (int)(uint32_t)v) | (uint64_t)(uint32_t)__builtin_amdgcn_ds_permute(place * 4, (int)(v >> 32)) << 32;
+  const uint64_t cum = wave_upto(back);
+  const double want = (double)s.u * (double)lane_value(cum, 63);
+  return __ffsll((unsigned long long)__ballot(back && (double)cum > want)) - 1;
 }
 
 // The short way for a small top-k: a threshold that leaves between k and 64 entries, these in index order to one wave.  -2: a crowd of equals
@@ -292,16 +342,19 @@ __device__ __forceinline__ int draw_few(uint32_t key, int n, uint32_t k, const W
 struct FewOrder { uint32_t key[64]; int hit; };
 template <int E, int NT>
 __device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, FewOrder* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t k, uint32_t key_min, uint32_t key_max) {
-  uint32_t lo = key_min, hi = key_max + 1, cnt_lo = n;
-  for (int step = 0; cnt_lo > 64 && hi - lo > 1; ++step) {
-    const uint32_t mid = probe(lo, hi, step);
+  uint32_t cnt_lo = n;
+  const float goal = __log2f(0.5f * (float)(k + 64));
+  Interval in{key_min, key_max + 1, log_count(n) - goal, -1.f - goal};
+  while (cnt_lo > 64 && in.hi - in.lo > 1) {
+    const uint32_t mid = in.probe();
     uint32_t cnt;
     uint64_t none = 0;
     r.template stat<false>(mid, cnt, none);
     cnt = blk.count(cnt);
-    if (cnt >= k) { lo = mid; cnt_lo = cnt; }
-    else hi = mid;
+    in.take(mid, log_count(cnt) - goal, cnt >= k);
+    if (cnt >= k) cnt_lo = cnt;
   }
+  const uint32_t lo = in.lo;
   if (cnt_lo > 64) return -2;
   uint32_t mine = 0, total;
 #pragma unroll
@@ -316,7 +369,7 @@ __device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, FewOrder
   __syncthreads();
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
-    const int hit = draw_few(lane < (int)cnt_lo ? few->key[lane] : 0u, (int)cnt_lo, k, weigh, s);
+    const int hit = draw_few(lane < (int)cnt_lo ? few->key[lane] : 0u, k, weigh, s);
     if (lane == 0) few->hit = hit;
   }
   __syncthreads();
@@ -335,24 +388,27 @@ __device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, FewOrder
 template <int E, int NT>
 __device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block<NT>& blk, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, double base, bool& enough) {
   enough = true;
+  Cut cut{key_min, 1u, 1u};
   if (s.k && (uint32_t)s.k < n) {
-    apply(r, blk, find_cut<false>(r, blk, few, weigh, key_min, n, key_max + 1, (uint32_t)s.k, 0.0));
+    cut = find_cut<false>(r, blk, few, weigh, key_min, n, 0, key_max + 1, (uint32_t)s.k, 0.0);
+    drop_ties(r, blk, cut);
     n = (uint32_t)s.k;
   }
   if (s.top_p < 1.f) {
-    uint32_t cnt = 0;
+    uint32_t cnt;
     uint64_t mass = 0;
-    r.template stat<true>(1u, cnt, mass);
+    r.template stat<true>(cut.key, cnt, mass);
     blk.template sum<true>(cnt, mass);
     const double want = target(s.top_p, base < 0.0 ? (double)mass : base);
     if ((double)mass < want) { enough = false; return -1; }
-    apply(r, blk, find_cut<true>(r, blk, few, weigh, key_min, n, key_max + 1, 0u, want));
+    cut = find_cut<true>(r, blk, few, weigh, cut.key, n, mass, key_max + 1, 0u, want);
+    drop_ties(r, blk, cut);
   }
   uint64_t mine = 0, total;
   const double least = (double)s.min_p * (double)(1ull << weigh.shift);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    r.w[e] = (double)r.w[e] < least ? 0 : r.w[e];
+    r.w[e] = r.key[e] < cut.key || (double)r.w[e] < least ? 0 : r.w[e];
     mine += r.w[e];
   }
   const uint64_t before = blk.before(mine, total);
@@ -368,14 +424,30 @@ __device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block<NT>& blk, Few
   return found;
 }
 
-template <int NT>
-__device__ __forceinline__ float block_max(float v, float* s) {
-  v = wave_max(v);
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+// maximum, minimum and count of the entries (values above -inf) of a block, in one exchange
+struct Extremes { float mx, mn; uint32_t n; };
+struct ExtremesLds { float mx[16], mn[16]; uint32_t n[16]; };
+template <int NT, int E>
+__device__ __forceinline__ Extremes extremes(const float (&v)[E], ExtremesLds* s) {
+  float mx = -INFINITY, mn = INFINITY;
+  uint32_t n = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    mx = fmaxf(mx, v[e]);
+    mn = v[e] > -INFINITY ? fminf(mn, v[e]) : mn;
+    n += __popcll(__ballot(v[e] > -INFINITY));
+  }
+  mx = wave_max(mx);
+  mn = -wave_max(-mn);
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) { s->mx[threadIdx.x >> 6] = mx; s->mn[threadIdx.x >> 6] = mn; s->n[threadIdx.x >> 6] = n; }
   __syncthreads();
-  float m = s[(threadIdx.x & 63) % (NT / 64)];
-  m = fmaxf(m, dpp_all<0xB1>(m)); m = fmaxf(m, dpp_all<0x4E>(m)); m = fmaxf(m, dpp_all<0x141>(m)); m = fmaxf(m, dpp_all<0x140>(m));
-  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(m)));
+  constexpr int W = NT / 64;
+  mx = s->mx[lane % W]; mn = -s->mn[lane % W];
+  n = over_waves<W>(s->n[lane % W]);
+  auto all = [](float m) { m = fmaxf(m, dpp_all<0xB1>(m)); m = fmaxf(m, dpp_all<0x4E>(m)); m = fmaxf(m, dpp_all<0x141>(m)); return fmaxf(m, dpp_all<0x140>(m)); };
+  auto uni = [](float m) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(m))); };
+  return {uni(all(mx)), -uni(all(mn)), lane_value(n, 0)};
 }
 
 // rows of at most NT * E entries
@@ -384,7 +456,7 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
   __shared__ Red red;
   __shared__ Few few;
   __shared__ FewOrder order;
-  __shared__ float mx_s[2][16];
+  __shared__ ExtremesLds ext;
   __shared__ int best;
   const int row = blockIdx.x, tid = threadIdx.x;
   const XT* x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
@@ -393,18 +465,14 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
   RegRow<E> r;
   r.per = (a.V + NT - 1) / NT;
   const int first = tid * r.per, mine = min(r.per, a.V - first);   // (mine <= 0 behind the row's end)
-  float v[E], mx = -INFINITY, mn = INFINITY;
+  float v[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = logit(x, min(first + e, a.V - 1));
-  uint32_t n = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    v[e] = e < mine ? v[e] : -INFINITY;
-    mx = fmaxf(mx, v[e]);
-    mn = v[e] > -INFINITY ? fminf(mn, v[e]) : mn;
-    n += __popcll(__ballot(v[e] > -INFINITY));
-  }
-  mx = block_max<NT>(mx, mx_s[0]);
+  for (int e = 0; e < E; ++e) v[e] = e < mine ? v[e] : -INFINITY;
+  const Extremes ex = extremes<NT>(v, &ext);
+  const float mx = ex.mx;
+  const uint32_t n = ex.n;
   if (mx == -INFINITY) {
     if (tid == 0) a.out[row] = -1;
     return;
@@ -420,10 +488,8 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
     if (tid == 0) a.out[row] = best;
     return;
   }
-  mn = -block_max<NT>(-mn, mx_s[1]);
-  n = blk.count(n);
   const Weigh weigh{mx, 1.4426950408889634074 / (double)s.T, a.shift};
-  const uint32_t key_min = order_key(mn), key_max = order_key(mx), k = s.k && (uint32_t)s.k < n ? (uint32_t)s.k : n;
+  const uint32_t key_min = order_key(ex.mn), key_max = order_key(mx), k = s.k && (uint32_t)s.k < n ? (uint32_t)s.k : n;
 #pragma unroll
   for (int e = 0; e < E; ++e) r.key[e] = v[e] > -INFINITY ? order_key(v[e]) : 0;
   int e = -2;
@@ -508,7 +574,7 @@ __global__ __launch_bounds__(256) void sample_threshold_kernel(SampleOpArgs a) {
   constexpr int NT = 256;
   __shared__ Red red;
   __shared__ Few few;
-  __shared__ float mx_s[2][16];
+  __shared__ ExtremesLds ext;
   const int row = blockIdx.x, tid = threadIdx.x;
   const XT* x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
   const Setting s = setting(a, row);
@@ -517,25 +583,17 @@ __global__ __launch_bounds__(256) void sample_threshold_kernel(SampleOpArgs a) {
     constexpr int E = SAMPLES / NT;
     Block<NT> blk{&red};
     RegRow<E> r;
-    uint32_t n = 0;
     float v[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = logit(x, (int)((int64_t)(tid * E + e) * a.V / SAMPLES));
-    float mx = -INFINITY, mn = INFINITY;
+    for (int e = 0; e < E; ++e) v[e] = logit(x, (int)((int64_t)(e * NT + tid) * a.V / SAMPLES));
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      r.key[e] = v[e] > -INFINITY ? order_key(v[e]) : 0;
-      n += __popcll(__ballot(v[e] > -INFINITY));
-      mx = fmaxf(mx, v[e]);
-      mn = v[e] > -INFINITY ? fminf(mn, v[e]) : mn;
-    }
-    mx = block_max<NT>(mx, mx_s[0]);
-    mn = -block_max<NT>(-mn, mx_s[1]);
-    n = blk.count(n);
+    for (int e = 0; e < E; ++e) r.key[e] = v[e] > -INFINITY ? order_key(v[e]) : 0;
+    const Extremes ex = extremes<NT>(v, &ext);
+    const uint32_t n = ex.n;
     const int aim = s.k && s.k < AIM / 4 - 512 ? 4 * s.k + 2048 : AIM;   // a short top-k needs a short list
     const uint32_t rank = max(1u, (uint32_t)((int64_t)aim * SAMPLES / a.V));
     thr = NEG_INF_KEY + 1;
-    if (n > rank) thr = find_cut<false>(r, blk, &few, Weigh{}, order_key(mn), n, order_key(mx) + 1, rank, 0.0).key;
+    if (n > rank) thr = find_cut<false>(r, blk, &few, Weigh{}, order_key(ex.mn), n, 0, order_key(ex.mx) + 1, rank, 0.0).key;
   }
   if (tid == 0) a.thr[row] = thr;
 }
@@ -560,13 +618,16 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
 #pragma unroll
     for (int j = 0; j < PER / 8; ++j) gather8(raw[j], x, i0 + 8 * j, a.V);
   }
+  float v[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const float y = raw[e / 8].get(e % 8) + 0.f;
+    v[e] = y != y ? -INFINITY : y;
+  }
   if (tid == 0) at_s = a.V;
-  auto value = [&](int j, int e) { const float v = raw[j].get(e) + 0.f; return v != v ? -INFINITY : v; };
   float mx = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < PER / 8; ++j)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, value(j, e));
+  for (int e = 0; e < PER; ++e) mx = fmaxf(mx, v[e]);
   const float my_mx = mx;
   mx = wave_max(mx);
   if (lane == 0) mx_s[wave] = mx;
@@ -575,33 +636,21 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
   if (my_mx == mx) {
     int at = a.V;
 #pragma unroll
-    for (int j = PER / 8 - 1; j >= 0; --j)
-#pragma unroll
-      for (int e = 7; e >= 0; --e) at = value(j, e) == mx ? i0 + 8 * j + e : at;
+    for (int e = PER - 1; e >= 0; --e) at = v[e] == mx ? i0 + e : at;
     atomicMin(&at_s, at);
   }
-  const uint32_t thr = a.thr[row];
+  const float thr = key_value(a.thr[row]);   // (~0 is a NaN: nothing is listed)
   uint32_t mine = 0;
 #pragma unroll
-  for (int j = 0; j < PER / 8; ++j)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mine += order_key(value(j, e)) >= thr;
+  for (int e = 0; e < PER; ++e) mine += v[e] >= thr;
   const uint32_t upto = wave_upto(mine);
   // the chunk's mass where it counts: no top-k, and a nucleus or nothing at all to cut
   double mass = 0.0;
   if (!s.k && (s.top_p < 1.f || s.min_p == 0.f) && mx > -INFINITY) {
     const Weigh weigh{mx, 1.4426950408889634074 / (double)s.T, 51};
     uint64_t m = 0;
-    W8<XT> left[PER / 8];
 #pragma unroll
-    for (int j = 0; j < PER / 8; ++j) left[j] = raw[j];
-#pragma unroll 1
-    for (int turn = 0; turn < PER / 8; ++turn) {   // (rolled: code that runs once is paid for by its size)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { const float v = left[0].get(e) + 0.f; m += weigh(v != v ? -INFINITY : v); }
-#pragma unroll
-      for (int j = 0; j + 1 < PER / 8; ++j) left[j] = left[j + 1];
-    }
+    for (int e = 0; e < PER; ++e) m += weigh(v[e]);
     m = wave_total(m);      // 64 * 32 weights of at most 2^51
     mass = (double)m * 0x1p-51;
   }
@@ -619,12 +668,8 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
     uint32_t p = before + upto - mine;
     uint2* list = a.lists + ((int64_t)row * a.chunks + chunk) * CHUNK_CAP;
 #pragma unroll
-    for (int j = 0; j < PER / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t key = order_key(value(j, e));
-        if (key >= thr) { if (p < CHUNK_CAP) list[p] = make_uint2(key, (uint32_t)(i0 + 8 * j + e)); ++p; }
-      }
+    for (int e = 0; e < PER; ++e)
+      if (v[e] >= thr) { if (p < CHUNK_CAP) list[p] = make_uint2(order_key(v[e]), (uint32_t)(i0 + e)); ++p; }
   }
 }
 
@@ -636,7 +681,7 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   __shared__ Red red;
   __shared__ Few few;
   __shared__ FewOrder order;
-  __shared__ float mx_s[16];
+  __shared__ ExtremesLds ext;
   __shared__ int best;
   __shared__ uint32_t start_s[MAX_CHUNKS], tie_s[16];
   __shared__ uint64_t mass_s[16];
@@ -650,7 +695,8 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   ChunkHead h{0.0, -INFINITY, a.V, 0u, 0u};
   if (tid < a.chunks) h = heads[tid];
   if (tid == 0) best = a.V;
-  const float mx = block_max<NT>(h.mx, mx_s);
+  const float hm[1] = {h.mx};
+  const float mx = extremes<NT>(hm, &ext).mx;
   if (mx == -INFINITY) {
     if (tid == 0) a.out[row] = -1;
     return;
@@ -759,13 +805,13 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   }
 
   // the list does not hold the answer: the same search over the row itself
-  Cut cut{0u, 0u};
+  Cut cut{0u, 0u, 0u};
   {
     uint32_t n;
     uint64_t none = 0;
     src.template stat<false>(NEG_INF_KEY + 1, n, none);
     n = blk.count(n);
-    if (s.k && (uint32_t)s.k < n) cut = find_cut<false>(src, blk, &few, weigh, NEG_INF_KEY + 1, n, key_max + 1, (uint32_t)s.k, 0.0);
+    if (s.k && (uint32_t)s.k < n) cut = find_cut<false>(src, blk, &few, weigh, NEG_INF_KEY + 1, n, 0, key_max + 1, (uint32_t)s.k, 0.0);
   }
   if (s.top_p < 1.f) {
     uint32_t cnt;
@@ -776,7 +822,7 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
     const double want = target(s.top_p, (double)(above + each * cut.ties));
     if ((double)above >= want) {
       src.floor_key = max(src.floor_key, cut.key + 1);
-      cut = find_cut<true>(src, blk, &few, weigh, src.floor_key, cnt, key_max + 1, 0u, want);
+      cut = find_cut<true>(src, blk, &few, weigh, src.floor_key, cnt, above, key_max + 1, 0u, want);
       src.floor_key = NEG_INF_KEY + 1;
     } else {
       const double q = each ? ceil((want - (double)above) / (double)each) : 1.0;
