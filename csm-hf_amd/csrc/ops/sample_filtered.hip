@@ -37,18 +37,30 @@ constexpr int SAMPLES = 4096, AIM = LIST * 3 / 4;   // the list's threshold is a
 constexpr int CHUNK = 8192, CHUNK_CAP = 2048, MAX_V = 1 << 21, MAX_CHUNKS = MAX_V / CHUNK;
 struct ChunkHead { double mass; float mx; int32_t at; uint32_t count, pad; };   // mass relative to the chunk's own maximum, `at` its first place
 
-__device__ __forceinline__ uint32_t order_key(float x) {   // larger float = larger key
-  const uint32_t u = __float_as_uint(x);
-  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
-}
-__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k >> 31) ? k ^ 0x80000000u : ~k); }
+// Order keys: larger value = larger key, one key per value of the type (a search that must end on a single key needs 16 fewer steps where
+// values are bf16).  value() of a key that no number has is a NaN.  Keys at or below NONE are no entries.
+template <typename T>
+struct Keys;
+template <>
+struct Keys<float> {
+  static constexpr uint32_t NONE = 0x007fffffu;   // of -inf
+  static __device__ __forceinline__ uint32_t key(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+  }
+  static __device__ __forceinline__ float value(uint32_t k) { return __uint_as_float((k >> 31) ? k ^ 0x80000000u : ~k); }
+};
+template <>
+struct Keys<bf16_t> {
+  static constexpr uint32_t NONE = Keys<float>::NONE >> 16;
+  static __device__ __forceinline__ uint32_t key(float x) { return Keys<float>::key(x) >> 16; }   // (other values than the type's: the next key below)
+  static __device__ __forceinline__ float value(uint32_t k) { return Keys<float>::value(k << 16 | ((k >> 15) ? 0u : 0xffffu)); }
+};
 template <typename T>
 __device__ __forceinline__ float logit(const T* x, int i) {   // NaN counts as -inf, -0 as +0
   const float v = to_f32(x[i]) + 0.f;
   return v != v ? -INFINITY : v;
 }
-constexpr uint32_t NEG_INF_KEY = 0x007fffffu;   // order_key(-inf); keys at or below it are no entries
-
 // w * 2^shift as an integer.  2^t = 2^n 2^f with f in [-1/2, 1/2] from its power series (up to f^11: below 2^-47); adding 2^52 leaves the rounded
 // integer in the mantissa (shift <= 51).  -inf ends as 0 without a test (the maximum also drops the NaN of 0 * -inf).
 struct Weigh {
@@ -77,6 +89,8 @@ template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_any(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
 template <int CTRL>
 __device__ __forceinline__ uint64_t dpp_any(uint64_t v) { return (uint64_t)dpp_any<CTRL>((uint32_t)v) | ((uint64_t)dpp_any<CTRL>((uint32_t)(v >> 32)) << 32); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp0(double v) { return __longlong_as_double((long long)dpp0<CTRL, ROWS>((uint64_t)__double_as_longlong(v))); }
 template <typename T>
 __device__ __forceinline__ T row_upto(T v) {   // within 16 lanes
   v += dpp0<0x111, 0xf>(v); v += dpp0<0x112, 0xf>(v); v += dpp0<0x114, 0xf>(v); v += dpp0<0x118, 0xf>(v);
@@ -172,14 +186,15 @@ struct Few { uint32_t key[64]; int n; };
 // The interval of a search and where to look next: a false-position step over the values (with the Illinois rule: an end that stays twice has its
 // residual halved), every fourth time the middle key -- few steps on a smooth row, a bound on any.  y: the measure's distance from its target
 // in a scale that is straight enough (counts: their logarithm, a tail falls fast; masses: themselves).
+template <typename K>
 struct Interval {
   uint32_t lo, hi;      // the target is reached at lo, not at hi
   float y_lo, y_hi;
   int step = 0, side = 0;
   __device__ __forceinline__ uint32_t probe() const {   // lo < probe < hi
-    const float a = key_value(lo), b = key_value(hi - 1);
+    const float a = K::value(lo), b = K::value(hi - 1);
     const float part = fminf(fmaxf(y_lo / (y_lo - y_hi), 0.03f), 0.97f);
-    const uint32_t kv = order_key((1.f - part) * a + part * b + 0.f);
+    const uint32_t kv = K::key((1.f - part) * a + part * b + 0.f);
     return (step & 3) != 3 && kv > lo && kv < hi ? kv : lo + (hi - lo) / 2;   // (a NaN's key is above any hi)
   }
   __device__ __forceinline__ void take(uint32_t mid, float y, bool reached) {
@@ -192,12 +207,12 @@ __device__ __forceinline__ float log_count(uint32_t n) { return __log2f(fmaxf((f
 
 // Largest interval end `lo` whose entries at or above it reach the target -- a count (MASS false) or a mass -- narrowed to the exact entry.
 // At entry: everything in [lo, ...) reaches it (cnt_lo entries, mass_lo), nothing at or above hi does.
-template <bool MASS, int NT, typename Src>
+template <typename K, bool MASS, int NT, typename Src>
 __device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, const Weigh& weigh, uint32_t lo, uint32_t cnt_lo, uint64_t mass_lo, uint32_t hi, uint32_t want_n, double want_m) {
   uint32_t cnt_hi = 0;
   uint64_t mass_hi = 0;
   const float goal = MASS ? 0.f : log_count(want_n);
-  Interval in{lo, hi, MASS ? (float)((double)mass_lo - want_m) : log_count(cnt_lo) - goal, MASS ? -(float)want_m : -1.f - goal};
+  Interval<K> in{lo, hi, MASS ? (float)((double)mass_lo - want_m) : log_count(cnt_lo) - goal, MASS ? -(float)want_m : -1.f - goal};
   while (cnt_lo - cnt_hi > 64 && in.hi - in.lo > 1) {
     const uint32_t mid = in.probe();
     uint32_t cnt;
@@ -213,7 +228,7 @@ __device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, cons
   if (hi - lo <= 1) {   // one key: equal entries, equal weights
     const uint32_t same = cnt_lo - cnt_hi;
     if (!MASS) return {lo, want_n - cnt_hi, same};
-    const uint64_t each = weigh(key_value(lo));
+    const uint64_t each = weigh(K::value(lo));
     const double q = each ? ceil((want_m - (double)mass_hi) / (double)each) : 1.0;
     return {lo, q < 1.0 ? 1u : q > (double)same ? same : (uint32_t)q, same};
   }
@@ -227,7 +242,7 @@ __device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, cons
   wave_sort(key);
   bool here = lane < n;
   if (MASS) {
-    const uint64_t upto = wave_upto(here ? weigh(key_value(key)) : (uint64_t)0);
+    const uint64_t upto = wave_upto(here ? weigh(K::value(key)) : (uint64_t)0);
     here = here && (double)(mass_hi + upto) >= want_m;
   } else {
     here = here && cnt_hi + lane + 1 >= want_n;
@@ -254,6 +269,7 @@ struct RegRow {
     cnt = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
+      if (E > 4 && e % 4 == 0 && e >= per) break;   // (uniform; in steps of four)
       const bool in = key[e] >= c;
       cnt += __popcll(__ballot(in));
       if (MASS) mass += in ? w[e] : 0;
@@ -321,12 +337,13 @@ __device__ __forceinline__ double target(float top_p, double base) { return fmax
 
 // All filters and the draw on at most 64 entries in index order, by one wave: lane i holds entry i (key 0: none), the first `k` of the order
 // count.  The entries are sorted with their places, cut, and their weights sent back to their places for the draw; the result is a place.
+template <typename K>
 __device__ __forceinline__ int draw_few(uint32_t key, uint32_t k, const Weigh& weigh, const Setting& s) {
   const int lane = threadIdx.x & 63;
   uint64_t c = (uint64_t)key << 32 | (uint32_t)(63 - lane);
   wave_sort(c);
   const uint32_t sorted = (uint32_t)(c >> 32);
-  const uint64_t w = sorted && (uint32_t)lane < k ? weigh(key_value(sorted)) : 0, upto = wave_upto(w);
+  const uint64_t w = sorted && (uint32_t)lane < k ? weigh(K::value(sorted)) : 0, upto = wave_upto(w);
   const double reach = target(s.top_p, (double)lane_value(upto, 63));
   const bool keep = w && (s.top_p >= 1.f || (double)(upto - w) < reach) && (double)w >= (double)s.min_p * (double)(1ull << weigh.shift);
   const int place = 63 - (int)(uint32_t)c;
@@ -340,11 +357,11 @@ __device__ __forceinline__ int draw_few(uint32_t key, uint32_t k, const Weigh& w
 // The short way for a small top-k: a threshold that leaves between k and 64 entries, these in index order to one wave.  -2: a crowd of equals
 // allows no such threshold.  Otherwise the place (e, in the thread that owns it) or -1.  Needs keys only.
 struct FewOrder { uint32_t key[64]; int hit; };
-template <int E, int NT>
+template <typename K, int E, int NT>
 __device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, FewOrder* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t k, uint32_t key_min, uint32_t key_max) {
   uint32_t cnt_lo = n;
   const float goal = __log2f(0.5f * (float)(k + 64));
-  Interval in{key_min, key_max + 1, log_count(n) - goal, -1.f - goal};
+  Interval<K> in{key_min, key_max + 1, log_count(n) - goal, -1.f - goal};
   while (cnt_lo > 64 && in.hi - in.lo > 1) {
     const uint32_t mid = in.probe();
     uint32_t cnt;
@@ -369,7 +386,7 @@ __device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, FewOrder
   __syncthreads();
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
-    const int hit = draw_few(lane < (int)cnt_lo ? few->key[lane] : 0u, k, weigh, s);
+    const int hit = draw_few<K>(lane < (int)cnt_lo ? few->key[lane] : 0u, k, weigh, s);
     if (lane == 0) few->hit = hit;
   }
   __syncthreads();
@@ -385,12 +402,12 @@ __device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, FewOrder
 
 // filters and draw on entries in registers; returns the place (e, in the thread that owns it) or -1.  `base`: the mass that top_p refers to when
 // it is not that of these entries (< 0: it is).  `enough` comes back false when these entries cannot hold the nucleus.
-template <int E, int NT>
+template <typename K, int E, int NT>
 __device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block<NT>& blk, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, double base, bool& enough) {
   enough = true;
   Cut cut{key_min, 1u, 1u};
   if (s.k && (uint32_t)s.k < n) {
-    cut = find_cut<false>(r, blk, few, weigh, key_min, n, 0, key_max + 1, (uint32_t)s.k, 0.0);
+    cut = find_cut<K, false>(r, blk, few, weigh, key_min, n, 0, key_max + 1, (uint32_t)s.k, 0.0);
     drop_ties(r, blk, cut);
     n = (uint32_t)s.k;
   }
@@ -401,7 +418,7 @@ __device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block<NT>& blk, Few
     blk.template sum<true>(cnt, mass);
     const double want = target(s.top_p, base < 0.0 ? (double)mass : base);
     if ((double)mass < want) { enough = false; return -1; }
-    cut = find_cut<true>(r, blk, few, weigh, cut.key, n, mass, key_max + 1, 0u, want);
+    cut = find_cut<K, true>(r, blk, few, weigh, cut.key, n, mass, key_max + 1, 0u, want);
     drop_ties(r, blk, cut);
   }
   uint64_t mine = 0, total;
@@ -453,6 +470,7 @@ __device__ __forceinline__ Extremes extremes(const float (&v)[E], ExtremesLds* s
 // rows of at most NT * E entries
 template <int NT, int E, typename XT>
 __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
+  using K = Keys<XT>;
   __shared__ Red red;
   __shared__ Few few;
   __shared__ FewOrder order;
@@ -489,16 +507,16 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
     return;
   }
   const Weigh weigh{mx, 1.4426950408889634074 / (double)s.T, a.shift};
-  const uint32_t key_min = order_key(ex.mn), key_max = order_key(mx), k = s.k && (uint32_t)s.k < n ? (uint32_t)s.k : n;
+  const uint32_t key_min = K::key(ex.mn), key_max = K::key(mx), k = s.k && (uint32_t)s.k < n ? (uint32_t)s.k : n;
 #pragma unroll
-  for (int e = 0; e < E; ++e) r.key[e] = v[e] > -INFINITY ? order_key(v[e]) : 0;
+  for (int e = 0; e < E; ++e) r.key[e] = v[e] > -INFINITY ? K::key(v[e]) : 0;
   int e = -2;
-  if (k <= 64) e = draw_small(r, blk, &order, weigh, s, n, k, key_min, key_max);
+  if (k <= 64) e = draw_small<K>(r, blk, &order, weigh, s, n, k, key_min, key_max);
   if (e == -2) {
 #pragma unroll
     for (int i = 0; i < E; ++i) r.w[i] = weigh(v[i]);
     bool enough;
-    e = filter_and_draw(r, blk, &few, weigh, s, n, key_min, key_max, -1.0, enough);
+    e = filter_and_draw<K>(r, blk, &few, weigh, s, n, key_min, key_max, -1.0, enough);
   }
   if (e >= 0) a.out[row] = first + e;
 }
@@ -525,6 +543,7 @@ __device__ __forceinline__ void gather8<bf16_t>(W8<bf16_t>& r, const bf16_t* x, 
 // The row as it lies in memory, for the search that streams.  A wave owns a run of consecutive entries (a multiple of 64 * VEC).
 template <typename XT, bool ALIGNED>
 struct LongRow {
+  using K = Keys<XT>;
   static constexpr int VEC = 8;
   const XT* x;
   int V, seg;
@@ -549,7 +568,7 @@ struct LongRow {
     uint32_t n = 0;
     uint64_t m = 0;
     each(begin(), end(), [&](int, float v, bool) {
-      const uint32_t key = order_key(v);
+      const uint32_t key = K::key(v);
       const bool in = key >= c && key >= floor_key;
       n += __popcll(__ballot(in));
       if (MASS) { const uint64_t w = (*weigh)(v); m += in ? w : 0; }
@@ -559,7 +578,7 @@ struct LongRow {
   }
   __device__ __forceinline__ void gather(uint32_t lo, uint32_t hi, Few* few) const {
     each(begin(), end(), [&](int, float v, bool) {
-      const uint32_t key = order_key(v);
+      const uint32_t key = K::key(v);
       if (key >= lo && key < hi && key >= floor_key) {
         const int at = atomicAdd(&few->n, 1);
         if (at < 64) few->key[at] = key;
@@ -571,6 +590,7 @@ struct LongRow {
 // ---- launch 1 of a long row: the list's threshold, from samples spread over the row.  ~0 = no list
 template <typename XT>
 __global__ __launch_bounds__(256) void sample_threshold_kernel(SampleOpArgs a) {
+  using K = Keys<XT>;
   constexpr int NT = 256;
   __shared__ Red red;
   __shared__ Few few;
@@ -583,17 +603,18 @@ __global__ __launch_bounds__(256) void sample_threshold_kernel(SampleOpArgs a) {
     constexpr int E = SAMPLES / NT;
     Block<NT> blk{&red};
     RegRow<E> r;
+    r.per = E;
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = logit(x, (int)((int64_t)(e * NT + tid) * a.V / SAMPLES));
 #pragma unroll
-    for (int e = 0; e < E; ++e) r.key[e] = v[e] > -INFINITY ? order_key(v[e]) : 0;
+    for (int e = 0; e < E; ++e) r.key[e] = v[e] > -INFINITY ? K::key(v[e]) : 0;
     const Extremes ex = extremes<NT>(v, &ext);
     const uint32_t n = ex.n;
     const int aim = s.k && s.k < AIM / 4 - 512 ? 4 * s.k + 2048 : AIM;   // a short top-k needs a short list
     const uint32_t rank = max(1u, (uint32_t)((int64_t)aim * SAMPLES / a.V));
-    thr = NEG_INF_KEY + 1;
-    if (n > rank) thr = find_cut<false>(r, blk, &few, Weigh{}, order_key(ex.mn), n, 0, order_key(ex.mx) + 1, rank, 0.0).key;
+    thr = K::NONE + 1;
+    if (n > rank) thr = find_cut<K, false>(r, blk, &few, Weigh{}, K::key(ex.mn), n, 0, K::key(ex.mx) + 1, rank, 0.0).key;
   }
   if (tid == 0) a.thr[row] = thr;
 }
@@ -601,6 +622,7 @@ __global__ __launch_bounds__(256) void sample_threshold_kernel(SampleOpArgs a) {
 // ---- launch 2: a workgroup per chunk.  A thread owns 32 consecutive entries.
 template <typename XT, bool ALIGNED>
 __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
+  using K = Keys<XT>;
   constexpr int PER = CHUNK / 256;
   __shared__ float mx_s[4];
   __shared__ double mass_s[4];
@@ -639,7 +661,7 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
     for (int e = PER - 1; e >= 0; --e) at = v[e] == mx ? i0 + e : at;
     atomicMin(&at_s, at);
   }
-  const float thr = key_value(a.thr[row]);   // (~0 is a NaN: nothing is listed)
+  const float thr = K::value(a.thr[row]);   // (~0 is a NaN: nothing is listed)
   uint32_t mine = 0;
 #pragma unroll
   for (int e = 0; e < PER; ++e) mine += v[e] >= thr;
@@ -669,13 +691,14 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
     uint2* list = a.lists + ((int64_t)row * a.chunks + chunk) * CHUNK_CAP;
 #pragma unroll
     for (int e = 0; e < PER; ++e)
-      if (v[e] >= thr) { if (p < CHUNK_CAP) list[p] = make_uint2(order_key(v[e]), (uint32_t)(i0 + e)); ++p; }
+      if (v[e] >= thr) { if (p < CHUNK_CAP) list[p] = make_uint2(K::key(v[e]), (uint32_t)(i0 + e)); ++p; }
   }
 }
 
 // ---- launch 3: a workgroup per row
 template <typename XT, bool ALIGNED>
 __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
+  using K = Keys<XT>;
   constexpr int NT = 1024;
   extern __shared__ __attribute__((aligned(16))) uint32_t keys[];   // [LIST]
   __shared__ Red red;
@@ -709,19 +732,25 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   }
   const double k2 = 1.4426950408889634074 / (double)s.T;
   const Weigh weigh{mx, k2, a.shift};
-  // masses of the chunks in one scale, summed in their order by one thread: the same bits every time
+  // masses of the chunks in one scale, summed by one wave in a fixed order: the same bits every time
   if (tid < a.chunks) cum_s[tid] = h.mx == mx ? h.mass : h.mx == -INFINITY || mx == INFINITY ? 0.0 : h.mass * exp2(fmax(((double)h.mx - (double)mx) * k2, -1200.0));
   uint64_t n_list;
   const uint64_t start = blk.before((uint64_t)(tid < a.chunks ? h.count : 0), n_list);
   if (tid < a.chunks) start_s[tid] = (uint32_t)start;
   const uint32_t crowded = blk.count(__popcll(__ballot(h.count > CHUNK_CAP)));
-  if (tid == 0) {
-    double c = 0.0;
-    for (int i = 0; i < a.chunks; ++i) { c += cum_s[i]; cum_s[i] = c; }
+  __syncthreads();
+  if (tid < 64) {   // 4 consecutive chunks a lane
+    double c[4], run = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = run += 4 * lane + i < a.chunks ? cum_s[4 * lane + i] : 0.0;
+    const double before = wave_upto(run) - run;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * lane + i < a.chunks) cum_s[4 * lane + i] = before + c[i];
   }
   __syncthreads();
   const double all = cum_s[a.chunks - 1];
-  const uint32_t key_max = order_key(mx);
+  const uint32_t key_max = K::key(mx);
 
   LongRow<XT, ALIGNED> src;
   constexpr int VEC = LongRow<XT, ALIGNED>::VEC;
@@ -729,7 +758,7 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   src.V = a.V;
   src.seg = (a.V + NT * VEC - 1) / (NT * VEC) * (64 * VEC);
   src.weigh = &weigh;
-  src.floor_key = NEG_INF_KEY + 1;
+  src.floor_key = K::NONE + 1;
 
   if (!s.k && s.top_p >= 1.f && s.min_p == 0.f) {   // nothing is cut: the chunk that holds u * total, then its entries
     const double want = (double)s.u * all;
@@ -770,12 +799,13 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   }
 
   bool ok = !crowded && n_list > 0 && n_list <= LIST;
-  if (ok && s.k) ok = n_list >= (uint64_t)s.k || thr <= NEG_INF_KEY + 1;
-  if (ok && !s.k && s.top_p >= 1.f) ok = thr <= NEG_INF_KEY + 1 || (double)weigh(key_value(thr)) < (double)s.min_p * (double)(1ull << a.shift);   // min-p alone: all it keeps is listed
+  if (ok && s.k) ok = n_list >= (uint64_t)s.k || thr <= K::NONE + 1;
+  if (ok && !s.k && s.top_p >= 1.f) ok = thr <= K::NONE + 1 || (double)weigh(K::value(thr)) < (double)s.min_p * (double)(1ull << a.shift);   // min-p alone: all it keeps is listed
   if (ok) {
     const uint2* lists = a.lists + (int64_t)row * a.chunks * CHUNK_CAP;
     for (int c = wave; c < a.chunks; c += 16) {
       const uint32_t at = start_s[c], cnt = (c + 1 < a.chunks ? start_s[c + 1] : (uint32_t)n_list) - at;
+#pragma unroll 8
       for (uint32_t i = lane; i < cnt; i += 64) keys[at + i] = lists[(int64_t)c * CHUNK_CAP + i].x;
     }
     __syncthreads();
@@ -789,11 +819,14 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
     }
     bool enough = true;
     int e = -2;
-    if (s.k && s.k <= 64) e = draw_small(r, blk, &order, weigh, s, n, min((uint32_t)s.k, n), thr, key_max);
+    if (s.k && s.k <= 64) e = draw_small<K>(r, blk, &order, weigh, s, n, min((uint32_t)s.k, n), thr, key_max);
     if (e == -2) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) r.w[i] = r.key[i] ? weigh(key_value(r.key[i])) : 0;
-      e = filter_and_draw(r, blk, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << a.shift), enough);
+      for (int i = 0; i < E; ++i) {
+        r.w[i] = 0;
+        if (i < r.per) r.w[i] = r.key[i] ? weigh(K::value(r.key[i])) : 0;
+      }
+      e = filter_and_draw<K>(r, blk, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << a.shift), enough);
     }
     if (e >= 0) {
       const uint32_t p = tid * r.per + e;
@@ -809,21 +842,21 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   {
     uint32_t n;
     uint64_t none = 0;
-    src.template stat<false>(NEG_INF_KEY + 1, n, none);
+    src.template stat<false>(K::NONE + 1, n, none);
     n = blk.count(n);
-    if (s.k && (uint32_t)s.k < n) cut = find_cut<false>(src, blk, &few, weigh, NEG_INF_KEY + 1, n, 0, key_max + 1, (uint32_t)s.k, 0.0);
+    if (s.k && (uint32_t)s.k < n) cut = find_cut<K, false>(src, blk, &few, weigh, K::NONE + 1, n, 0, key_max + 1, (uint32_t)s.k, 0.0);
   }
   if (s.top_p < 1.f) {
     uint32_t cnt;
     uint64_t above = 0;
     src.template stat<true>(cut.key + 1, cnt, above);
     blk.template sum<true>(cnt, above);
-    const uint64_t each = cut.ties ? weigh(key_value(cut.key)) : 0;
+    const uint64_t each = cut.ties ? weigh(K::value(cut.key)) : 0;
     const double want = target(s.top_p, (double)(above + each * cut.ties));
     if ((double)above >= want) {
       src.floor_key = max(src.floor_key, cut.key + 1);
-      cut = find_cut<true>(src, blk, &few, weigh, src.floor_key, cnt, above, key_max + 1, 0u, want);
-      src.floor_key = NEG_INF_KEY + 1;
+      cut = find_cut<K, true>(src, blk, &few, weigh, src.floor_key, cnt, above, key_max + 1, 0u, want);
+      src.floor_key = K::NONE + 1;
     } else {
       const double q = each ? ceil((want - (double)above) / (double)each) : 1.0;
       if (q < (double)cut.ties) cut.ties = q < 1.0 ? 1u : (uint32_t)q;
@@ -835,14 +868,14 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   uint64_t mass = 0;
   uint32_t ties = 0;
   src.each(src.begin(), src.end(), [&](int, float v, bool) {
-    const uint32_t key = order_key(v);
+    const uint32_t key = K::key(v);
     const uint64_t w = value(v);
-    mass += key > cut.key && key > NEG_INF_KEY ? w : 0;
+    mass += key > cut.key && key > K::NONE ? w : 0;
     ties += key == cut.key;
   });
   mass = wave_total(mass);
   ties = wave_total(ties);
-  const uint64_t each = cut.ties ? value(key_value(cut.key)) : 0;
+  const uint64_t each = cut.ties ? value(K::value(cut.key)) : 0;
   if (lane == 0) { mass_s[wave] = mass; tie_s[wave] = ties; }
   __syncthreads();
   uint64_t total = 0, run_before = 0;
@@ -867,13 +900,13 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   const int lo = min(at * src.seg, a.V), hi = min(lo + src.seg, a.V), per = (hi - lo + NT - 1) / NT;
   const int i0 = min(lo + tid * per, hi), i1 = min(i0 + per, hi);
   uint64_t my_ties = 0, unused;
-  for (int i = i0; i < i1; ++i) my_ties += order_key(logit(src.x, i)) == cut.key;
+  for (int i = i0; i < i1; ++i) my_ties += K::key(logit(src.x, i)) == cut.key;
   const uint64_t seen0 = tie_before + blk.before(my_ties, unused);
   uint64_t seen = seen0, mine = 0;
   auto kept = [&](int i) -> uint64_t {
     const float v = logit(src.x, i);
-    const uint32_t key = order_key(v);
-    if (key <= NEG_INF_KEY || key < cut.key || (key == cut.key && seen++ >= cut.ties)) return 0;
+    const uint32_t key = K::key(v);
+    if (key <= K::NONE || key < cut.key || (key == cut.key && seen++ >= cut.ties)) return 0;
     return value(v);
   };
   for (int i = i0; i < i1; ++i) mine += kept(i);
