@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Optional, Union
 
 import torch
@@ -52,6 +53,13 @@ class SampleArgs(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+# A call packs its arguments in one go (setting two dozen ctypes fields takes longer than the smallest kernels run); the ctypes structures above
+# describe the same layout.
+_P_PAGED = "PPiiiiiqqqqqqPqiiPPi0P"
+_PACK_APPEND = struct.Struct("@" + _P_PAGED + "PPqqiiPPii0P").pack
+_PACK_ATTENTION = struct.Struct("@" + _P_PAGED + "PPqqiiPiifPN").pack
+_PACK_SAMPLE = struct.Struct("@PqiiiPPPPPfffiPPN").pack
+
 _lib = None
 
 
@@ -63,35 +71,52 @@ def load_ops_library():
             raise RuntimeError(f"{OPS_LIB_PATH} not found: build it with `python -m csm_hf_amd.build` (hipcc, gfx950); csm_hf_amd has no CPU fallback")
         lib = C.CDLL(OPS_LIB_PATH)
         for name in OPS_EXPORTS:
-            getattr(lib, name).restype = C.c_int
+            fn = getattr(lib, name)
+            fn.restype = C.c_int
+            if name.endswith("_workspace"):
+                fn.argtypes = [C.c_char_p, C.POINTER(C.c_size_t)]
+            elif name not in ("csm_ops_last_error", "csm_ops_abi_version"):
+                fn.argtypes = [C.c_char_p, C.c_void_p]
         lib.csm_ops_last_error.restype = C.c_char_p
         if lib.csm_ops_abi_version() != OPS_ABI_VERSION:
             raise RuntimeError(f"libcsm_ops.so ABI {lib.csm_ops_abi_version()} != binding {OPS_ABI_VERSION}")
-        lib.csm_ops_paged_rope_append.argtypes = [C.POINTER(RopeAppendArgs), C.c_void_p]
-        lib.csm_ops_paged_attention_workspace.argtypes = [C.POINTER(AttentionArgs), C.POINTER(C.c_size_t)]
-        lib.csm_ops_paged_prefix_attention.argtypes = [C.POINTER(AttentionArgs), C.c_void_p]
-        lib.csm_ops_sample_workspace.argtypes = [C.POINTER(SampleArgs), C.POINTER(C.c_size_t)]
-        lib.csm_ops_sample_filtered.argtypes = [C.POINTER(SampleArgs), C.c_void_p]
         _lib = lib
     return _lib
 
 
 def _ck(lib, rc: int):
-    if rc != 0:
-        msg = lib.csm_ops_last_error().decode(errors="replace")
-        if rc == -3:
-            raise ValueError(f"csm_ops capacity error: {msg}")
-        raise RuntimeError(f"csm_ops error {rc}: {msg}")
+    msg = lib.csm_ops_last_error().decode(errors="replace")
+    if rc == -3:
+        raise ValueError(f"csm_ops capacity error: {msg}")
+    raise RuntimeError(f"csm_ops error {rc}: {msg}")
 
 
-def _call(fn, args, device):
-    """One launch on the current stream of `device`."""
-    lib = load_ops_library()
-    if device.index == torch.cuda.current_device():
-        _ck(lib, fn(C.byref(args), torch.cuda.current_stream().cuda_stream))
+def _call(fn, args: bytes, device: int):
+    """One launch on the current stream of GPU `device`."""
+    if device == torch.cuda.current_device():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            _ck(lib, fn(C.byref(args), torch.cuda.current_stream().cuda_stream))
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        _ck(_lib, rc)
+
+
+_workspace_sizes = {}
+
+
+def _workspace(fn, args: bytes, key, device: int) -> Optional[torch.Tensor]:
+    """Scratch memory of one call, on the current stream like everything a call allocates.  How much depends on the sizes in `key` alone."""
+    need = _workspace_sizes.get(key)
+    if need is None:
+        size = C.c_size_t()
+        rc = fn(args, C.byref(size))
+        if rc:
+            _ck(_lib, rc)
+        if len(_workspace_sizes) > 4096:
+            _workspace_sizes.clear()
+        need = _workspace_sizes[key] = size.value
+    return torch.empty(need, dtype=torch.uint8, device=f"cuda:{device}") if need else None
 
 
 def _need(ok: bool, what: str):
@@ -99,50 +124,60 @@ def _need(ok: bool, what: str):
         raise ValueError(what)
 
 
-def _on_device(first: torch.Tensor, *named):
-    """Every tensor on the GPU of `first`, dense, and none that asks for a gradient."""
-    if first.device.type != "cuda":
+def _on_device(first: torch.Tensor, named) -> int:
+    """The GPU that holds `first`; every other tensor must be there too, and none may ask for a gradient."""
+    dev = first.get_device()
+    if dev < 0:
         raise RuntimeError("csm_hf_amd operators need tensors on the GPU (no CPU fallback)")
+    grad = torch.is_grad_enabled()
     for name, t in named:
-        if t is None:
-            continue
-        if t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, expected {first.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{name} requires a gradient: this operator has no backward pass (call it under torch.no_grad())")
+        if t is not None:
+            if t.get_device() != dev:
+                raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
+            if grad and t.requires_grad:
+                raise RuntimeError(f"{name} requires a gradient: this operator has no backward pass (call it under torch.no_grad())")
+    return dev
 
 
-def _ints(name: str, t: torch.Tensor, shape):
-    _need(t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and t.is_contiguous(), f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}")
+def _index(name: str, v) -> int:
+    if not -2 ** 31 <= int(v) < 2 ** 31:
+        raise ValueError(f"{name} = {v} is out of range")
+    return int(v)
+
+
+def _ints(name: str, t: torch.Tensor, n: int) -> int:
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape ({n},)")
     return t.data_ptr()
 
 
-def _paged(p: PagedArgs, k_cache, v_cache, page_table, seq_lens, cu_rows, rows: int):
-    _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype and k_cache.dtype in _DT,
-          "k_cache and v_cache must be float32 or bfloat16 tensors [n_pages, n_kv, page_size, head_dim] of one shape and dtype")
-    p.n_pages, p.n_kv, p.page_size, p.head_dim = k_cache.shape
-    p.k_page_stride, p.k_head_stride, p.k_slot_stride, k_inner = k_cache.stride()
-    p.v_page_stride, p.v_head_stride, p.v_slot_stride, v_inner = v_cache.stride()
-    _need((k_inner == 1 and v_inner == 1) or p.head_dim == 1, "the last dimension of k_cache and v_cache must be contiguous")
-    p.k, p.v, p.dtype = k_cache.data_ptr(), v_cache.data_ptr(), _DT[k_cache.dtype]
-    _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and (page_table.shape[1] <= 1 or page_table.stride(1) == 1),
-          "page_table must be an int32 tensor [n_seqs, pages] with contiguous rows")
-    p.n_seqs, p.table_width = page_table.shape
-    p.page_table, p.table_stride = page_table.data_ptr(), page_table.stride(0)
-    p.seq_lens = _ints("seq_lens", seq_lens, (p.n_seqs,))
-    if cu_rows is not None:
-        p.cu_rows = _ints("cu_rows", cu_rows, (p.n_seqs + 1,))
-    else:
-        _need(rows == p.n_seqs, f"without cu_rows every sequence has one row: {rows} rows, {p.n_seqs} sequences")
-    p.rows = rows
+def _paged(k_cache, v_cache, page_table, seq_lens, cu_rows, rows: int):
+    """the fields of csm_ops_paged_t"""
+    shape, dt = k_cache.shape, _DT.get(k_cache.dtype)
+    if dt is None or len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype:
+        raise ValueError("k_cache and v_cache must be float32 or bfloat16 tensors [n_pages, n_kv, page_size, head_dim] of one shape and dtype")
+    n_pages, n_kv, page, hd = shape
+    kp, kh, ks, ki = k_cache.stride()
+    vp, vh, vs, vi = v_cache.stride()
+    if (ki != 1 or vi != 1) and hd != 1:
+        raise ValueError("the last dimension of k_cache and v_cache must be contiguous")
+    if page_table.dim() != 2 or page_table.dtype is not torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table must be an int32 tensor [n_seqs, pages] with contiguous rows")
+    n_seqs, width = page_table.shape
+    if cu_rows is None and rows != n_seqs:
+        raise ValueError(f"without cu_rows every sequence has one row: {rows} rows, {n_seqs} sequences")
+    return (k_cache.data_ptr(), v_cache.data_ptr(), dt, n_pages, page, n_kv, hd, kp, kh, ks, vp, vh, vs, page_table.data_ptr(), page_table.stride(0),
+            width, n_seqs, _ints("seq_lens", seq_lens, n_seqs), 0 if cu_rows is None else _ints("cu_rows", cu_rows, n_seqs + 1), rows)
 
 
 def _heads(name: str, t: torch.Tensor, shape, dtype):
     """[rows, heads, dim] with contiguous heads; returns (pointer, row stride)"""
-    _need(t.dtype == dtype and tuple(t.shape) == tuple(shape), f"{name} must be a {dtype} tensor of shape {tuple(shape)}")
-    _need(t.numel() == 0 or ((t.shape[2] == 1 or t.stride(2) == 1) and (t.shape[1] == 1 or t.stride(1) == t.shape[2])),
-          f"the heads of a row of {name} must be contiguous")
-    return t.data_ptr(), t.stride(0)
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)}")
+    a, b, c = t.stride()
+    if (c != 1 and shape[2] > 1) or (b != shape[2] and shape[1] > 1):
+        _need(t.numel() == 0, f"the heads of a row of {name} must be contiguous")
+    return t.data_ptr(), a
 
 
 def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -162,24 +197,28 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
     A sequence with `seq_lens < 0` is padding.  Its rows, rows behind `cu_rows[-1]` and rows whose slot, page or rotary position lies outside the
     table, the cache or the tables are skipped: nothing is written for them, in q_out either.  Two rows that share a cache slot (a page that
     two sequences write to) leave either row's values there.  q, k and v must not overlap in memory with the cache."""
-    _on_device(qkv, ("qkv", qkv), ("cos", cos), ("sin", sin), ("k_cache", k_cache), ("v_cache", v_cache), ("page_table", page_table),
-               ("seq_lens", seq_lens), ("cu_rows", cu_rows), ("q_out", q_out))
-    a = RopeAppendArgs()
-    _need(qkv.dim() == 2 and qkv.dtype in _DT and (qkv.shape[1] <= 1 or qkv.stride(1) == 1), "qkv must be a float32 or bfloat16 tensor [rows, (n_q + 2 n_kv) * head_dim] with contiguous rows")
-    rows = qkv.shape[0]
-    _paged(a.c, k_cache, v_cache, page_table, seq_lens, cu_rows, rows)
-    hd, n_kv = a.c.head_dim, a.c.n_kv
-    n_q = qkv.shape[1] // hd - 2 * n_kv if hd else 0
-    _need(n_q >= 1 and qkv.shape[1] == (n_q + 2 * n_kv) * hd, f"qkv rows of {qkv.shape[1]} elements are not n_q + 2 * {n_kv} heads of {hd}")
+    dev = _on_device(qkv, (("qkv", qkv), ("cos", cos), ("sin", sin), ("k_cache", k_cache), ("v_cache", v_cache), ("page_table", page_table),
+                           ("seq_lens", seq_lens), ("cu_rows", cu_rows), ("q_out", q_out)))
+    x = _DT.get(qkv.dtype)
+    if x is None or qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+        raise ValueError("qkv must be a float32 or bfloat16 tensor [rows, (n_q + 2 n_kv) * head_dim] with contiguous rows")
+    rows, width = qkv.shape
+    c = _paged(k_cache, v_cache, page_table, seq_lens, cu_rows, rows)
+    n_kv, hd = c[5], c[6]
+    n_q = width // hd - 2 * n_kv if hd else 0
+    if n_q < 1 or width != (n_q + 2 * n_kv) * hd:
+        raise ValueError(f"qkv rows of {width} elements are not n_q + 2 * {n_kv} heads of {hd}")
+    half = hd // 2
     for name, t in (("cos", cos), ("sin", sin)):
-        _need(t.dtype == torch.float32 and t.dim() == 2 and t.shape[1] == hd // 2 and t.is_contiguous(), f"{name} must be a contiguous float32 tensor [positions, {hd // 2}]")
-    _need(cos.shape == sin.shape, "cos and sin must have one shape")
+        if t.dtype is not torch.float32 or t.dim() != 2 or t.shape[1] != half or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 tensor [positions, {half}]")
+    if cos.shape != sin.shape:
+        raise ValueError("cos and sin must have one shape")
     if q_out is None:
-        q_out = torch.empty(rows, n_q, hd, dtype=qkv.dtype, device=qkv.device)
-    a.q_out, a.q_out_stride = _heads("q_out", q_out, (rows, n_q, hd), qkv.dtype)
-    a.qkv, a.qkv_stride, a.x_dtype, a.n_q = qkv.data_ptr(), qkv.stride(0), _DT[qkv.dtype], n_q
-    a.cos, a.sin, a.rope_positions, a.pos_offset = cos.data_ptr(), sin.data_ptr(), cos.shape[0], int(pos_offset)
-    _call(load_ops_library().csm_ops_paged_rope_append, a, qkv.device)
+        q_out = qkv.new_empty((rows, n_q, hd))
+    q, q_stride = _heads("q_out", q_out, (rows, n_q, hd), qkv.dtype)
+    args = _PACK_APPEND(*c, qkv.data_ptr(), q, qkv.stride(0), q_stride, x, n_q, cos.data_ptr(), sin.data_ptr(), cos.shape[0], _index("pos_offset", pos_offset))
+    _call((_lib or load_ops_library()).csm_ops_paged_rope_append, args, dev)
     return q_out
 
 
@@ -196,28 +235,28 @@ def paged_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
     A row that sees no key gives zeros.  Rows of padding (`seq_lens < 0`) and rows behind `cu_rows[-1]` keep what `out` held.  Slots on pages
     outside the cache are not seen.  `prefix_len` and all sizes are fixed in a captured graph; lengths, tables and `cu_rows` are read at replay."""
-    _on_device(q, ("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("page_table", page_table), ("seq_lens", seq_lens),
-               ("prefix_table", prefix_table), ("cu_rows", cu_rows), ("out", out))
-    a = AttentionArgs()
-    _need(q.dim() == 3 and q.dtype in _DT, "q must be a float32 or bfloat16 tensor [rows, n_q, head_dim]")
-    _paged(a.c, k_cache, v_cache, page_table, seq_lens, cu_rows, q.shape[0])
-    _need(q.shape[2] == a.c.head_dim, f"q has heads of {q.shape[2]}, the cache of {a.c.head_dim}")
+    dev = _on_device(q, (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("page_table", page_table), ("seq_lens", seq_lens),
+                         ("prefix_table", prefix_table), ("cu_rows", cu_rows), ("out", out)))
+    x, shape = _DT.get(q.dtype), q.shape
+    if x is None or len(shape) != 3:
+        raise ValueError("q must be a float32 or bfloat16 tensor [rows, n_q, head_dim]")
+    c = _paged(k_cache, v_cache, page_table, seq_lens, cu_rows, shape[0])
+    if shape[2] != c[6]:
+        raise ValueError(f"q has heads of {shape[2]}, the cache of {c[6]}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    a.q, a.q_stride = _heads("q", q, q.shape, q.dtype)
-    a.out, a.out_stride = _heads("out", out, q.shape, q.dtype)
-    a.x_dtype, a.n_q = _DT[q.dtype], q.shape[1]
-    a.prefix_len = int(prefix_len)
+        out = q.new_empty(shape)
+    pq, q_stride = _heads("q", q, shape, q.dtype)
+    po, o_stride = _heads("out", out, shape, q.dtype)
+    prefix_len, n_prefix, pp = _index("prefix_len", prefix_len), 0, 0
     if prefix_table is not None:
-        a.prefix_pages, a.prefix_table = prefix_table.numel(), _ints("prefix_table", prefix_table, (prefix_table.numel(),))
-    a.scale = q.shape[2] ** -0.5 if scale is None else float(scale)
-    lib = load_ops_library()
-    need = C.c_size_t()
-    _ck(lib, lib.csm_ops_paged_attention_workspace(C.byref(a), C.byref(need)))
-    if need.value:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
-    _call(lib.csm_ops_paged_prefix_attention, a, q.device)
+        n_prefix = prefix_table.numel()
+        pp = _ints("prefix_table", prefix_table, n_prefix)
+    rest = (pq, po, q_stride, o_stride, x, shape[1], pp, n_prefix, prefix_len, shape[2] ** -0.5 if scale is None else scale)
+    lib = _lib or load_ops_library()
+    # (what the split of the work goes by: types, sizes of rows, heads, pages and table, prefix)
+    ws = _workspace(lib.csm_ops_paged_attention_workspace, _PACK_ATTENTION(*c, *rest, 0, 0),
+                    (shape, x, c[2], c[4], c[5], c[15], c[16], cu_rows is None, prefix_len, n_prefix), dev)
+    _call(lib.csm_ops_paged_prefix_attention, _PACK_ATTENTION(*c, *rest, *((0, 0) if ws is None else (ws.data_ptr(), ws.numel()))), dev)
     return out
 
 
@@ -232,35 +271,36 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, *, temperature:
     index at which the running sum of kept probability passes `uniform` times its total.  `temperature = 0` is the arg-max, the lowest index
     of equals, like `sample_topk`; exactly `topk` entries stay, so `topk = 1` is the arg-max too (`sample_topk` keeps every entry that ties with
     the k-th).  V up to 2^21; a NaN logit counts as -inf; a row with nothing but -inf gives -1."""
-    _on_device(logits, ("logits", logits), ("uniform", uniform))
-    _need(logits.dim() >= 1 and logits.dtype in _DT, "logits must be a float32 or bfloat16 tensor [..., V]")
-    V, lead = logits.shape[-1], logits.shape[:-1]
+    dev = _on_device(logits, (("logits", logits), ("uniform", uniform)))
+    x, lead = _DT.get(logits.dtype), logits.shape[:-1]
+    if x is None or logits.dim() < 1:
+        raise ValueError("logits must be a float32 or bfloat16 tensor [..., V]")
+    V = logits.shape[-1]
     lg = logits if logits.dim() == 2 and (V <= 1 or logits.stride(1) == 1) else logits.reshape(-1, V).contiguous()
     rows = lg.shape[0]
-    a = SampleArgs()
     keep = []
 
     def per_row(name, t, dtype):
-        _need(t.dtype == dtype and t.numel() == rows and (t.dim() <= 1 or t.shape == lead), f"{name} must be a {dtype} tensor with one value per row")
-        if t.device != logits.device:
-            raise ValueError(f"{name} is on {t.device}, expected {logits.device}")
-        t = t.reshape(-1).contiguous()
-        keep.append(t)
+        if t.dtype is not dtype or t.numel() != rows or (t.dim() > 1 and t.shape != lead):
+            raise ValueError(f"{name} must be a {dtype} tensor with one value per row")
+        if t.get_device() != dev:
+            raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
+        if t.dim() != 1 or not t.is_contiguous():
+            t = t.reshape(-1).contiguous()
+            keep.append(t)
         return t.data_ptr()
-    a.uniform = per_row("uniform", uniform, torch.float32)
-    for name, one, many, value, dtype in (("temperature", "temperature", "temperatures", temperature, torch.float32), ("topk", "topk", "topks", topk, torch.int32),
-                                          ("top_p", "top_p", "top_ps", top_p, torch.float32), ("min_p", "min_p", "min_ps", min_p, torch.float32)):
+    pu = per_row("uniform", uniform, torch.float32)
+    one, many = [1.0, 1.0, 0.0, 0], [0, 0, 0, 0]
+    for i, (name, value) in enumerate((("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("topk", topk))):
         if torch.is_tensor(value):
-            setattr(a, many, per_row(name, value, dtype))
+            many[i] = per_row(name, value, torch.int32 if i == 3 else torch.float32)
         else:
-            setattr(a, one, int(value) if dtype is torch.int32 else float(value))
-    out = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    a.logits, a.logits_stride, a.x_dtype, a.rows, a.V, a.out = lg.data_ptr(), lg.stride(0), _DT[lg.dtype], rows, V, out.data_ptr()
-    lib = load_ops_library()
-    need = C.c_size_t()
-    _ck(lib, lib.csm_ops_sample_workspace(C.byref(a), C.byref(need)))
-    if need.value:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=logits.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
-    _call(lib.csm_ops_sample_filtered, a, logits.device)
-    return out.view(*lead, 1)
+            one[i] = _index(name, value) if i == 3 else value
+    out = logits.new_empty((*lead, 1), dtype=torch.int32)
+    args = (lg.data_ptr(), lg.stride(0), x, rows, V, pu, *many, *one, out.data_ptr())
+    lib = _lib or load_ops_library()
+    ws = None
+    if V > 4096:
+        ws = _workspace(lib.csm_ops_sample_workspace, _PACK_SAMPLE(*args, 0, 0), (rows, V), dev)
+    _call(lib.csm_ops_sample_filtered, _PACK_SAMPLE(*args, *((0, 0) if ws is None else (ws.data_ptr(), ws.numel()))), dev)
+    return out

@@ -50,6 +50,20 @@ def test_header_is_plain_c_and_structs_match(tmp_path):
         assert got == [n, str(C.sizeof(s))] + [str(getattr(s, f[0]).offset) for f in s._fields_]
 
 
+def test_packed_arguments_match_the_structures():
+    """the wrappers pack their arguments; every value must land in the field that the header names"""
+    def leaves(s):
+        for f in s._fields_:
+            v = getattr(s, f[0])
+            if isinstance(v, C.Structure):
+                yield from leaves(v)
+            else:
+                yield v
+    for struct_type, pack, n in ((ops.RopeAppendArgs, ops._PACK_APPEND, 30), (ops.AttentionArgs, ops._PACK_ATTENTION, 32), (ops.SampleArgs, ops._PACK_SAMPLE, 17)):
+        values = list(range(1, n + 1))
+        assert list(leaves(struct_type.from_buffer_copy(pack(*values)))) == values
+
+
 def _paged_args(p, **over):
     """a valid description of 2 sequences on made-up addresses: only ever handed to calls that must refuse it"""
     for k, v in dict(dict(k=1 << 20, v=1 << 21, dtype=1, n_pages=4, page_size=16, n_kv=2, head_dim=64, k_page_stride=2048, k_head_stride=1024, k_slot_stride=64,
@@ -69,7 +83,7 @@ def test_append_refusals(over):
     for k, v in over.items():
         if not hasattr(a.c, k):
             setattr(a, k, v)
-    assert lib.csm_ops_paged_rope_append(C.byref(a), None) in (-1, -3) and lib.csm_ops_last_error()
+    assert lib.csm_ops_paged_rope_append(bytes(a), None) in (-1, -3) and lib.csm_ops_last_error()
     assert lib.csm_ops_paged_rope_append(None, None) == -1
 
 
@@ -84,8 +98,8 @@ def test_attention_refusals(over):
         if not hasattr(a.c, k):
             setattr(a, k, v)
     need = C.c_size_t()
-    assert lib.csm_ops_paged_attention_workspace(C.byref(a), C.byref(need)) in (-1, -3)
-    assert lib.csm_ops_paged_prefix_attention(C.byref(a), None) in (-1, -3) and lib.csm_ops_last_error()
+    assert lib.csm_ops_paged_attention_workspace(bytes(a), C.byref(need)) in (-1, -3)
+    assert lib.csm_ops_paged_prefix_attention(bytes(a), None) in (-1, -3) and lib.csm_ops_last_error()
 
 
 @pytest.mark.parametrize("over", [
@@ -96,7 +110,7 @@ def test_sample_refusals(over):
     a = ops.SampleArgs(logits=1 << 20, logits_stride=100, x_dtype=0, rows=2, V=100, uniform=1 << 21, temperature=1.0, top_p=1.0, min_p=0.0, topk=0, out=1 << 22)
     for k, v in over.items():
         setattr(a, k, v)
-    assert lib.csm_ops_sample_filtered(C.byref(a), None) in (-1, -3) and lib.csm_ops_last_error()
+    assert lib.csm_ops_sample_filtered(bytes(a), None) in (-1, -3) and lib.csm_ops_last_error()
 
 
 def test_cpu_tensors_are_refused():
