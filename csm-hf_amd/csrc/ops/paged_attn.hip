@@ -2,13 +2,15 @@
 //   out[r, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q.k_j - m),   j over the prefix's slots and own slots 0 .. slot(r)
 //
 // The keys of a row form one axis: prefix slots 0 .. P-1, then own slots.  Query rows of one kv-head are FLATTENED to (token row, head of the
-// group): f = row * rep + h.  A workgroup takes up to 64 such rows and a range of the axis:
-//   prefix item : rows of the WHOLE batch, range inside the prefix -- a prefix slot is fetched once per 64 rows, not once per sequence;
+// group): f = row * rep + h.  A workgroup takes up to 128 (bf16) or 64 such rows and a range of the axis:
+//   prefix item : rows of the WHOLE batch, range inside the prefix -- a prefix slot is fetched once per 128 rows, not once per sequence;
 //   own item    : rows of one sequence, range inside its own slots (its prefix too, where every sequence brings rows enough of its own);
-// and leaves (max, sum, unnormalised output) per row, which a second small launch joins.  Up to 16 live rows: the four waves split the keys and
-// join through LDS.  More: the waves split the rows.
+// and leaves (max, sum, unnormalised output) per row, which a second small launch joins.
+//   up to 16 live rows (decode): the launch waits for memory.  The four waves split the keys, each streams its own, and they join through LDS.
+//   more rows, bf16 cache:       64-key tiles of K and V are staged once per workgroup in LDS (two buffers), every wave takes 16-row tiles.
+//   more rows, fp32 cache:       every wave streams all keys for its 16 rows.
 //
-// One pass per wave, 16 query rows at a time, both products transposed so that a lane owns one query row from score to result:
+// Per wave and 16 query rows, both products are transposed so that a lane owns one query row from score to result:
 //   S^T[key][row] = K Q^T   lane (row = lane % 16, g = lane / 16) ends with the scores of keys 4g .. 4g+3 of each 16-key group
 //   O^T[d][row]  += V^T P^T contracted over keys in exactly that order, so P never leaves its lane
 // K goes from memory straight into the A operand (a lane's 16 bytes are 8 elements of one key); V passes through a wave-private LDS tile and
@@ -36,7 +38,8 @@ struct AttnOpArgs {
   float2* ml;             // [rows * n_q][nsplit] (reference in log2 units, sum)
 };
 
-constexpr int AT = 256, MAX_SPLIT = 64, ROWS = 64;
+constexpr int AT = 256, MAX_SPLIT = 64;
+constexpr int tile_rows(int x_dtype) { return x_dtype == CSM_OPS_BF16 ? 128 : 64; }
 constexpr float SLACK = 8.f;
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {   // round to nearest even
@@ -302,12 +305,148 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const Prod<XT, 
   l = xor32_sum(xor16_sum(l));
 }
 
+// ---- many rows on a bf16 cache: 64-key tiles shared by the workgroup ---------------------------------------------------------------------------
+// bf16 queries: two 16-row tiles per wave, so that a K or V operand read from LDS feeds two products; p is ONE bf16 piece here -- a second rounding of
+// the size of the result's own (the sum l is of the same rounded p) against half again as many matrix instructions.  fp32 queries: one tile
+// per wave, q and p in three exact pieces.  l comes off the matrix pipe too, as a product with ones.
+template <typename XT, int HD>
+struct Wide {
+  static constexpr int RT = sizeof(XT) == 2 ? 2 : 1, NQ = sizeof(XT) == 2 ? 1 : 3, NP = NQ, T = HD / 32, KEYS = 64, CH = HD / 8, KPP = AT / CH, NL = KEYS / KPP;
+  static constexpr int TILE = KEYS * HD * 2, LDS_BYTES = 4 * TILE;   // K, V, two buffers
+  b16x8 q[RT][NQ][T];
+  f32x4 o[RT][HD / 16], l4[RT];
+  float m[RT];
+
+  __device__ __forceinline__ void run(const AttnOpArgs& a, const KeyAxis& ax, int kvh, int k0, int k1, const int (&lim)[RT], const int (&lim_min)[RT], int n_rt, char* lds) {
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g = lane >> 4;
+    const bf16_t* kb = reinterpret_cast<const bf16_t*>(a.k) + kvh * a.c.kh;
+    const bf16_t* vb = reinterpret_cast<const bf16_t*>(a.v) + kvh * a.c.vh;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      m[r] = -INFINITY;
+      l4[r] = (f32x4)(0.f);
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) o[r][i] = (f32x4)(0.f);
+    }
+    if (k0 >= k1) return;
+    // every wave looks up the pages of a tile's 64 keys, lane = key; a thread stages chunk tid % CH of keys i * KPP + tid / CH
+    auto look = [&](int j0) { const int j = j0 + lane; return j < k1 ? ax.page(j, a.c) : -1; };
+    u32x4 kr[NL], vr[NL];
+    const int ch = tid % CH, key0 = tid / CH;
+    auto fetch = [&](int j0, int page) -> uint64_t {
+      const uint64_t valid = __ballot(page >= 0);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int kk = i * KPP + key0;
+        const int pg = max(__shfl(page, kk), 0), sl = ax.slot(min(j0 + kk, k1 - 1), a.c);
+        kr[i] = *reinterpret_cast<const u32x4*>(kb + pg * a.c.kp + sl * a.c.ks + ch * 8);
+        vr[i] = *reinterpret_cast<const u32x4*>(vb + pg * a.c.vp + sl * a.c.vs + ch * 8);
+      }
+      return valid;
+    };
+    uint64_t valid = fetch(k0, look(k0));
+    int page = look(k0 + KEYS);
+    const b16x8 ones = (b16x8)((short)0x3f80);
+    int buf = 0;
+    for (int j = k0; j < k1; j += KEYS, buf ^= 1) {
+      char* const ks = lds + buf * 2 * TILE;
+      char* const vs = ks + TILE;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int kk = i * KPP + key0, at = kk * HD * 2 + ((ch ^ (kk & 7)) << 4);
+        if (valid != ~0ull && !((valid >> kk) & 1)) vr[i] = (u32x4)(0u);   // 0 * (what an unused slot holds) must be 0
+        *reinterpret_cast<u32x4*>(ks + at) = kr[i];
+        *reinterpret_cast<u32x4*>(vs + at) = vr[i];
+      }
+      __syncthreads();   // (one per tile: a buffer is written again only two tiles later)
+      const uint64_t now = valid;
+      if (j + KEYS < k1) {
+        valid = fetch(j + KEYS, page);
+        page = look(j + 2 * KEYS);
+      }
+      if (n_rt == 0) continue;
+      f32x4 s[RT][4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        b16x8 k[T];
+#pragma unroll
+        for (int x = 0; x < T; ++x) k[x] = *reinterpret_cast<const b16x8*>(ks + (16 * kt + li) * HD * 2 + (((4 * x + g) ^ (li & 7)) << 4));
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          if (r && n_rt < 2) break;
+          s[r][kt] = (f32x4)(0.f);
+#pragma unroll
+          for (int n = NQ - 1; n >= 0; --n)
+#pragma unroll
+            for (int x = 0; x < T; ++x) s[r][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[x], q[r][n][x], s[r][kt], 0, 0, 0);
+        }
+      }
+      b16x8 p[RT][2][NP];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        if (r && n_rt < 2) break;
+        if (now != ~0ull || j + KEYS > lim_min[r]) {
+          const uint64_t seen = now >> (4 * g);
+          const int left = lim[r] - j - 4 * g;
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[r][kt][e] = ((seen >> (16 * kt + e)) & 1) && 16 * kt + e < left ? s[r][kt][e] : -INFINITY;
+        }
+        float top = s[r][0][0];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[r][kt][e]);
+        top *= a.c2;
+        if (__any(top > m[r] + SLACK)) {
+          top = xor32_max(xor16_max(top));
+          const float m_new = fmaxf(m[r], top), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - m_new);
+          l4[r] *= alpha;
+#pragma unroll
+          for (int i = 0; i < HD / 16; ++i) o[r][i] *= alpha;
+          m[r] = m_new;
+        }
+        const float ref = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[r][kt][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[r][kt][e], a.c2, -ref));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float x[8] = {s[r][2 * h][0], s[r][2 * h][1], s[r][2 * h][2], s[r][2 * h][3], s[r][2 * h + 1][0], s[r][2 * h + 1][1], s[r][2 * h + 1][2], s[r][2 * h + 1][3]};
+          split8<NP>(x, p[r][h]);
+#pragma unroll
+          for (int n = NP - 1; n >= 0; --n) l4[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][h][n], l4[r], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; ++dt) {
+          const int kk = 32 * h + 4 * g + (li >> 2), at = (((2 * dt + ((li & 3) >> 1)) ^ (kk & 7)) << 4) + (li & 1) * 8;
+          typedef __attribute__((address_space(3))) b16x4* lp;
+          const b16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + kk * HD * 2 + at));
+          const b16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + (kk + 16) * HD * 2 + at));
+          const b16x8 v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            if (r && n_rt < 2) break;
+#pragma unroll
+            for (int n = NP - 1; n >= 0; --n) o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[r][h][n], o[r][dt], 0, 0, 0);
+          }
+        }
+    }
+  }
+};
+
 // ---- results ------------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
 __device__ __forceinline__ void store4(bf16_t* p, const f32x4& v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])); }
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }   // a row without a key: zeros
 
 // sequence and tile of own item `tile` when rows are ragged: tiles are counted per sequence in order
+template <int ROWS>
 __device__ __forceinline__ bool find_tile(const AttnOpArgs& a, int tile, int& seq, int& first, int& n_rows, int& in_seq) {
   const Paged& c = a.c;
   const int lane = threadIdx.x & 63;
@@ -340,11 +479,30 @@ __device__ __forceinline__ bool find_tile(const AttnOpArgs& a, int tile, int& se
   return false;
 }
 
+// a finished 16-row tile: the result itself, or partial result number `slot`.  The lane holds elements 16 dt + 4 g .. + 3 of its row
+template <typename XT, int HD>
+__device__ __forceinline__ void put(const AttnOpArgs& a, int row, int head, int slot, int g, const f32x4 (&o)[HD / 16], float m, float l) {
+  if (a.nsplit == 1) {
+    const float inv = inverse(l);
+    XT* y = reinterpret_cast<XT*>(a.out) + row * a.out_stride + (int64_t)head * HD + 4 * g;
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) store4(y + 16 * dt, o[dt] * inv);
+  } else {
+    const int64_t at = ((int64_t)row * a.n_q + head) * a.nsplit + slot;
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) store4(a.part + at * HD + 16 * dt + 4 * g, o[dt]);
+    if (g == 0) a.ml[at] = make_float2(m, l);
+  }
+}
+
 template <typename XT, typename CT, int HD>
 __global__ __launch_bounds__(AT, 2) void paged_attn_kernel(AttnOpArgs a) {
   using P = Prod<XT, CT, HD>;
+  constexpr bool WIDE = sizeof(CT) == 2;
+  constexpr int ROWS = tile_rows(sizeof(XT) == 2 ? CSM_OPS_BF16 : CSM_OPS_F32);
   constexpr int WAVE_LDS = P::LDS_BYTES > 16 * (HD + 4) * 4 ? P::LDS_BYTES : 16 * (HD + 4) * 4;   // V tile; at the end 16 rows of fp32 results
-  __shared__ __attribute__((aligned(16))) char lds[4 * WAVE_LDS];
+  constexpr int LDS = WIDE && Wide<XT, HD>::LDS_BYTES > 4 * WAVE_LDS ? Wide<XT, HD>::LDS_BYTES : 4 * WAVE_LDS;
+  __shared__ __attribute__((aligned(16))) char lds[LDS];
   __shared__ float ml_s[4][16][2];
   const Paged& c = a.c;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
@@ -366,12 +524,12 @@ __global__ __launch_bounds__(AT, 2) void paged_attn_kernel(AttnOpArgs a) {
     slot_bias = 0;
     k0 = 0; axis_end = a.prefix_len;
   } else {
-    it -= a.np_tiles * a.nsp;
+    it = a.np_tiles * a.nsp + a.no_tiles * a.nso - 1 - it;   // the last rows of a sequence see most keys: they start first
     split = it % a.nso;
     const int tile = it / a.nso;
     int seq, in_seq;
     if (c.cu) {
-      if (!find_tile(a, tile, seq, row0, n_rows, in_seq)) return;
+      if (!find_tile<ROWS>(a, tile, seq, row0, n_rows, in_seq)) return;
     } else {
       seq = tile / a.per_seq_tiles;
       in_seq = tile - seq * a.per_seq_tiles;
@@ -388,14 +546,50 @@ __global__ __launch_bounds__(AT, 2) void paged_attn_kernel(AttnOpArgs a) {
   }
   const int nsplit = own ? a.nso : a.nsp, slot0 = own ? a.nsplit - a.nso : 0;
   {
-    constexpr int KT = 16 * P::NG;
+    constexpr int KT = 64;   // ranges of whole tiles
     const int span = max(axis_end - k0, 0), chunk = ((span + nsplit - 1) / nsplit + KT - 1) / KT * KT;
     k0 = min(k0 + split * chunk, axis_end);
     k1 = min(k0 + chunk, axis_end);
     if (c.n_pages == 0) k1 = k0;
   }
-  // rows of this wave: all waves the same 16 (keys split over the waves), or 16 each
   const bool by_keys = live <= 16;
+  if constexpr (WIDE) {
+    if (!by_keys) {   // 16-row tiles wave, wave + 4
+      using Wd = Wide<XT, HD>;
+      Wd w;
+      int lim[Wd::RT], lim_min[Wd::RT], n_rt = 0;
+#pragma unroll
+      for (int r = 0; r < Wd::RT; ++r) {
+        const int first = 16 * (wave + 4 * r), f = f0 + first + li;
+        n_rt += first < live;
+        lim[r] = own ? sees(f / a.rep) : a.prefix_len;
+        lim_min[r] = own ? sees((f0 + first) / a.rep) : a.prefix_len;   // rows ascend: the first sees least
+        const bool on = first + li < live;
+        const XT* qp = on ? reinterpret_cast<const XT*>(a.q) + (row0 + f / a.rep) * a.q_stride + (int64_t)(kvh * a.rep + f % a.rep) * HD : nullptr;
+#pragma unroll
+        for (int t = 0; t < Wd::T; ++t) {
+          float x[8];
+          W8<XT> raw;
+          if (qp) raw.load(qp + 32 * t + 8 * g); else raw.zero();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(__float_as_uint(raw.get(i)) ^ a.q_flip);
+          b16x8 piece[Wd::NQ];
+          split8<Wd::NQ>(x, piece);
+#pragma unroll
+          for (int n = 0; n < Wd::NQ; ++n) w.q[r][n][t] = piece[n];
+        }
+      }
+      w.run(a, ax, kvh, k0, k1, lim, lim_min, n_rt, lds);
+#pragma unroll
+      for (int r = 0; r < Wd::RT; ++r) {
+        const int first = 16 * (wave + 4 * r), f = f0 + first + li;
+        if (first + li >= live) continue;
+        put<XT, HD>(a, row0 + f / a.rep, kvh * a.rep + f % a.rep, slot0 + split, g, w.o[r], w.m[r], w.l4[r][0]);
+      }
+      return;
+    }
+  }
+  // rows of this wave: all waves the same 16 (keys split over the waves), or 16 each
   const int mine = by_keys ? 0 : 16 * wave, n_mine = min(16, live - mine);
   char* my_lds = lds + wave * WAVE_LDS;
   f32x4 o[HD / 16];
@@ -442,48 +636,33 @@ __global__ __launch_bounds__(AT, 2) void paged_attn_kernel(AttnOpArgs a) {
     }
     return;
   }
-  if (!row_live) return;
-  const int64_t at = (int64_t)row * a.n_q + head;
-  if (a.nsplit == 1) {
-    const float inv = inverse(l);
-    XT* y = reinterpret_cast<XT*>(a.out) + row * a.out_stride + (int64_t)head * HD + 4 * g;
-#pragma unroll
-    for (int dt = 0; dt < HD / 16; ++dt) store4(y + 16 * dt, o[dt] * inv);
-  } else {
-    float* y = a.part + (at * a.nsplit + slot0 + split) * HD + 4 * g;
-#pragma unroll
-    for (int dt = 0; dt < HD / 16; ++dt) store4(y + 16 * dt, o[dt]);
-    if (g == 0) a.ml[at * a.nsplit + slot0 + split] = make_float2(m, l);
-  }
+  if (row_live) put<XT, HD>(a, row, head, slot0 + split, g, o, m, l);
 }
 
-// join the partial results of a (row, head): one wave each
+// join the partial results: a thread per 4 elements of a (row, head)
 template <typename XT, int HD>
 __global__ __launch_bounds__(AT) void paged_attn_join_kernel(AttnOpArgs a) {
   const Paged& c = a.c;
-  const int lane = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int PER = HD / 4;
+  const int64_t i = (int64_t)blockIdx.x * AT + threadIdx.x, at = i / PER;
+  const int d = (int)(i % PER) * 4;
   if (at >= (int64_t)c.rows * a.n_q) return;
   const int row = (int)(at / a.n_q), head = (int)(at - (int64_t)row * a.n_q);
   const int seq = c.cu ? ops_find_seq(c.cu, c.n_seqs, row) : row;
   if (seq < 0 || c.lens[seq] < 0) return;
-  const float2 x = lane < a.nsplit ? a.ml[at * a.nsplit + lane] : make_float2(-INFINITY, 0.f);
-  const float top = wave_max(x.x);
-  const float w = lane < a.nsplit ? (x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x.x - top)) : 0.f;
-  const float inv = inverse(wave_sum(w * x.y));
-  constexpr int N = HD / 64;
-  float o[N] = {};
-  const float* p = a.part + at * a.nsplit * HD + lane * N;
+  const float2* ml = a.ml + at * a.nsplit;
+  const float* p = a.part + at * a.nsplit * HD + d;
+  float top = -INFINITY, l = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, ml[s].x);
+  f32x4 o = (f32x4)(0.f);
+#pragma unroll 4
   for (int s = 0; s < a.nsplit; ++s) {
-    const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
-    if (ws != 0.f) {   // (0: a split without a key)
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] += ws * p[(int64_t)s * HD + i];
-    }
+    const float2 x = ml[s];
+    const float w = x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x.x - top);   // (no key: sum 0; nothing but NaN: let it through)
+    l += w * x.y;
+    o += *reinterpret_cast<const f32x4*>(p + (int64_t)s * HD) * w;
   }
-  XT* y = reinterpret_cast<XT*>(a.out) + row * a.out_stride + (int64_t)head * HD + lane * N;
-#pragma unroll
-  for (int i = 0; i < N; ++i) store_kv(y + i, o[i] * inv);
+  store4(reinterpret_cast<XT*>(a.out) + row * a.out_stride + (int64_t)head * HD + d, o * inverse(l));
 }
 
 // ---- entry points -----------------------------------------------------------------------------------------------------------------------
@@ -514,10 +693,11 @@ static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
   a.c = ops_paged(c);
   a.n_q = p->n_q; a.rep = p->n_q / c.n_kv; a.prefix_len = p->prefix_len;
   const int64_t flat = (int64_t)c.rows * a.rep;
+  const int ROWS = tile_rows(p->x_dtype);
   a.per_seq_tiles = (a.rep + ROWS - 1) / ROWS;
   const int64_t own_tiles = c.cu_rows ? flat / ROWS + c.n_seqs : (int64_t)c.n_seqs * a.per_seq_tiles;
-  // sequences that bring half a tile of rows of their own read the prefix with them: nothing to share, nothing to join
-  a.with_prefix = p->prefix_len > 0 && c.cu_rows && c.n_seqs > 0 && flat / c.n_seqs >= ROWS / 2;
+  // sequences that bring two tiles of 16 rows and more of their own read the prefix with them: nothing to share, nothing to join
+  a.with_prefix = p->prefix_len > 0 && c.cu_rows && c.n_seqs > 0 && flat / c.n_seqs >= 32;
   const int64_t np = p->prefix_len && !a.with_prefix ? (flat + ROWS - 1) / ROWS : 0;
   const int64_t own_keys = (int64_t)c.table_width * c.page_size + (a.with_prefix ? p->prefix_len : 0);
   auto splits = [&](int64_t tiles, int64_t keys) {
@@ -553,7 +733,7 @@ static int launch(const AttnOpArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD>), dim3(items), dim3(AT), 0, st, a);
   OPS_HIP(hipGetLastError());
   if (a.nsplit > 1) {
-    const unsigned n = (unsigned)(((int64_t)a.c.rows * a.n_q + 3) / 4);
+    const unsigned n = (unsigned)(((int64_t)a.c.rows * a.n_q * (HD / 4) + AT - 1) / AT);
     hipLaunchKernelGGL((paged_attn_join_kernel<XT, HD>), dim3(n), dim3(AT), 0, st, a);
     OPS_HIP(hipGetLastError());
   }
