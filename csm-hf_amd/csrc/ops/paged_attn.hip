@@ -31,6 +31,7 @@ struct AttnOpArgs {
   const int32_t* prefix;
   int64_t q_stride, out_stride;
   int n_q, rep, prefix_len;
+  uint32_t kp16, ks16, vp16, vs16;   // page and slot strides in 16-byte units: a slot's place inside the cache fits 32 bits up to 64 GB
   float c2;               // |scale| log2(e); the sign of scale is folded into q
   uint32_t q_flip;
   int np_tiles, nsp, no_tiles, nso, per_seq_tiles, with_prefix, nsplit;   // nsplit = partial results per row
@@ -99,20 +100,20 @@ struct Prod<XT, bf16_t, HD> {
       for (int n = 0; n < NQ; ++n) q[n][t] = f[n];
     }
   }
-  // pg[kt], sl[kt]: page (0 where there is none) and slot in it of key 16 kt + lane % 16
-  static __device__ __forceinline__ void load(Tile& t, const bf16_t* kb, const bf16_t* vb, const Paged& c, const int (&pg)[NG], const int (&sl)[NG], int lane) {
-    const int g = lane >> 4;
+  // ko[kt], vo[kt]: place of key 16 kt + lane % 16; kb, vb point at the lane's own piece of a slot
+  static __device__ __forceinline__ int k_piece(int lane) { return 8 * (lane >> 4); }
+  static __device__ __forceinline__ int v_piece(int lane) { return (lane % LPK) * 8; }
+  static __device__ __forceinline__ void load(Tile& t, const char* kb, const char* vb, const uint32_t (&ko)[NG], const uint32_t (&vo)[NG], int lane) {
 #pragma unroll
     for (int kt = 0; kt < NG; ++kt) {
-      const bf16_t* p = kb + pg[kt] * c.kp + sl[kt] * c.ks + 8 * g;
+      const char* p = kb + ((uint64_t)ko[kt] << 4);
 #pragma unroll
-      for (int s = 0; s < T; ++s) t.k[kt][s] = *reinterpret_cast<const u32x4*>(p + 32 * s);
+      for (int s = 0; s < T; ++s) t.k[kt][s] = *reinterpret_cast<const u32x4*>(p + 64 * s);
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int kk = i * KPP, from = (kk & 15) + lane / LPK;   // key kk + lane / LPK of the tile
-      const int page = __shfl(pg[kk >> 4], from), slot = __shfl(sl[kk >> 4], from);
-      t.v[i] = *reinterpret_cast<const u32x4*>(vb + page * c.vp + slot * c.vs + (lane % LPK) * 8);
+    for (int i = 0; i < NV; ++i) {   // key i * KPP + lane / LPK
+      const int kk = i * KPP, from = (kk & 15) + lane / LPK;
+      t.v[i] = *reinterpret_cast<const u32x4*>(vb + ((uint64_t)__shfl(vo[kk >> 4], from) << 4));
     }
   }
   __device__ __forceinline__ void scores(const Tile& t, f32x4 (&s)[NG]) const {
@@ -125,7 +126,8 @@ struct Prod<XT, bf16_t, HD> {
         for (int x = 0; x < T; ++x) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const b16x8*>(&t.k[kt][x]), q[n][x], s[kt], 0, 0, 0);
     }
   }
-  // 16-byte chunk ch of key kk lies at chunk ch ^ (kk & 7): the rows of a transposing read then cover all banks
+  // 16-byte chunk ch of key kk lies at chunk ch ^ (kk & 7): the rows of a transposing read then cover all banks.  Key i * KPP + lane / LPK: only the
+  // KPP part of the key moves the XOR
   static __device__ __forceinline__ void stage_v(const Tile& t, char* lds, int lane, uint32_t valid) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -135,18 +137,20 @@ struct Prod<XT, bf16_t, HD> {
       *reinterpret_cast<u32x4*>(lds + kk * HD * 2 + ((ch ^ (kk & 7)) << 4)) = x;
     }
   }
-  static __device__ __forceinline__ void accumulate(const f32x4 (&p)[NG], char* lds, f32x4 (&o)[HD / 16], int lane) {
-    const int g = lane >> 4, li = lane & 15;
+  // where a lane's transposing reads start: 4 keys from 4 g, columns 16 dt ..; the other columns of the row are an XOR away, keys + 16 a constant
+  static __device__ __forceinline__ int v_place(int lane) {
+    const int g = lane >> 4, li = lane & 15, k0 = 4 * g + (li >> 2);
+    return k0 * HD * 2 + ((((li & 3) >> 1) ^ (k0 & 7)) << 4) + (li & 1) * 8;
+  }
+  static __device__ __forceinline__ void accumulate(const f32x4 (&p)[NG], char* lds, int place, f32x4 (&o)[HD / 16], int) {
     const float x[8] = {p[0][0], p[0][1], p[0][2], p[0][3], p[1][0], p[1][1], p[1][2], p[1][3]};
     b16x8 f[NP];
     split8<NP>(x, f);
-    const int k0 = 4 * g + (li >> 2), k1 = 16 + k0;   // k0 & 7 == k1 & 7
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt) {
-      const int at = (((2 * dt + ((li & 3) >> 1)) ^ (k0 & 7)) << 4) + (li & 1) * 8;
       typedef __attribute__((address_space(3))) b16x4* lp;
-      const b16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + k0 * HD * 2 + at));
-      const b16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + k1 * HD * 2 + at));
+      const b16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + (place ^ (dt << 5))));
+      const b16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + (place ^ (dt << 5)) + 16 * HD * 2));
       const b16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 #pragma unroll
       for (int n = NP - 1; n >= 0; --n) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, f[n], o[dt], 0, 0, 0);
@@ -172,16 +176,14 @@ struct Prod<float, float, HD> {
       for (int e = 0; e < 4; ++e) q[u][e] = __uint_as_float(__float_as_uint(x[e]) ^ flip);
     }
   }
-  static __device__ __forceinline__ void load(Tile& t, const float* kb, const float* vb, const Paged& c, const int (&pg)[NG], const int (&sl)[NG], int lane) {
-    const float* p = kb + pg[0] * c.kp + sl[0] * c.ks + 4 * (lane >> 4);
+  static __device__ __forceinline__ int k_piece(int lane) { return 4 * (lane >> 4); }
+  static __device__ __forceinline__ int v_piece(int lane) { return (lane % LPK) * 4; }
+  static __device__ __forceinline__ void load(Tile& t, const char* kb, const char* vb, const uint32_t (&ko)[NG], const uint32_t (&vo)[NG], int lane) {
+    const char* p = kb + ((uint64_t)ko[0] << 4);
 #pragma unroll
-    for (int u = 0; u < U; ++u) t.k[0][u] = *reinterpret_cast<const f32x4*>(p + 16 * u);
+    for (int u = 0; u < U; ++u) t.k[0][u] = *reinterpret_cast<const f32x4*>(p + 64 * u);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int from = i * KPP + lane / LPK;
-      const int page = __shfl(pg[0], from), slot = __shfl(sl[0], from);
-      t.v[i] = *reinterpret_cast<const f32x4*>(vb + page * c.vp + slot * c.vs + (lane % LPK) * 4);
-    }
+    for (int i = 0; i < NV; ++i) t.v[i] = *reinterpret_cast<const f32x4*>(vb + ((uint64_t)__shfl(vo[0], i * KPP + lane / LPK) << 4));
   }
   __device__ __forceinline__ void scores(const Tile& t, f32x4 (&s)[NG]) const {
     f32x4 a = (f32x4)(0.f);
@@ -200,8 +202,9 @@ struct Prod<float, float, HD> {
       *reinterpret_cast<f32x4*>(lds + (kk * LD + (lane % LPK) * 4) * 4) = x;
     }
   }
-  static __device__ __forceinline__ void accumulate(const f32x4 (&p)[NG], char* lds, f32x4 (&o)[HD / 16], int lane) {
-    const float* v = reinterpret_cast<const float*>(lds) + 4 * (lane >> 4) * LD + (lane & 15);
+  static __device__ __forceinline__ int v_place(int lane) { return 4 * (lane >> 4) * LD + (lane & 15); }
+  static __device__ __forceinline__ void accumulate(const f32x4 (&p)[NG], char* lds, int place, f32x4 (&o)[HD / 16], int) {
+    const float* v = reinterpret_cast<const float*>(lds) + place;
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt)
 #pragma unroll
@@ -213,12 +216,16 @@ struct Prod<float, float, HD> {
 struct KeyAxis {
   const int32_t *prefix, *own;
   int prefix_len;
-  __device__ __forceinline__ int page(int j, const Paged& c) const {   // of axis position j, -1 where it does not exist
-    const int s = j < prefix_len ? j : j - prefix_len;
-    const int p = (j < prefix_len ? prefix : own)[s >> c.shift];
-    return (unsigned)p < (unsigned)c.n_pages ? p : -1;
+  // page and slot of axis position j, false where the page does not exist (then page 0, which does: callers have n_pages >= 1)
+  __device__ __forceinline__ bool at(int j, const Paged& c, uint32_t& page, uint32_t& slot) const {
+    const bool p = j < prefix_len;
+    const uint32_t s = j - (p ? 0 : prefix_len);
+    page = (uint32_t)(p ? prefix : own)[s >> c.shift];
+    slot = s & ((1u << c.shift) - 1);
+    const bool ok = page < (uint32_t)c.n_pages;
+    page = ok ? page : 0;
+    return ok;
   }
-  __device__ __forceinline__ int slot(int j, const Paged& c) const { return (j < prefix_len ? j : j - prefix_len) & ((1 << c.shift) - 1); }
 };
 
 template <typename XT, typename CT, int HD>
@@ -227,39 +234,44 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const Prod<XT, 
   using P = Prod<XT, CT, HD>;
   constexpr int NG = P::NG, KT = 16 * NG;
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-  const CT* kb = reinterpret_cast<const CT*>(a.k) + kvh * a.c.kh;
-  const CT* vb = reinterpret_cast<const CT*>(a.v) + kvh * a.c.vh;
+  const char* kb = reinterpret_cast<const char*>(reinterpret_cast<const CT*>(a.k) + kvh * a.c.kh + P::k_piece(lane));
+  const char* vb = reinterpret_cast<const char*>(reinterpret_cast<const CT*>(a.v) + kvh * a.c.vh + P::v_piece(lane));
+  const int place = P::v_place(lane);
   m = -INFINITY; l = 0.f;
 #pragma unroll
   for (int i = 0; i < HD / 16; ++i) o[i] = (f32x4)(0.f);
 
-  auto look = [&](int j0, int (&pg)[NG], int (&sl)[NG]) {
+  uint32_t pg[NG], sl[NG];
+  uint64_t there[NG];
+  auto look = [&](int j0) {
 #pragma unroll
     for (int kt = 0; kt < NG; ++kt) {
       const int j = j0 + 16 * kt + li;
-      pg[kt] = j < k1 ? ax.page(j, a.c) : -1;
-      sl[kt] = j < k1 ? ax.slot(j, a.c) : 0;
+      pg[kt] = sl[kt] = 0;
+      bool ok = false;
+      if (j < k1) ok = ax.at(j, a.c, pg[kt], sl[kt]);
+      there[kt] = __ballot(ok);
     }
   };
-  auto fetch = [&](typename P::Tile& t, const int (&pg)[NG], const int (&sl)[NG], uint32_t& valid) {
-    int safe[NG];
+  auto fetch = [&](typename P::Tile& t, uint32_t& valid) {
+    uint32_t ko[NG], vo[NG];
     valid = 0;
 #pragma unroll
     for (int kt = 0; kt < NG; ++kt) {
-      valid |= ((uint32_t)__ballot(pg[kt] >= 0) & 0xffffu) << (16 * kt);
-      safe[kt] = pg[kt] < 0 ? 0 : pg[kt];   // page 0 exists: n_pages >= 1 here
+      valid |= ((uint32_t)there[kt] & 0xffffu) << (16 * kt);
+      ko[kt] = pg[kt] * a.kp16 + sl[kt] * a.ks16;
+      vo[kt] = pg[kt] * a.vp16 + sl[kt] * a.vs16;
     }
-    P::load(t, kb, vb, a.c, safe, sl, lane);
+    P::load(t, kb, vb, ko, vo, lane);
   };
   int j = k0 + first * KT;
   const int hop = step * KT;
   if (j >= k1) return;
   typename P::Tile t;
   uint32_t valid;
-  int pg[NG], sl[NG];
-  look(j, pg, sl);
-  fetch(t, pg, sl, valid);
-  look(j + hop, pg, sl);
+  look(j);
+  fetch(t, valid);
+  look(j + hop);
   for (; j < k1; j += hop) {
     constexpr uint32_t ALL = NG == 2 ? 0xffffffffu : 0xffffu;
     f32x4 s[NG];
@@ -275,8 +287,8 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const Prod<XT, 
         }
     }
     if (j + hop < k1) {   // the tile's registers are free: the next one is in flight behind the softmax and the second product
-      fetch(t, pg, sl, valid);
-      look(j + 2 * hop, pg, sl);
+      fetch(t, valid);
+      look(j + 2 * hop);
     }
     float top = s[0][0];
 #pragma unroll
@@ -300,7 +312,7 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const Prod<XT, 
         s[kt][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[kt][e], a.c2, -ref));
         l += s[kt][e];
       }
-    P::accumulate(s, lds, o, lane);
+    P::accumulate(s, lds, place, o, lane);
   }
   l = xor32_sum(xor16_sum(l));
 }
@@ -319,8 +331,9 @@ struct Wide {
 
   __device__ __forceinline__ void run(const AttnOpArgs& a, const KeyAxis& ax, int kvh, int k0, int k1, const int (&lim)[RT], const int (&lim_min)[RT], int n_rt, char* lds) {
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g = lane >> 4;
-    const bf16_t* kb = reinterpret_cast<const bf16_t*>(a.k) + kvh * a.c.kh;
-    const bf16_t* vb = reinterpret_cast<const bf16_t*>(a.v) + kvh * a.c.vh;
+    const int ch = tid % CH, key0 = tid / CH;
+    const char* kb = reinterpret_cast<const char*>(reinterpret_cast<const bf16_t*>(a.k) + kvh * a.c.kh + ch * 8);
+    const char* vb = reinterpret_cast<const char*>(reinterpret_cast<const bf16_t*>(a.v) + kvh * a.c.vh + ch * 8);
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       m[r] = -INFINITY;
@@ -330,22 +343,36 @@ struct Wide {
     }
     if (k0 >= k1) return;
     // every wave looks up the pages of a tile's 64 keys, lane = key; a thread stages chunk tid % CH of keys i * KPP + tid / CH
-    auto look = [&](int j0) { const int j = j0 + lane; return j < k1 ? ax.page(j, a.c) : -1; };
+    uint32_t page = 0, slot = 0;
+    uint64_t there = 0;
+    auto look = [&](int j0) {
+      const int j = j0 + lane;
+      page = slot = 0;
+      bool ok = false;
+      if (j < k1) ok = ax.at(j, a.c, page, slot);
+      there = __ballot(ok);
+    };
     u32x4 kr[NL], vr[NL];
-    const int ch = tid % CH, key0 = tid / CH;
-    auto fetch = [&](int j0, int page) -> uint64_t {
-      const uint64_t valid = __ballot(page >= 0);
+    auto fetch = [&]() {
+      const uint32_t ko = page * a.kp16 + slot * a.ks16, vo = page * a.vp16 + slot * a.vs16;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int kk = i * KPP + key0;
-        const int pg = max(__shfl(page, kk), 0), sl = ax.slot(min(j0 + kk, k1 - 1), a.c);
-        kr[i] = *reinterpret_cast<const u32x4*>(kb + pg * a.c.kp + sl * a.c.ks + ch * 8);
-        vr[i] = *reinterpret_cast<const u32x4*>(vb + pg * a.c.vp + sl * a.c.vs + ch * 8);
+        kr[i] = *reinterpret_cast<const u32x4*>(kb + ((uint64_t)__shfl(ko, i * KPP + key0) << 4));
+        vr[i] = *reinterpret_cast<const u32x4*>(vb + ((uint64_t)__shfl(vo, i * KPP + key0) << 4));
       }
-      return valid;
+      return there;
     };
-    uint64_t valid = fetch(k0, look(k0));
-    int page = look(k0 + KEYS);
+    look(k0);
+    uint64_t valid = fetch();
+    look(k0 + KEYS);
+    // LDS places of this lane: what it stages (keys KPP apart), its K operands (16-key tiles and 32-element steps apart), its V columns
+    int st[NL], kp[T], vp[HD / 16];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) st[i] = (i * KPP + key0) * HD * 2 + ((ch ^ ((i * KPP + key0) & 7)) << 4);
+#pragma unroll
+    for (int x = 0; x < T; ++x) kp[x] = li * HD * 2 + (((4 * x + g) ^ (li & 7)) << 4);
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) vp[dt] = Prod<XT, bf16_t, HD>::v_place(lane) ^ (dt << 5);
     const b16x8 ones = (b16x8)((short)0x3f80);
     int buf = 0;
     for (int j = k0; j < k1; j += KEYS, buf ^= 1) {
@@ -353,16 +380,15 @@ struct Wide {
       char* const vs = ks + TILE;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int kk = i * KPP + key0, at = kk * HD * 2 + ((ch ^ (kk & 7)) << 4);
-        if (valid != ~0ull && !((valid >> kk) & 1)) vr[i] = (u32x4)(0u);   // 0 * (what an unused slot holds) must be 0
-        *reinterpret_cast<u32x4*>(ks + at) = kr[i];
-        *reinterpret_cast<u32x4*>(vs + at) = vr[i];
+        if (valid != ~0ull && !((valid >> (i * KPP + key0)) & 1)) vr[i] = (u32x4)(0u);   // 0 * (what an unused slot holds) must be 0
+        *reinterpret_cast<u32x4*>(ks + st[i]) = kr[i];
+        *reinterpret_cast<u32x4*>(vs + st[i]) = vr[i];
       }
       __syncthreads();   // (one per tile: a buffer is written again only two tiles later)
       const uint64_t now = valid;
       if (j + KEYS < k1) {
-        valid = fetch(j + KEYS, page);
-        page = look(j + 2 * KEYS);
+        valid = fetch();
+        look(j + 2 * KEYS);
       }
       if (n_rt == 0) continue;
       f32x4 s[RT][4];
@@ -370,7 +396,7 @@ struct Wide {
       for (int kt = 0; kt < 4; ++kt) {
         b16x8 k[T];
 #pragma unroll
-        for (int x = 0; x < T; ++x) k[x] = *reinterpret_cast<const b16x8*>(ks + (16 * kt + li) * HD * 2 + (((4 * x + g) ^ (li & 7)) << 4));
+        for (int x = 0; x < T; ++x) k[x] = *reinterpret_cast<const b16x8*>(ks + kp[x] + 16 * kt * HD * 2);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           if (r && n_rt < 2) break;
@@ -424,10 +450,9 @@ struct Wide {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int dt = 0; dt < HD / 16; ++dt) {
-          const int kk = 32 * h + 4 * g + (li >> 2), at = (((2 * dt + ((li & 3) >> 1)) ^ (kk & 7)) << 4) + (li & 1) * 8;
           typedef __attribute__((address_space(3))) b16x4* lp;
-          const b16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + kk * HD * 2 + at));
-          const b16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + (kk + 16) * HD * 2 + at));
+          const b16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + vp[dt] + 32 * h * HD * 2));
+          const b16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + vp[dt] + (32 * h + 16) * HD * 2));
           const b16x8 v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
@@ -639,30 +664,40 @@ __global__ __launch_bounds__(AT, 2) void paged_attn_kernel(AttnOpArgs a) {
   if (row_live) put<XT, HD>(a, row, head, slot0 + split, g, o, m, l);
 }
 
-// join the partial results: a thread per 4 elements of a (row, head)
+// join the partial results of a (row, head): one wave, its halves on alternate splits, lane = split for the weights
 template <typename XT, int HD>
 __global__ __launch_bounds__(AT) void paged_attn_join_kernel(AttnOpArgs a) {
   const Paged& c = a.c;
-  constexpr int PER = HD / 4;
-  const int64_t i = (int64_t)blockIdx.x * AT + threadIdx.x, at = i / PER;
-  const int d = (int)(i % PER) * 4;
+  constexpr int N = HD / 32;
+  typedef __attribute__((ext_vector_type(N))) float vec;
+  const int lane = threadIdx.x & 63, d = (lane & 31) * N;
+  const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (at >= (int64_t)c.rows * a.n_q) return;
   const int row = (int)(at / a.n_q), head = (int)(at - (int64_t)row * a.n_q);
   const int seq = c.cu ? ops_find_seq(c.cu, c.n_seqs, row) : row;
   if (seq < 0 || c.lens[seq] < 0) return;
-  const float2* ml = a.ml + at * a.nsplit;
+  const float2 x = lane < a.nsplit ? a.ml[at * a.nsplit + lane] : make_float2(-INFINITY, 0.f);
+  const float top = wave_max(x.x);
+  const float w = x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x.x - top);   // (no key: sum 0; nothing but NaN: let it through)
+  const float inv = inverse(wave_sum(w * x.y));
   const float* p = a.part + at * a.nsplit * HD + d;
-  float top = -INFINITY, l = 0.f;
-  for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, ml[s].x);
-  f32x4 o = (f32x4)(0.f);
+  vec o = (vec)(0.f);
 #pragma unroll 4
-  for (int s = 0; s < a.nsplit; ++s) {
-    const float2 x = ml[s];
-    const float w = x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x.x - top);   // (no key: sum 0; nothing but NaN: let it through)
-    l += w * x.y;
-    o += *reinterpret_cast<const f32x4*>(p + (int64_t)s * HD) * w;
+  for (int s0 = 0; s0 < a.nsplit; s0 += 2) {
+    const int s = min(s0 + (lane >> 5), a.nsplit - 1);
+    const float lo = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s0));
+    const float hi = s0 + 1 < a.nsplit ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s0 + 1)) : 0.f;
+    const float ws = lane < 32 ? lo : hi;
+    const vec v = *reinterpret_cast<const vec*>(p + (int64_t)s * HD);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] += ws * v[i];
   }
-  store4(reinterpret_cast<XT*>(a.out) + row * a.out_stride + (int64_t)head * HD + d, o * inverse(l));
+  XT* y = reinterpret_cast<XT*>(a.out) + row * a.out_stride + (int64_t)head * HD + d;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float t = xor32_sum(o[i]) * inv;
+    if (lane < 32) store_kv(y + i, t);
+  }
 }
 
 // ---- entry points -----------------------------------------------------------------------------------------------------------------------
@@ -678,6 +713,9 @@ static int check(const csm_ops_attention_t* p) {
   if ((int64_t)p->prefix_pages * c.page_size < p->prefix_len) return ops_fail(CSM_OPS_ERR_ARG, "%d pages of %d slots do not hold a prefix of %d", p->prefix_pages, c.page_size, p->prefix_len);
   if ((int64_t)c.table_width * c.page_size + p->prefix_len > 0x7fff0000) return ops_fail(CSM_OPS_ERR_CAPACITY, "more than 2^31 slots");
   if ((int64_t)c.rows * p->n_q > (1 << 28) || c.n_seqs > (1 << 28)) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
+  const int64_t unit = c.dtype == CSM_OPS_BF16 ? 8 : 4, most_k = (c.n_pages - 1) * c.k_page_stride + (c.page_size - 1) * c.k_slot_stride,
+                most_v = (c.n_pages - 1) * c.v_page_stride + (c.page_size - 1) * c.v_slot_stride;
+  if (c.n_pages && (most_k / unit > 0xffffffffll || most_v / unit > 0xffffffffll)) return ops_fail(CSM_OPS_ERR_CAPACITY, "a cache of more than 64 GB");
   if (!isfinite(p->scale)) return ops_fail(CSM_OPS_ERR_ARG, "scale must be finite");
   if (!c.rows) return 0;
   if (!p->q || !p->out || (p->prefix_len && !p->prefix_table)) return ops_fail(CSM_OPS_ERR_ARG, "null pointer");
@@ -696,17 +734,23 @@ static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
   const int ROWS = tile_rows(p->x_dtype);
   a.per_seq_tiles = (a.rep + ROWS - 1) / ROWS;
   const int64_t own_tiles = c.cu_rows ? flat / ROWS + c.n_seqs : (int64_t)c.n_seqs * a.per_seq_tiles;
-  // sequences that bring two tiles of 16 rows and more of their own read the prefix with them: nothing to share, nothing to join
-  a.with_prefix = p->prefix_len > 0 && c.cu_rows && c.n_seqs > 0 && flat / c.n_seqs >= 32;
+  const int64_t own_cap = (int64_t)c.table_width * c.page_size;
+  // the prefix goes with each sequence's own slots (read once per sequence, nothing to join) where sequences bring two tiles of 16 rows and more of their
+  // own, and where the whole axis is short: then it is a few iterations from L2, and a second launch would cost more than sharing it saves
+  const bool short_axis = p->prefix_len + own_cap <= 256;
+  a.with_prefix = p->prefix_len > 0 && (short_axis || (c.cu_rows && c.n_seqs > 0 && flat / c.n_seqs >= 32));
   const int64_t np = p->prefix_len && !a.with_prefix ? (flat + ROWS - 1) / ROWS : 0;
-  const int64_t own_keys = (int64_t)c.table_width * c.page_size + (a.with_prefix ? p->prefix_len : 0);
-  auto splits = [&](int64_t tiles, int64_t keys) {
-    const int64_t want = 1024 / (tiles * c.n_kv < 1 ? 1 : tiles * c.n_kv), most = (keys + 127) / 128;
-    int64_t n = want < most ? want : most;
+  const int64_t own_keys = own_cap + (a.with_prefix ? p->prefix_len : 0);
+  auto splits = [](int64_t items, int64_t keys, int64_t fill, int64_t more) {   // `fill` items of 128 keys and more, `more` of 256 and more
+    if (items < 1) items = 1;
+    const int64_t a = fill / items < (keys + 127) / 128 ? fill / items : (keys + 127) / 128;
+    const int64_t b = more / items < (keys + 255) / 256 ? more / items : (keys + 255) / 256;
+    const int64_t n = a > b ? a : b;
     return (int)(n < 1 ? 1 : n > MAX_SPLIT / 2 ? MAX_SPLIT / 2 : n);
   };
-  a.nsp = np ? splits(np, p->prefix_len) : 0;
-  a.nso = splits(own_tiles, own_keys);
+  const bool narrow = c.n_seqs > 0 && flat / c.n_seqs <= 16;   // such items wait for memory and are cheap to cut; a tile of many rows has much to join
+  a.nsp = np ? splits(np * c.n_kv, p->prefix_len, 256, 0) : 0;
+  a.nso = short_axis && a.with_prefix ? 1 : splits(own_tiles * c.n_kv, own_keys, 512, narrow ? 2048 : 0);
   a.np_tiles = (int)np; a.no_tiles = (int)own_tiles; a.nsplit = a.nsp + a.nso;
   if (((int64_t)a.np_tiles * a.nsp + (int64_t)a.no_tiles * a.nso) * c.n_kv > 0x7fffffff) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
   return 0;
@@ -733,7 +777,7 @@ static int launch(const AttnOpArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD>), dim3(items), dim3(AT), 0, st, a);
   OPS_HIP(hipGetLastError());
   if (a.nsplit > 1) {
-    const unsigned n = (unsigned)(((int64_t)a.c.rows * a.n_q * (HD / 4) + AT - 1) / AT);
+    const unsigned n = (unsigned)(((int64_t)a.c.rows * a.n_q + 3) / 4);
     hipLaunchKernelGGL((paged_attn_join_kernel<XT, HD>), dim3(n), dim3(AT), 0, st, a);
     OPS_HIP(hipGetLastError());
   }
@@ -750,6 +794,9 @@ extern "C" int csm_ops_paged_prefix_attention(const csm_ops_attention_t* p, void
   if (need && (!p->workspace || p->workspace_bytes < need || !ops_aligned(p->workspace)))
     return ops_fail(CSM_OPS_ERR_CAPACITY, "workspace of %zu bytes: %zu on 16 bytes are needed", p->workspace_bytes, need);
   a.q = p->q; a.k = c.k; a.v = c.v; a.out = p->out; a.prefix = p->prefix_table; a.q_stride = p->q_stride; a.out_stride = p->out_stride;
+  const int unit = c.dtype == CSM_OPS_BF16 ? 8 : 4;
+  a.kp16 = (uint32_t)(c.k_page_stride / unit); a.ks16 = (uint32_t)(c.k_slot_stride / unit);
+  a.vp16 = (uint32_t)(c.v_page_stride / unit); a.vs16 = (uint32_t)(c.v_slot_stride / unit);
   a.part = reinterpret_cast<float*>(p->workspace);
   a.ml = need ? reinterpret_cast<float2*>(a.part + (size_t)c.rows * p->n_q * a.nsplit * c.head_dim) : nullptr;
   a.q_flip = p->scale < 0.f ? 0x80000000u : 0u;

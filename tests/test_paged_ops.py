@@ -471,9 +471,12 @@ def test_attention_and_append_past_32_bit_offsets():
     k[-1], v[-1] = small.k[0], small.v[0]
     table = torch.tensor([[n_pages - 1]], dtype=torch.int32, device=DEV)
     q = torch.randn(1, 4, 64, device=DEV).bfloat16()
-    assert torch.equal(paged_prefix_attention(q, k, v, table, small.lens), paged_prefix_attention(q, *small.args()))
-    assert torch.equal(paged_prefix_attention(q, k, v, table, small.lens, prefix_table=table[0], prefix_len=70),
-                       paged_prefix_attention(q, *small.args(), prefix_table=small.table[0, :1].contiguous(), prefix_len=70))
+    # (against the 64-bit result: how the work is cut, and with it the order of sums, goes by the table's width)
+    want, tol = attention64(q, small, [100], [1], 4, 0.125, True)
+    check(paged_prefix_attention(q, k, v, table, small.lens), want, tol, 0.0)
+    small.prefix, small.prefix_len = small.table[0, :1], 70
+    want, tol = attention64(q, small, [100], [1], 4, 0.125, True)
+    check(paged_prefix_attention(q, k, v, table, small.lens, prefix_table=table[0], prefix_len=70), want, tol, 0.0)
     qkv, tab = torch.randn(1, 8 * 64, device=DEV).bfloat16(), torch.rand(128, 32, device=DEV)
     paged_rope_append(qkv, tab, tab, k, v, table, small.lens)
     paged_rope_append(qkv, tab, tab, *small.args())
