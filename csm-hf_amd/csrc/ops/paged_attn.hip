@@ -216,15 +216,13 @@ struct Prod<float, float, HD> {
 struct KeyAxis {
   const int32_t *prefix, *own;
   int prefix_len;
-  // page and slot of axis position j, false where the page does not exist (then page 0, which does: callers have n_pages >= 1)
-  __device__ __forceinline__ bool at(int j, const Paged& c, uint32_t& page, uint32_t& slot) const {
+  // the table entry that names axis position j's page, and its slot there.  The entry is only looked at when the tile is fetched, a tile later:
+  // loads return in order, so a wait for it here would wait for every K and V load in flight
+  __device__ __forceinline__ uint32_t entry(int j, const Paged& c, uint32_t& slot) const {
     const bool p = j < prefix_len;
     const uint32_t s = j - (p ? 0 : prefix_len);
-    page = (uint32_t)(p ? prefix : own)[s >> c.shift];
     slot = s & ((1u << c.shift) - 1);
-    const bool ok = page < (uint32_t)c.n_pages;
-    page = ok ? page : 0;
-    return ok;
+    return (uint32_t)(p ? prefix : own)[s >> c.shift];
   }
 };
 
@@ -242,15 +240,13 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const Prod<XT, 
   for (int i = 0; i < HD / 16; ++i) o[i] = (f32x4)(0.f);
 
   uint32_t pg[NG], sl[NG];
-  uint64_t there[NG];
   auto look = [&](int j0) {
 #pragma unroll
     for (int kt = 0; kt < NG; ++kt) {
       const int j = j0 + 16 * kt + li;
-      pg[kt] = sl[kt] = 0;
-      bool ok = false;
-      if (j < k1) ok = ax.at(j, a.c, pg[kt], sl[kt]);
-      there[kt] = __ballot(ok);
+      pg[kt] = ~0u;
+      sl[kt] = 0;
+      if (j < k1) pg[kt] = ax.entry(j, a.c, sl[kt]);
     }
   };
   auto fetch = [&](typename P::Tile& t, uint32_t& valid) {
@@ -258,9 +254,11 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const Prod<XT, 
     valid = 0;
 #pragma unroll
     for (int kt = 0; kt < NG; ++kt) {
-      valid |= ((uint32_t)there[kt] & 0xffffu) << (16 * kt);
-      ko[kt] = pg[kt] * a.kp16 + sl[kt] * a.ks16;
-      vo[kt] = pg[kt] * a.vp16 + sl[kt] * a.vs16;
+      const bool ok = pg[kt] < (uint32_t)a.c.n_pages;
+      const uint32_t page = ok ? pg[kt] : 0;   // page 0 exists: callers have n_pages >= 1
+      valid |= ((uint32_t)__ballot(ok) & 0xffffu) << (16 * kt);
+      ko[kt] = page * a.kp16 + sl[kt] * a.ks16;
+      vo[kt] = page * a.vp16 + sl[kt] * a.vs16;
     }
     P::load(t, kb, vb, ko, vo, lane);
   };
@@ -343,24 +341,23 @@ struct Wide {
     }
     if (k0 >= k1) return;
     // every wave looks up the pages of a tile's 64 keys, lane = key; a thread stages chunk tid % CH of keys i * KPP + tid / CH
-    uint32_t page = 0, slot = 0;
-    uint64_t there = 0;
+    uint32_t entry = 0, slot = 0;
     auto look = [&](int j0) {
       const int j = j0 + lane;
-      page = slot = 0;
-      bool ok = false;
-      if (j < k1) ok = ax.at(j, a.c, page, slot);
-      there = __ballot(ok);
+      entry = ~0u;
+      slot = 0;
+      if (j < k1) entry = ax.entry(j, a.c, slot);
     };
     u32x4 kr[NL], vr[NL];
-    auto fetch = [&]() {
-      const uint32_t ko = page * a.kp16 + slot * a.ks16, vo = page * a.vp16 + slot * a.vs16;
+    auto fetch = [&]() -> uint64_t {
+      const bool ok = entry < (uint32_t)a.c.n_pages;
+      const uint32_t page = ok ? entry : 0, ko = page * a.kp16 + slot * a.ks16, vo = page * a.vp16 + slot * a.vs16;   // (page 0 exists)
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         kr[i] = *reinterpret_cast<const u32x4*>(kb + ((uint64_t)__shfl(ko, i * KPP + key0) << 4));
         vr[i] = *reinterpret_cast<const u32x4*>(vb + ((uint64_t)__shfl(vo, i * KPP + key0) << 4));
       }
-      return there;
+      return __ballot(ok);
     };
     look(k0);
     uint64_t valid = fetch();
@@ -373,7 +370,6 @@ struct Wide {
     for (int x = 0; x < T; ++x) kp[x] = li * HD * 2 + (((4 * x + g) ^ (li & 7)) << 4);
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt) vp[dt] = Prod<XT, bf16_t, HD>::v_place(lane) ^ (dt << 5);
-    const b16x8 ones = (b16x8)((short)0x3f80);
     int buf = 0;
     for (int j = k0; j < k1; j += KEYS, buf ^= 1) {
       char* const ks = lds + buf * 2 * TILE;
@@ -390,78 +386,84 @@ struct Wide {
         valid = fetch();
         look(j + 2 * KEYS);
       }
-      if (n_rt == 0) continue;
-      f32x4 s[RT][4];
+      if (n_rt) tile(a, ks, vs, kp, vp, now, j, g, lim, lim_min, n_rt);
+    }
+  }
+
+  // one staged tile for the wave's first n_rt row tiles.  (A branch per product of the second one, not a copy without it: the copy let the scheduler hold
+  // 30 registers more, and two waves per SIMD instead of three took 10 percent longer)
+  __device__ __forceinline__ void tile(const AttnOpArgs& a, const char* ks, char* vs, const int (&kp)[T], const int (&vp)[HD / 16], uint64_t now, int j, int g, const int (&lim)[RT], const int (&lim_min)[RT], int n_rt) {
+    const b16x8 ones = (b16x8)((short)0x3f80);
+    f32x4 s[RT][4];
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        b16x8 k[T];
+    for (int kt = 0; kt < 4; ++kt) {
+      b16x8 k[T];
 #pragma unroll
-        for (int x = 0; x < T; ++x) k[x] = *reinterpret_cast<const b16x8*>(ks + kp[x] + 16 * kt * HD * 2);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          if (r && n_rt < 2) break;
-          s[r][kt] = (f32x4)(0.f);
-#pragma unroll
-          for (int n = NQ - 1; n >= 0; --n)
-#pragma unroll
-            for (int x = 0; x < T; ++x) s[r][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[x], q[r][n][x], s[r][kt], 0, 0, 0);
-        }
-      }
-      b16x8 p[RT][2][NP];
+      for (int x = 0; x < T; ++x) k[x] = *reinterpret_cast<const b16x8*>(ks + kp[x] + 16 * kt * HD * 2);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         if (r && n_rt < 2) break;
-        if (now != ~0ull || j + KEYS > lim_min[r]) {
-          const uint64_t seen = now >> (4 * g);
-          const int left = lim[r] - j - 4 * g;
+        s[r][kt] = (f32x4)(0.f);
 #pragma unroll
-          for (int kt = 0; kt < 4; ++kt)
+        for (int n = NQ - 1; n >= 0; --n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[r][kt][e] = ((seen >> (16 * kt + e)) & 1) && 16 * kt + e < left ? s[r][kt][e] : -INFINITY;
-        }
-        float top = s[r][0][0];
+          for (int x = 0; x < T; ++x) s[r][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[x], q[r][n][x], s[r][kt], 0, 0, 0);
+      }
+    }
+    b16x8 p[RT][2][NP];
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[r][kt][e]);
-        top *= a.c2;
-        if (__any(top > m[r] + SLACK)) {
-          top = xor32_max(xor16_max(top));
-          const float m_new = fmaxf(m[r], top), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - m_new);
-          l4[r] *= alpha;
-#pragma unroll
-          for (int i = 0; i < HD / 16; ++i) o[r][i] *= alpha;
-          m[r] = m_new;
-        }
-        const float ref = m[r] == -INFINITY ? 0.f : m[r];
+    for (int r = 0; r < RT; ++r) {
+      if (r && n_rt < 2) break;
+      if (now != ~0ull || j + KEYS > lim_min[r]) {
+        const uint64_t seen = now >> (4 * g);
+        const int left = lim[r] - j - 4 * g;
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[r][kt][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[r][kt][e], a.c2, -ref));
+          for (int e = 0; e < 4; ++e) s[r][kt][e] = ((seen >> (16 * kt + e)) & 1) && 16 * kt + e < left ? s[r][kt][e] : -INFINITY;
+      }
+      float top = s[r][0][0];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float x[8] = {s[r][2 * h][0], s[r][2 * h][1], s[r][2 * h][2], s[r][2 * h][3], s[r][2 * h + 1][0], s[r][2 * h + 1][1], s[r][2 * h + 1][2], s[r][2 * h + 1][3]};
-          split8<NP>(x, p[r][h]);
+      for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-          for (int n = NP - 1; n >= 0; --n) l4[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][h][n], l4[r], 0, 0, 0);
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[r][kt][e]);
+      top *= a.c2;
+      if (__any(top > m[r] + SLACK)) {
+        top = xor32_max(xor16_max(top));
+        const float m_new = fmaxf(m[r], top), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - m_new);
+        l4[r] *= alpha;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) o[r][i] *= alpha;
+        m[r] = m_new;
+      }
+      const float ref = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r][kt][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[r][kt][e], a.c2, -ref));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x[8] = {s[r][2 * h][0], s[r][2 * h][1], s[r][2 * h][2], s[r][2 * h][3], s[r][2 * h + 1][0], s[r][2 * h + 1][1], s[r][2 * h + 1][2], s[r][2 * h + 1][3]};
+        split8<NP>(x, p[r][h]);
+#pragma unroll
+        for (int n = NP - 1; n >= 0; --n) l4[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][h][n], l4[r], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int dt = 0; dt < HD / 16; ++dt) {
+        typedef __attribute__((address_space(3))) b16x4* lp;
+        const b16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + vp[dt] + 32 * h * HD * 2));
+        const b16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + vp[dt] + (32 * h + 16) * HD * 2));
+        const b16x8 v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          if (r && n_rt < 2) break;
+#pragma unroll
+          for (int n = NP - 1; n >= 0; --n) o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[r][h][n], o[r][dt], 0, 0, 0);
         }
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int dt = 0; dt < HD / 16; ++dt) {
-          typedef __attribute__((address_space(3))) b16x4* lp;
-          const b16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + vp[dt] + 32 * h * HD * 2));
-          const b16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + vp[dt] + (32 * h + 16) * HD * 2));
-          const b16x8 v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            if (r && n_rt < 2) break;
-#pragma unroll
-            for (int n = NP - 1; n >= 0; --n) o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[r][h][n], o[r][dt], 0, 0, 0);
-          }
-        }
-    }
   }
 };
 
