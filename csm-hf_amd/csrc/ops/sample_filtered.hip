@@ -4,9 +4,9 @@
 // Sums are uint64 fixed point (w scaled by 2^min(62 - ceil log2 V, 51)) of weights computed in fp64: exact integer additions, so neither the
 // split over threads nor any order of arrival changes a result, and what is rounded away per weight is below 2^-45 of the largest.
 //
-// No sort: a cut is found by narrowing an interval of order keys (count and mass at or above a probe, one block sum per step; the probe
-// alternates between the middle VALUE, which a smooth row needs few of, and the middle KEY, which bounds any row) until at most 32 entries or
-// one single key are left, which a wave then ranks exactly.
+// No sort of the row: a histogram over its values (counts and masses, a few bins per thread, LDS atomics on integers) is summed from the top, the bin in
+// which a cut falls is gathered (at most 64 entries) and ranked exactly by one wave.  Rows whose values crowd in one bin go the long way:
+// an interval of order keys is narrowed by false position and bisection, one block sum per step, until 64 entries or one single key are left.
 //   V <= 16 384: one workgroup, the row in registers (4 or 16 consecutive entries per thread), read once.  Such a launch is a chain of dependent
 //                steps over code that runs once, so its loops carry no branches and its sums stay on the DPP path.  A top-k of at most 64 narrows
 //                the row to 64 entries at once, and one wave does the rest without a barrier.
@@ -137,7 +137,21 @@ struct Block {
     sum<false>(wave_cnt, none);
     return wave_cnt;
   }
-  // sum over the threads before this one, and over all
+  // sums over the threads before this one, and over all
+  __device__ __forceinline__ void before2(uint32_t& c, uint64_t& m, uint32_t& all_c, uint64_t& all_m) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const uint32_t x = wave_upto(c);
+    const uint64_t y = wave_upto(m);
+    const int g = gen ^= 1;
+    if (lane == 63) { r->c[g][wave] = x; r->m[g][wave] = y; }
+    __syncthreads();
+    const uint32_t wc = r->c[g][lane % W];
+    const uint64_t wm = r->m[g][lane % W];
+    all_c = lane_value(over_waves<W>(wc), 0);
+    all_m = lane_value(over_waves<W>(wm), 0);
+    c = lane_value(over_waves<W>(lane % W < wave ? wc : 0u), 0) + x - c;
+    m = lane_value(over_waves<W>(lane % W < wave ? wm : (uint64_t)0), 0) + y - m;
+  }
   template <typename T>
   __device__ __forceinline__ T before(T v, T& total) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -205,6 +219,23 @@ struct Interval {
 };
 __device__ __forceinline__ float log_count(uint32_t n) { return __log2f(fmaxf((float)n, 0.5f)); }
 
+// The exact cut among the gathered entries, above which lie `above` entries of mass `mass`; every wave does it for itself.  kept: the mass that stays
+template <typename K, bool MASS>
+__device__ __forceinline__ void rank_few(Few* few, const Weigh& weigh, uint32_t above, uint64_t mass, uint32_t want_n, double want_m, Cut& cut, uint64_t& kept) {
+  const int lane = threadIdx.x & 63, n = min(few->n, 64);
+  uint32_t key = lane < n ? few->key[lane] : 0;
+  wave_sort(key);
+  const uint64_t upto = mass + wave_upto(lane < n ? weigh(K::value(key)) : (uint64_t)0);
+  const uint64_t at = __ballot(lane < n && (MASS ? (double)upto >= want_m : above + lane + 1 >= want_n));
+  const int first = at ? __ffsll((unsigned long long)at) - 1 : 0;
+  cut.key = lane_value(key, first);
+  kept = lane_value(upto, first);
+  const uint64_t equal = __ballot(key == cut.key);
+  cut.same = __popcll(equal);
+  cut.ties = __popcll(equal & ((2ull << first) - 1));
+  __syncthreads();   // `few` may be filled again
+}
+
 // Largest interval end `lo` whose entries at or above it reach the target -- a count (MASS false) or a mass -- narrowed to the exact entry.
 // At entry: everything in [lo, ...) reaches it (cnt_lo entries, mass_lo), nothing at or above hi does.
 template <typename K, bool MASS, int NT, typename Src>
@@ -236,26 +267,10 @@ __device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, cons
   __syncthreads();
   src.gather(lo, hi, few);
   __syncthreads();
-  // every wave sorts the entries itself
-  const int lane = threadIdx.x & 63, n = min(few->n, 64);
-  uint32_t key = lane < n ? few->key[lane] : 0;
-  wave_sort(key);
-  bool here = lane < n;
-  if (MASS) {
-    const uint64_t upto = wave_upto(here ? weigh(K::value(key)) : (uint64_t)0);
-    here = here && (double)(mass_hi + upto) >= want_m;
-  } else {
-    here = here && cnt_hi + lane + 1 >= want_n;
-  }
-  const uint64_t at = __ballot(here);
-  const int first = at ? __ffsll((unsigned long long)at) - 1 : 0;
-  Cut r;
-  r.key = lane_value(key, first);
-  const uint64_t equal = __ballot(key == r.key);
-  r.same = __popcll(equal);
-  r.ties = __popcll(equal & ((2ull << first) - 1));
-  __syncthreads();   // `few` may be filled again
-  return r;
+  Cut cut;
+  uint64_t kept;
+  rank_few<K, MASS>(few, weigh, cnt_hi, mass_hi, want_n, want_m, cut, kept);
+  return cut;
 }
 
 // a row (or list) in registers: thread t holds entries t * per .. t * per + per - 1; key 0, w 0 = not (or no longer) an entry
@@ -313,6 +328,101 @@ __device__ __forceinline__ void drop_ties(RegRow<E>& r, Block<NT>& blk, const Cu
   }
 }
 
+// ---- histogram of a row in registers ----------------------------------------------------------------------------------------------------------
+// Bins count from the top.  Where the row spans few enough keys a bin is a key; otherwise it is a slice of the value range.
+template <int NT>
+struct HistLds { uint32_t c[4 * NT]; uint64_t m[4 * NT]; uint32_t bin[2], above[2], in[2]; uint64_t mass[2]; };
+struct Where { uint32_t bin, above, in; uint64_t mass; };   // the bin of a cut, its entries, and what lies above it
+
+template <typename K, int NT>
+struct Hist {
+  static constexpr int N = 4 * NT;
+  HistLds<NT>* h;
+  uint32_t key_min, key_max, c[4], cb, all_c;   // this thread's four bins and what lies above them
+  uint64_t m[4], mb, all_m;
+  float top, inv;
+  bool exact, usable;
+  int turn = 0;
+  __device__ __forceinline__ Hist(HistLds<NT>* lds, uint32_t lo, uint32_t hi) : h(lds), key_min(lo), key_max(hi) {
+    exact = hi - lo < N;
+    top = K::value(hi);
+    const float span = top - K::value(lo);
+    inv = (float)N / span;
+    usable = exact || (span > 0.f && span < INFINITY && inv < INFINITY);
+  }
+  __device__ __forceinline__ uint32_t bin(uint32_t key) const { return exact ? key_max - key : min((uint32_t)((top - K::value(key)) * inv), (uint32_t)N - 1); }
+  template <bool MASS, int E>
+  __device__ __forceinline__ void build(const RegRow<E>& r, Block<NT>& blk) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { h->c[i * NT + tid] = 0; if (MASS) h->m[i * NT + tid] = 0; }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (E > 4 && e % 4 == 0 && e >= r.per) break;
+      if (r.key[e]) {
+        const uint32_t b = bin(r.key[e]);
+        atomicAdd(&h->c[b], 1u);
+        if (MASS) atomicAdd(reinterpret_cast<unsigned long long*>(&h->m[b]), (unsigned long long)r.w[e]);
+      }
+    }
+    __syncthreads();
+    cb = 0; mb = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = h->c[4 * tid + i];
+      m[i] = MASS ? h->m[4 * tid + i] : 0;
+      cb += c[i];
+      mb += m[i];
+    }
+    blk.before2(cb, mb, all_c, all_m);
+  }
+  // the bin in which the running count (or mass) from the top first reaches its target, which the row does reach
+  template <bool MASS>
+  __device__ __forceinline__ Where locate(uint32_t want_n, double want_m) {
+    uint32_t run = cb;
+    uint64_t mass = mb;
+    const int t = turn;
+    turn ^= 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool here = MASS ? (double)mass < want_m && (double)(mass + m[i]) >= want_m : run < want_n && run + c[i] >= want_n;
+      if (here) { h->bin[t] = 4 * threadIdx.x + i; h->above[t] = run; h->in[t] = c[i]; h->mass[t] = mass; }
+      run += c[i];
+      mass += m[i];
+    }
+    __syncthreads();
+    return {h->bin[t], h->above[t], h->in[t], h->mass[t]};
+  }
+  // the exact cut in that bin; false: more than 64 entries of several keys crowd there
+  template <bool MASS, int E>
+  __device__ __forceinline__ bool resolve(const RegRow<E>& r, const Where& w, Few* few, const Weigh& weigh, uint32_t want_n, double want_m, Cut& cut, uint64_t& kept) {
+    if (exact) {
+      cut.key = key_max - w.bin;
+      cut.same = w.in;
+      const uint64_t each = weigh(K::value(cut.key));
+      const double q = each ? ceil((want_m - (double)w.mass) / (double)each) : 1.0;
+      cut.ties = MASS ? q < 1.0 ? 1u : q > (double)w.in ? w.in : (uint32_t)q : want_n - w.above;
+      kept = w.mass + cut.ties * each;
+      return true;
+    }
+    if (w.in > 64) return false;
+    if (threadIdx.x == 0) few->n = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (E > 4 && e % 4 == 0 && e >= r.per) break;
+      if (r.key[e] && bin(r.key[e]) == w.bin) {
+        const int at = atomicAdd(&few->n, 1);
+        if (at < 64) few->key[at] = r.key[e];
+      }
+    }
+    __syncthreads();
+    rank_few<K, MASS>(few, weigh, w.above, w.mass, want_n, want_m, cut, kept);
+    return true;
+  }
+};
+
 struct Setting {
   float T, top_p, min_p, u;
   int k;   // 0 = off
@@ -354,71 +464,79 @@ __device__ __forceinline__ int draw_few(uint32_t key, uint32_t k, const Weigh& w
   return __ffsll((unsigned long long)__ballot(back && (double)cum > want)) - 1;
 }
 
-// The short way for a small top-k: a threshold that leaves between k and 64 entries, these in index order to one wave.  -2: a crowd of equals
-// allows no such threshold.  Otherwise the place (e, in the thread that owns it) or -1.  Needs keys only.
+// The short way for a small top-k: the top bins that hold k entries and no more than 64 go in index order to one wave.  -2: too many crowd in the last
+// of these bins.  Otherwise the place (e, in the thread that owns it) or -1.  Needs keys only.
 struct FewOrder { uint32_t key[64]; int hit; };
 template <typename K, int E, int NT>
-__device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, FewOrder* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t k, uint32_t key_min, uint32_t key_max) {
-  uint32_t cnt_lo = n;
-  const float goal = __log2f(0.5f * (float)(k + 64));
-  Interval<K> in{key_min, key_max + 1, log_count(n) - goal, -1.f - goal};
-  while (cnt_lo > 64 && in.hi - in.lo > 1) {
-    const uint32_t mid = in.probe();
-    uint32_t cnt;
-    uint64_t none = 0;
-    r.template stat<false>(mid, cnt, none);
-    cnt = blk.count(cnt);
-    in.take(mid, log_count(cnt) - goal, cnt >= k);
-    if (cnt >= k) cnt_lo = cnt;
+__device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, HistLds<NT>* lds, FewOrder* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t k, uint32_t key_min, uint32_t key_max) {
+  uint32_t cnt = n, last = ~0u;   // the listed bins end with `last`
+  Hist<K, NT> hist(lds, key_min, key_max);
+  if (n > 64) {
+    if (!hist.usable) return -2;
+    hist.template build<false>(r, blk);
+    const Where w = hist.template locate<false>(k, 0.0);
+    cnt = w.above + w.in;
+    last = w.bin;
+    if (cnt > 64) return -2;
   }
-  const uint32_t lo = in.lo;
-  if (cnt_lo > 64) return -2;
-  uint32_t mine = 0, total;
+  uint32_t in = 0, total;   // which of this thread's entries are listed
 #pragma unroll
-  for (int e = 0; e < E; ++e) mine += r.key[e] >= lo;
-  const uint32_t first = blk.before(mine, total);
-  uint32_t p = first;
+  for (int e = 0; e < E; ++e) {
+    if (E > 4 && e % 4 == 0 && e >= r.per) break;
+    if (r.key[e] && (last == ~0u || hist.bin(r.key[e]) <= last)) in |= 1u << e;
+  }
+  const uint32_t mine = __popc(in), first = blk.before(mine, total);
   if (mine) {
+    uint32_t p = first;
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (r.key[e] >= lo) few->key[p++] = r.key[e];
+      if ((in >> e) & 1) few->key[p++] = r.key[e];
   }
   __syncthreads();
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
-    const int hit = draw_few<K>(lane < (int)cnt_lo ? few->key[lane] : 0u, k, weigh, s);
+    const int hit = draw_few<K>(lane < (int)cnt ? few->key[lane] : 0u, k, weigh, s);
     if (lane == 0) few->hit = hit;
   }
   __syncthreads();
-  const uint32_t hit = (uint32_t)few->hit;
-  if (hit - first >= mine) return -1;
-  int found = 0;
-  p = first + mine;
-#pragma unroll
-  for (int e = E - 1; e >= 0; --e)
-    if (r.key[e] >= lo) found = --p == hit ? e : found;
-  return found;
+  uint32_t nth = (uint32_t)few->hit - first;
+  if (nth >= mine) return -1;
+  for (; nth; --nth) in &= in - 1;
+  return __ffs(in) - 1;
 }
 
 // filters and draw on entries in registers; returns the place (e, in the thread that owns it) or -1.  `base`: the mass that top_p refers to when
 // it is not that of these entries (< 0: it is).  `enough` comes back false when these entries cannot hold the nucleus.
 template <typename K, int E, int NT>
-__device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block<NT>& blk, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, double base, bool& enough) {
+__device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block<NT>& blk, HistLds<NT>* lds, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, double base, bool& enough) {
   enough = true;
   Cut cut{key_min, 1u, 1u};
-  if (s.k && (uint32_t)s.k < n) {
-    cut = find_cut<K, false>(r, blk, few, weigh, key_min, n, 0, key_max + 1, (uint32_t)s.k, 0.0);
+  const bool cut_k = s.k && (uint32_t)s.k < n;
+  Hist<K, NT> hist(lds, key_min, key_max);
+  bool binned = hist.usable && (cut_k || s.top_p < 1.f);
+  uint64_t mass = 0;
+  if (binned) {
+    hist.template build<true>(r, blk);
+    mass = hist.all_m;
+  }
+  if (cut_k) {
+    if (binned) binned = hist.template resolve<false>(r, hist.template locate<false>((uint32_t)s.k, 0.0), few, weigh, (uint32_t)s.k, 0.0, cut, mass);
+    if (!binned) cut = find_cut<K, false>(r, blk, few, weigh, key_min, n, 0, key_max + 1, (uint32_t)s.k, 0.0);
     drop_ties(r, blk, cut);
     n = (uint32_t)s.k;
   }
   if (s.top_p < 1.f) {
-    uint32_t cnt;
-    uint64_t mass = 0;
-    r.template stat<true>(cut.key, cnt, mass);
-    blk.template sum<true>(cnt, mass);
+    if (!binned) {
+      uint32_t cnt;
+      mass = 0;
+      r.template stat<true>(cut.key, cnt, mass);
+      blk.template sum<true>(cnt, mass);
+    }
     const double want = target(s.top_p, base < 0.0 ? (double)mass : base);
     if ((double)mass < want) { enough = false; return -1; }
-    cut = find_cut<K, true>(r, blk, few, weigh, cut.key, n, mass, key_max + 1, 0u, want);
+    uint64_t kept;
+    if (binned) binned = hist.template resolve<true>(r, hist.template locate<true>(0u, want), few, weigh, 0u, want, cut, kept);
+    if (!binned) cut = find_cut<K, true>(r, blk, few, weigh, cut.key, n, mass, key_max + 1, 0u, want);
     drop_ties(r, blk, cut);
   }
   uint64_t mine = 0, total;
@@ -475,6 +593,7 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
   __shared__ Few few;
   __shared__ FewOrder order;
   __shared__ ExtremesLds ext;
+  __shared__ HistLds<NT> hist;
   __shared__ int best;
   const int row = blockIdx.x, tid = threadIdx.x;
   const XT* x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
@@ -511,12 +630,15 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
 #pragma unroll
   for (int e = 0; e < E; ++e) r.key[e] = v[e] > -INFINITY ? K::key(v[e]) : 0;
   int e = -2;
-  if (k <= 64) e = draw_small<K>(r, blk, &order, weigh, s, n, k, key_min, key_max);
+  if (k <= 64) e = draw_small<K>(r, blk, &hist, &order, weigh, s, n, k, key_min, key_max);
   if (e == -2) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) r.w[i] = weigh(v[i]);
+    for (int i = 0; i < E; ++i) {
+      r.w[i] = 0;
+      if (i < r.per) r.w[i] = weigh(v[i]);
+    }
     bool enough;
-    e = filter_and_draw<K>(r, blk, &few, weigh, s, n, key_min, key_max, -1.0, enough);
+    e = filter_and_draw<K>(r, blk, &hist, &few, weigh, s, n, key_min, key_max, -1.0, enough);
   }
   if (e >= 0) a.out[row] = first + e;
 }
@@ -595,6 +717,7 @@ __global__ __launch_bounds__(256) void sample_threshold_kernel(SampleOpArgs a) {
   __shared__ Red red;
   __shared__ Few few;
   __shared__ ExtremesLds ext;
+  __shared__ HistLds<NT> lds;
   const int row = blockIdx.x, tid = threadIdx.x;
   const XT* x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
   const Setting s = setting(a, row);
@@ -614,7 +737,17 @@ __global__ __launch_bounds__(256) void sample_threshold_kernel(SampleOpArgs a) {
     const int aim = s.k && s.k < AIM / 4 - 512 ? 4 * s.k + 2048 : AIM;   // a short top-k needs a short list
     const uint32_t rank = max(1u, (uint32_t)((int64_t)aim * SAMPLES / a.V));
     thr = K::NONE + 1;
-    if (n > rank) thr = find_cut<K, false>(r, blk, &few, Weigh{}, K::key(ex.mn), n, 0, K::key(ex.mx) + 1, rank, 0.0).key;
+    if (n > rank) {   // (the lower end of the bin is near enough, unless too many crowd there)
+      Hist<K, NT> hist(&lds, K::key(ex.mn), K::key(ex.mx));
+      Where w{0, 0, ~0u, 0};
+      if (hist.usable) {
+        hist.template build<false>(r, blk);
+        w = hist.template locate<false>(rank, 0.0);
+      }
+      if (hist.exact) thr = hist.key_max - w.bin;
+      else if (w.in <= 64) thr = K::key(hist.top - (float)(w.bin + 1) / hist.inv + 0.f);
+      else thr = find_cut<K, false>(r, blk, &few, Weigh{}, K::key(ex.mn), n, 0, K::key(ex.mx) + 1, rank, 0.0).key;
+    }
   }
   if (tid == 0) a.thr[row] = thr;
 }
@@ -705,6 +838,7 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   __shared__ Few few;
   __shared__ FewOrder order;
   __shared__ ExtremesLds ext;
+  __shared__ HistLds<NT> hist;
   __shared__ int best;
   __shared__ uint32_t start_s[MAX_CHUNKS], tie_s[16];
   __shared__ uint64_t mass_s[16];
@@ -819,14 +953,14 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
     }
     bool enough = true;
     int e = -2;
-    if (s.k && s.k <= 64) e = draw_small<K>(r, blk, &order, weigh, s, n, min((uint32_t)s.k, n), thr, key_max);
+    if (s.k && s.k <= 64) e = draw_small<K>(r, blk, &hist, &order, weigh, s, n, min((uint32_t)s.k, n), thr, key_max);
     if (e == -2) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         r.w[i] = 0;
         if (i < r.per) r.w[i] = r.key[i] ? weigh(K::value(r.key[i])) : 0;
       }
-      e = filter_and_draw<K>(r, blk, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << a.shift), enough);
+      e = filter_and_draw<K>(r, blk, &hist, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << a.shift), enough);
     }
     if (e >= 0) {
       const uint32_t p = tid * r.per + e;
