@@ -91,13 +91,19 @@ def _ck(lib, rc: int):
     raise RuntimeError(f"csm_ops error {rc}: {msg}")
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
+_grad_enabled = torch.is_grad_enabled
+_int32, _float32 = torch.int32, torch.float32
+
+
 def _call(fn, args: bytes, device: int):
     """One launch on the current stream of GPU `device`."""
-    if device == torch.cuda.current_device():
-        rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
+    if device == _current_device():
+        rc = fn(args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
+            rc = fn(args, _raw_stream(device))
     if rc:
         _ck(_lib, rc)
 
@@ -105,18 +111,18 @@ def _call(fn, args: bytes, device: int):
 _workspace_sizes = {}
 
 
-def _workspace(fn, args: bytes, key, device: int) -> Optional[torch.Tensor]:
-    """Scratch memory of one call, on the current stream like everything a call allocates.  How much depends on the sizes in `key` alone."""
+def _workspace(fn, key, args) -> int:
+    """Bytes of scratch memory of a call, which depend on the sizes in `key` alone.  The memory itself is allocated by every call."""
     need = _workspace_sizes.get(key)
     if need is None:
         size = C.c_size_t()
-        rc = fn(args, C.byref(size))
+        rc = fn(args(), C.byref(size))
         if rc:
             _ck(_lib, rc)
         if len(_workspace_sizes) > 4096:
             _workspace_sizes.clear()
         need = _workspace_sizes[key] = size.value
-    return torch.empty(need, dtype=torch.uint8, device=f"cuda:{device}") if need else None
+    return need
 
 
 def _need(ok: bool, what: str):
@@ -124,25 +130,26 @@ def _need(ok: bool, what: str):
         raise ValueError(what)
 
 
-def _on_device(first: torch.Tensor, named) -> int:
-    """The GPU that holds `first`; every other tensor must be there too, and none may ask for a gradient."""
-    dev = first.get_device()
+def _on_device(named) -> int:
+    """The GPU of the first tensor; every other one must be there too, and none may ask for a gradient."""
+    dev = named[0][1].get_device()
     if dev < 0:
         raise RuntimeError("csm_hf_amd operators need tensors on the GPU (no CPU fallback)")
-    grad = torch.is_grad_enabled()
     for name, t in named:
         if t is not None:
             if t.get_device() != dev:
                 raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
-            if grad and t.requires_grad:
+            if t.requires_grad and _grad_enabled():
                 raise RuntimeError(f"{name} requires a gradient: this operator has no backward pass (call it under torch.no_grad())")
     return dev
 
 
 def _index(name: str, v) -> int:
-    if not -2 ** 31 <= int(v) < 2 ** 31:
+    if type(v) is not int:
+        v = int(v)
+    if not -0x80000000 <= v <= 0x7fffffff:
         raise ValueError(f"{name} = {v} is out of range")
-    return int(v)
+    return v
 
 
 def _ints(name: str, t: torch.Tensor, n: int) -> int:
@@ -153,27 +160,36 @@ def _ints(name: str, t: torch.Tensor, n: int) -> int:
 
 def _paged(k_cache, v_cache, page_table, seq_lens, cu_rows, rows: int):
     """the fields of csm_ops_paged_t"""
-    shape, dt = k_cache.shape, _DT.get(k_cache.dtype)
-    if dt is None or len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype:
+    shape, dtype = k_cache.shape, k_cache.dtype
+    dt = _DT.get(dtype)
+    if dt is None or len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not dtype:
         raise ValueError("k_cache and v_cache must be float32 or bfloat16 tensors [n_pages, n_kv, page_size, head_dim] of one shape and dtype")
     n_pages, n_kv, page, hd = shape
-    kp, kh, ks, ki = k_cache.stride()
-    vp, vh, vs, vi = v_cache.stride()
-    if (ki != 1 or vi != 1) and hd != 1:
+    strides = k_cache.stride()
+    v_strides = strides if k_cache.is_contiguous() and v_cache.is_contiguous() else v_cache.stride()
+    if (strides[3] != 1 or v_strides[3] != 1) and hd != 1:
         raise ValueError("the last dimension of k_cache and v_cache must be contiguous")
-    if page_table.dim() != 2 or page_table.dtype is not torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    if page_table.dim() != 2 or page_table.dtype is not _int32 or not (page_table.is_contiguous() or page_table.stride(1) == 1):
         raise ValueError("page_table must be an int32 tensor [n_seqs, pages] with contiguous rows")
     n_seqs, width = page_table.shape
-    if cu_rows is None and rows != n_seqs:
-        raise ValueError(f"without cu_rows every sequence has one row: {rows} rows, {n_seqs} sequences")
-    return (k_cache.data_ptr(), v_cache.data_ptr(), dt, n_pages, page, n_kv, hd, kp, kh, ks, vp, vh, vs, page_table.data_ptr(), page_table.stride(0),
-            width, n_seqs, _ints("seq_lens", seq_lens, n_seqs), 0 if cu_rows is None else _ints("cu_rows", cu_rows, n_seqs + 1), rows)
+    if seq_lens.dtype is not _int32 or seq_lens.shape != (n_seqs,) or not seq_lens.is_contiguous():
+        raise ValueError(f"seq_lens must be a contiguous int32 tensor of shape ({n_seqs},)")
+    if cu_rows is None:
+        cu = 0
+        if rows != n_seqs:
+            raise ValueError(f"without cu_rows every sequence has one row: {rows} rows, {n_seqs} sequences")
+    else:
+        cu = _ints("cu_rows", cu_rows, n_seqs + 1)
+    return (k_cache.data_ptr(), v_cache.data_ptr(), dt, n_pages, page, n_kv, hd, *strides[:3], *v_strides[:3], page_table.data_ptr(), page_table.stride(0),
+            width, n_seqs, seq_lens.data_ptr(), cu, rows)
 
 
 def _heads(name: str, t: torch.Tensor, shape, dtype):
     """[rows, heads, dim] with contiguous heads; returns (pointer, row stride)"""
     if t.dtype is not dtype or t.shape != shape:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)}")
+    if t.is_contiguous():
+        return t.data_ptr(), shape[1] * shape[2]
     a, b, c = t.stride()
     if (c != 1 and shape[2] > 1) or (b != shape[2] and shape[1] > 1):
         _need(t.numel() == 0, f"the heads of a row of {name} must be contiguous")
@@ -197,7 +213,7 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
     A sequence with `seq_lens < 0` is padding.  Its rows, rows behind `cu_rows[-1]` and rows whose slot, page or rotary position lies outside the
     table, the cache or the tables are skipped: nothing is written for them, in q_out either.  Two rows that share a cache slot (a page that
     two sequences write to) leave either row's values there.  q, k and v must not overlap in memory with the cache."""
-    dev = _on_device(qkv, (("qkv", qkv), ("cos", cos), ("sin", sin), ("k_cache", k_cache), ("v_cache", v_cache), ("page_table", page_table),
+    dev = _on_device((("qkv", qkv), ("cos", cos), ("sin", sin), ("k_cache", k_cache), ("v_cache", v_cache), ("page_table", page_table),
                            ("seq_lens", seq_lens), ("cu_rows", cu_rows), ("q_out", q_out)))
     x = _DT.get(qkv.dtype)
     if x is None or qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
@@ -209,15 +225,13 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
     if n_q < 1 or width != (n_q + 2 * n_kv) * hd:
         raise ValueError(f"qkv rows of {width} elements are not n_q + 2 * {n_kv} heads of {hd}")
     half = hd // 2
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t.dtype is not torch.float32 or t.dim() != 2 or t.shape[1] != half or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous float32 tensor [positions, {half}]")
-    if cos.shape != sin.shape:
-        raise ValueError("cos and sin must have one shape")
+    positions = cos.shape[0] if cos.dim() else 0
+    if cos.dtype is not _float32 or sin.dtype is not _float32 or cos.shape != (positions, half) or sin.shape != (positions, half) or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError(f"cos and sin must be contiguous float32 tensors [positions, {half}]")
     if q_out is None:
         q_out = qkv.new_empty((rows, n_q, hd))
     q, q_stride = _heads("q_out", q_out, (rows, n_q, hd), qkv.dtype)
-    args = _PACK_APPEND(*c, qkv.data_ptr(), q, qkv.stride(0), q_stride, x, n_q, cos.data_ptr(), sin.data_ptr(), cos.shape[0], _index("pos_offset", pos_offset))
+    args = _PACK_APPEND(*c, qkv.data_ptr(), q, qkv.stride(0), q_stride, x, n_q, cos.data_ptr(), sin.data_ptr(), positions, _index("pos_offset", pos_offset))
     _call((_lib or load_ops_library()).csm_ops_paged_rope_append, args, dev)
     return q_out
 
@@ -235,7 +249,7 @@ def paged_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
     A row that sees no key gives zeros.  Rows of padding (`seq_lens < 0`) and rows behind `cu_rows[-1]` keep what `out` held.  Slots on pages
     outside the cache are not seen.  `prefix_len` and all sizes are fixed in a captured graph; lengths, tables and `cu_rows` are read at replay."""
-    dev = _on_device(q, (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("page_table", page_table), ("seq_lens", seq_lens),
+    dev = _on_device((("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("page_table", page_table), ("seq_lens", seq_lens),
                          ("prefix_table", prefix_table), ("cu_rows", cu_rows), ("out", out)))
     x, shape = _DT.get(q.dtype), q.shape
     if x is None or len(shape) != 3:
@@ -254,9 +268,14 @@ def paged_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     rest = (pq, po, q_stride, o_stride, x, shape[1], pp, n_prefix, prefix_len, shape[2] ** -0.5 if scale is None else scale)
     lib = _lib or load_ops_library()
     # (what the split of the work goes by: types, sizes of rows, heads, pages and table, prefix)
-    ws = _workspace(lib.csm_ops_paged_attention_workspace, _PACK_ATTENTION(*c, *rest, 0, 0),
-                    (shape, x, c[2], c[4], c[5], c[15], c[16], cu_rows is None, prefix_len, n_prefix), dev)
-    _call(lib.csm_ops_paged_prefix_attention, _PACK_ATTENTION(*c, *rest, *((0, 0) if ws is None else (ws.data_ptr(), ws.numel()))), dev)
+    need = _workspace(lib.csm_ops_paged_attention_workspace, (shape, x, c[2], c[4], c[5], c[15], c[16], cu_rows is None, prefix_len, n_prefix),
+                      lambda: _PACK_ATTENTION(*c, *rest, 0, 0))
+    if need:
+        ws = q.new_empty(need, dtype=torch.uint8)
+        args = _PACK_ATTENTION(*c, *rest, ws.data_ptr(), need)
+    else:
+        args = _PACK_ATTENTION(*c, *rest, 0, 0)
+    _call(lib.csm_ops_paged_prefix_attention, args, dev)
     return out
 
 
@@ -271,7 +290,7 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, *, temperature:
     index at which the running sum of kept probability passes `uniform` times its total.  `temperature = 0` is the arg-max, the lowest index
     of equals, like `sample_topk`; exactly `topk` entries stay, so `topk = 1` is the arg-max too (`sample_topk` keeps every entry that ties with
     the k-th).  V up to 2^21; a NaN logit counts as -inf; a row with nothing but -inf gives -1."""
-    dev = _on_device(logits, (("logits", logits), ("uniform", uniform)))
+    dev = _on_device((("logits", logits), ("uniform", uniform)))
     x, lead = _DT.get(logits.dtype), logits.shape[:-1]
     if x is None or logits.dim() < 1:
         raise ValueError("logits must be a float32 or bfloat16 tensor [..., V]")
@@ -299,8 +318,11 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, *, temperature:
     out = logits.new_empty((*lead, 1), dtype=torch.int32)
     args = (lg.data_ptr(), lg.stride(0), x, rows, V, pu, *many, *one, out.data_ptr())
     lib = _lib or load_ops_library()
-    ws = None
-    if V > 4096:
-        ws = _workspace(lib.csm_ops_sample_workspace, _PACK_SAMPLE(*args, 0, 0), (rows, V), dev)
-    _call(lib.csm_ops_sample_filtered, _PACK_SAMPLE(*args, *((0, 0) if ws is None else (ws.data_ptr(), ws.numel()))), dev)
+    need = _workspace(lib.csm_ops_sample_workspace, (rows, V), lambda: _PACK_SAMPLE(*args, 0, 0)) if V > 4096 else 0
+    if need:
+        ws = logits.new_empty(need, dtype=torch.uint8)
+        packed = _PACK_SAMPLE(*args, ws.data_ptr(), need)
+    else:
+        packed = _PACK_SAMPLE(*args, 0, 0)
+    _call(lib.csm_ops_sample_filtered, packed, dev)
     return out
