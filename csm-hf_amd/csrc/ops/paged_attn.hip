@@ -34,7 +34,7 @@ struct AttnOpArgs {
   uint32_t kp16, ks16, vp16, vs16;   // page and slot strides in 16-byte units: a slot's place inside the cache fits 32 bits up to 64 GB
   float c2;               // |scale| log2(e); the sign of scale is folded into q
   uint32_t q_flip;
-  int np_tiles, nsp, no_tiles, nso, per_seq_tiles, with_prefix, nsplit;   // nsplit = partial results per row
+  int np_tiles, nsp, no_tiles, nso, per_seq_tiles, with_prefix, tall, nsplit;   // nsplit = partial results per row
   float* part;            // [rows * n_q][nsplit][hd]
   float2* ml;             // [rows * n_q][nsplit] (reference in log2 units, sum)
 };
@@ -522,15 +522,15 @@ __device__ __forceinline__ void put(const AttnOpArgs& a, int row, int head, int 
   }
 }
 
-template <typename XT, typename CT, int HD>
-__global__ __launch_bounds__(AT, 2) void paged_attn_kernel(AttnOpArgs a) {
+template <typename XT, typename CT, int HD, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void paged_attn_kernel(AttnOpArgs a) {
   using P = Prod<XT, CT, HD>;
-  constexpr bool WIDE = sizeof(CT) == 2;
+  constexpr bool WIDE = sizeof(CT) == 2 && NW == 4;
   constexpr int ROWS = tile_rows(sizeof(XT) == 2 ? CSM_OPS_BF16 : CSM_OPS_F32);
   constexpr int WAVE_LDS = P::LDS_BYTES > 16 * (HD + 4) * 4 ? P::LDS_BYTES : 16 * (HD + 4) * 4;   // V tile; at the end 16 rows of fp32 results
-  constexpr int LDS = WIDE && Wide<XT, HD>::LDS_BYTES > 4 * WAVE_LDS ? Wide<XT, HD>::LDS_BYTES : 4 * WAVE_LDS;
+  constexpr int LDS = WIDE && Wide<XT, HD>::LDS_BYTES > NW * WAVE_LDS ? Wide<XT, HD>::LDS_BYTES : NW * WAVE_LDS;
   __shared__ __attribute__((aligned(16))) char lds[LDS];
-  __shared__ float ml_s[4][16][2];
+  __shared__ float ml_s[NW][16][2];
   const Paged& c = a.c;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x % c.n_kv;   // fastest: with 8 kv-heads the items of one head share an XCD's L2
@@ -617,7 +617,7 @@ __global__ __launch_bounds__(AT, 2) void paged_attn_kernel(AttnOpArgs a) {
     }
   }
   // rows of this wave: all waves the same 16 (keys split over the waves), or 16 each
-  const int mine = by_keys ? 0 : 16 * wave, n_mine = min(16, live - mine);
+  const int mine = by_keys ? 0 : 16 * wave, n_mine = min(16, live - mine);   // (ROWS <= 16 NW)
   char* my_lds = lds + wave * WAVE_LDS;
   f32x4 o[HD / 16];
   float m = -INFINITY, l = 0.f;
@@ -627,28 +627,28 @@ __global__ __launch_bounds__(AT, 2) void paged_attn_kernel(AttnOpArgs a) {
     P pr;
     pr.load_q(row_live ? reinterpret_cast<const XT*>(a.q) + row * a.q_stride + (int64_t)head * HD : nullptr, g, a.q_flip);
     const int lim = own ? sees(f / a.rep) : a.prefix_len, lim_min = own ? sees((f0 + mine) / a.rep) : a.prefix_len;   // rows ascend: the first sees least
-    wave_attend<XT, CT, HD>(a, pr, ax, kvh, k0, k1, by_keys ? wave : 0, by_keys ? 4 : 1, lim, lim_min, my_lds, o, m, l);
+    wave_attend<XT, CT, HD>(a, pr, ax, kvh, k0, k1, by_keys ? wave : 0, by_keys ? NW : 1, lim, lim_min, my_lds, o, m, l);
   }
-  if (by_keys) {   // join the four waves: every one rescales to the common reference and leaves its rows in LDS
+  if (by_keys) {   // join the waves: every one rescales to the common reference and leaves its rows in LDS
     if (g == 0) { ml_s[wave][li][0] = m; ml_s[wave][li][1] = l; }
     __syncthreads();
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml_s[w][li][0]);
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, ml_s[w][li][0]);
     const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
     float* mine_o = reinterpret_cast<float*>(my_lds) + li * (HD + 4);
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt) store4(mine_o + 16 * dt + 4 * g, o[dt] * alpha);
     __syncthreads();
-    for (int i = threadIdx.x; i < live * (HD / 4); i += AT) {
+    for (int i = threadIdx.x; i < live * (HD / 4); i += 64 * NW) {
       const int r = i / (HD / 4), d = (i % (HD / 4)) * 4, ff = f0 + r;
       const int rr = row0 + ff / a.rep, hh = kvh * a.rep + ff % a.rep;
       f32x4 sum = (f32x4)(0.f);
       float top_r = -INFINITY, l_r = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top_r = fmaxf(top_r, ml_s[w][r][0]);
+      for (int w = 0; w < NW; ++w) top_r = fmaxf(top_r, ml_s[w][r][0]);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < NW; ++w) {
         sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * WAVE_LDS) + r * (HD + 4) + d);
         const float mw = ml_s[w][r][0];
         l_r += mw == -INFINITY ? ml_s[w][r][1] : ml_s[w][r][1] * __builtin_amdgcn_exp2f(mw - top_r);
@@ -737,10 +737,14 @@ static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
   a.per_seq_tiles = (a.rep + ROWS - 1) / ROWS;
   const int64_t own_tiles = c.cu_rows ? flat / ROWS + c.n_seqs : (int64_t)c.n_seqs * a.per_seq_tiles;
   const int64_t own_cap = (int64_t)c.table_width * c.page_size;
-  // the prefix goes with each sequence's own slots (read once per sequence, nothing to join) where sequences bring two tiles of 16 rows and more of their
-  // own, and where the whole axis is short: then it is a few iterations from L2, and a second launch would cost more than sharing it saves
-  const bool short_axis = p->prefix_len + own_cap <= 256;
-  a.with_prefix = p->prefix_len > 0 && (short_axis || (c.cu_rows && c.n_seqs > 0 && flat / c.n_seqs >= 32));
+  const bool narrow = c.n_seqs > 0 && flat / c.n_seqs <= 16;   // decode: items wait for memory and are cheap to cut; a tile of many rows has much to join
+  const int64_t axis = p->prefix_len + own_cap;
+  // few sequences and a short axis: ONE launch of tall workgroups (16 or 8 waves split the keys, the prefix among them) -- the prefix is read once per
+  // sequence, from L2, and there is nothing to join.  32 sequences, 200 + 50 slots of 64 bf16: 7.4 us against 10.7; 1 sequence, 512 + 130: 8.8
+  // against 7.8 and a launch of 3.5 us saved on the host; 1 sequence, 512 + 1000: 12.5 against 8.6, and 128 sequences, 200 + 50: 22 against 12
+  a.tall = narrow && p->prefix_len > 0 && own_tiles * c.n_kv <= 256 && axis * c.head_dim * (c.dtype == CSM_OPS_BF16 ? 2 : 4) <= 128 * 1024;
+  // sequences that bring two tiles of 16 rows and more of their own read the prefix with them: nothing to share, nothing to join
+  a.with_prefix = a.tall || (p->prefix_len > 0 && c.cu_rows && c.n_seqs > 0 && flat / c.n_seqs >= 32);
   const int64_t np = p->prefix_len && !a.with_prefix ? (flat + ROWS - 1) / ROWS : 0;
   const int64_t own_keys = own_cap + (a.with_prefix ? p->prefix_len : 0);
   auto splits = [](int64_t items, int64_t keys, int64_t fill, int64_t more) {   // `fill` items of 128 keys and more, `more` of 256 and more
@@ -750,9 +754,8 @@ static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
     const int64_t n = a > b ? a : b;
     return (int)(n < 1 ? 1 : n > MAX_SPLIT / 2 ? MAX_SPLIT / 2 : n);
   };
-  const bool narrow = c.n_seqs > 0 && flat / c.n_seqs <= 16;   // such items wait for memory and are cheap to cut; a tile of many rows has much to join
   a.nsp = np ? splits(np * c.n_kv, p->prefix_len, 256, 0) : 0;
-  a.nso = short_axis && a.with_prefix ? 1 : splits(own_tiles * c.n_kv, own_keys, 512, narrow ? 2048 : 0);
+  a.nso = a.tall ? 1 : splits(own_tiles * c.n_kv, own_keys, 512, narrow ? 2048 : 0);
   a.np_tiles = (int)np; a.no_tiles = (int)own_tiles; a.nsplit = a.nsp + a.nso;
   if (((int64_t)a.np_tiles * a.nsp + (int64_t)a.no_tiles * a.nso) * c.n_kv > 0x7fffffff) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
   return 0;
@@ -776,7 +779,9 @@ extern "C" int csm_ops_paged_attention_workspace(const csm_ops_attention_t* p, s
 template <typename XT, typename CT, int HD>
 static int launch(const AttnOpArgs& a, hipStream_t st) {
   const unsigned items = (unsigned)(((int64_t)a.np_tiles * a.nsp + (int64_t)a.no_tiles * a.nso) * a.c.n_kv);
-  hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD>), dim3(items), dim3(AT), 0, st, a);
+  constexpr int TALL = HD == 64 ? 16 : 8;   // as many waves as their registers allow
+  if (a.tall) hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD, TALL>), dim3(items), dim3(64 * TALL), 0, st, a);
+  else hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD, 4>), dim3(items), dim3(AT), 0, st, a);
   OPS_HIP(hipGetLastError());
   if (a.nsplit > 1) {
     const unsigned n = (unsigned)(((int64_t)a.c.rows * a.n_q + 3) / 4);
