@@ -726,8 +726,10 @@ static int check(const csm_ops_attention_t* p) {
   return 0;
 }
 
-// How the work is cut.  Items should fill 256 CUs a few times over (a CU holds two workgroups), but an item shorter than 128 keys is mostly
-// start-up, and every split costs a partial result per row.
+// How the work is cut.  Items should fill 256 CUs (of two to four workgroups each), but a short item is mostly start-up, and every piece costs a
+// partial result per row, written and read again.  Measured (us): 128 sequences behind 4096 slots, prefix in 2 / 4 / 8 / 16 pieces 93 / 94 / 95 / 103 and
+// alone 48 / 30 / 22 / 25; 64 sequences of 128-wide heads behind 2048 slots in 4 / 8 / 16 pieces 27 / 20 / 24; 16 fp32 sequences behind 512 slots in
+// 4 / 8 pieces 16 / 13; own slots of 128 sequences whole / halved 95 / 90; tiles of many rows whole / in 3 pieces 88 / 110.
 static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
   const csm_ops_paged_t& c = p->c;
   a.c = ops_paged(c);
@@ -747,15 +749,16 @@ static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
   a.with_prefix = a.tall || (p->prefix_len > 0 && c.cu_rows && c.n_seqs > 0 && flat / c.n_seqs >= 32);
   const int64_t np = p->prefix_len && !a.with_prefix ? (flat + ROWS - 1) / ROWS : 0;
   const int64_t own_keys = own_cap + (a.with_prefix ? p->prefix_len : 0);
-  auto splits = [](int64_t items, int64_t keys, int64_t fill, int64_t more) {   // `fill` items of 128 keys and more, `more` of 256 and more
+  // pieces of `keys` for each of `items`: up to `few` of them may be as short as `small` keys, up to `many` as short as 256
+  auto splits = [](int64_t items, int64_t keys, int64_t few, int64_t small, int64_t many) {
     if (items < 1) items = 1;
-    const int64_t a = fill / items < (keys + 127) / 128 ? fill / items : (keys + 127) / 128;
-    const int64_t b = more / items < (keys + 255) / 256 ? more / items : (keys + 255) / 256;
+    const int64_t a = few / items < (keys + small - 1) / small ? few / items : (keys + small - 1) / small;
+    const int64_t b = many / items < (keys + 255) / 256 ? many / items : (keys + 255) / 256;
     const int64_t n = a > b ? a : b;
     return (int)(n < 1 ? 1 : n > MAX_SPLIT / 2 ? MAX_SPLIT / 2 : n);
   };
-  a.nsp = np ? splits(np * c.n_kv, p->prefix_len, 256, 0) : 0;
-  a.nso = a.tall ? 1 : splits(own_tiles * c.n_kv, own_keys, 512, narrow ? 2048 : 0);
+  a.nsp = np ? splits(np * c.n_kv, p->prefix_len, 64, 64, 256) : 0;
+  a.nso = a.tall ? 1 : splits(own_tiles * c.n_kv, own_keys, 512, 128, narrow ? 2048 : 0);
   a.np_tiles = (int)np; a.no_tiles = (int)own_tiles; a.nsplit = a.nsp + a.nso;
   if (((int64_t)a.np_tiles * a.nsp + (int64_t)a.no_tiles * a.nso) * c.n_kv > 0x7fffffff) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
   return 0;
