@@ -247,8 +247,9 @@ def paged_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     `head_dim ** -0.5`.  head_dim is 64 or 128, n_q any multiple of n_kv.  With float32 q everything is float32; with bfloat16 q the products
     run on the bf16 matrix pipe with float32 sums and one rounding of the result.
 
-    A row that sees no key gives zeros.  Rows of padding (`seq_lens < 0`) and rows behind `cu_rows[-1]` keep what `out` held.  Slots on pages
-    outside the cache are not seen.  `prefix_len` and all sizes are fixed in a captured graph; lengths, tables and `cu_rows` are read at replay."""
+    A row that sees no key gives zeros.  Rows of padding (`seq_lens < 0`) and rows behind `cu_rows[-1]` keep what `out` held (`out` may be `q`).
+    Slots on pages outside the cache are not seen.  Slots that no row of the call sees may hold anything; a NaN or infinity in v of a slot that
+    some new rows of a sequence see also reaches its earlier rows of the call (0 * NaN), never another sequence.  `prefix_len` and all sizes are fixed in a captured graph; lengths, tables and `cu_rows` are read at replay."""
     dev = _on_device((("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("page_table", page_table), ("seq_lens", seq_lens),
                          ("prefix_table", prefix_table), ("cu_rows", cu_rows), ("out", out)))
     x, shape = _DT.get(q.dtype), q.shape

@@ -113,6 +113,22 @@ def test_sample_refusals(over):
     assert lib.csm_ops_sample_filtered(bytes(a), None) in (-1, -3) and lib.csm_ops_last_error()
 
 
+def test_small_workspaces_are_refused():
+    lib = ops.load_ops_library()
+    need = C.c_size_t()
+    a = ops.AttentionArgs(q=1 << 24, out=1 << 25, q_stride=256, out_stride=256, x_dtype=1, n_q=4, scale=0.125, prefix_table=1 << 26, prefix_pages=512, prefix_len=8192)
+    _paged_args(a.c)
+    assert lib.csm_ops_paged_attention_workspace(bytes(a), C.byref(need)) == 0 and need.value > 0
+    for ws, size in ((None, 0), (1 << 28, need.value - 1), ((1 << 28) + 4, need.value)):
+        a.workspace, a.workspace_bytes = ws, size
+        assert lib.csm_ops_paged_prefix_attention(bytes(a), None) == -3
+    s = ops.SampleArgs(logits=1 << 20, logits_stride=20000, rows=2, V=20000, uniform=1 << 21, temperature=1.0, top_p=0.5, out=1 << 22)
+    assert lib.csm_ops_sample_workspace(bytes(s), C.byref(need)) == 0 and need.value > 0
+    for ws, size in ((None, 0), (1 << 28, need.value - 1), ((1 << 28) + 4, need.value)):
+        s.workspace, s.workspace_bytes = ws, size
+        assert lib.csm_ops_sample_filtered(bytes(s), None) == -3
+
+
 def test_cpu_tensors_are_refused():
     z, i = torch.zeros(1, 4, 64), torch.zeros(1, 1, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
@@ -484,6 +500,40 @@ def test_attention_and_append_past_32_bit_offsets():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("x", [BF16, F32])
+@pytest.mark.parametrize("prefix", [0, 40, 3000])
+def test_attention_mixed_sequences(x, prefix):
+    """one long text among many single tokens: every way of cutting the work meets every kind of sequence in one launch"""
+    new = [1] * 20 + [45] + [1, 0, 2] + [1] * 7
+    lens = [1 + (i * 53) % 190 for i in range(20)] + [60] + [700, 5, 2] + [-1, 3, 3, 900, 17, 0, 64]
+    _attn_case(lens, new, 4, 2, 64, x, BF16, prefix=prefix, seed=prefix)
+    _attn_case(lens, new, 2, 1, 128, x, BF16, prefix=prefix, seed=prefix + 1)
+    if x == F32:
+        _attn_case(lens, new, 4, 2, 64, x, F32, prefix=prefix, seed=prefix + 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x,c", [(BF16, BF16), (F32, BF16), (F32, F32)])
+@pytest.mark.parametrize("lens,new,prefix", [([30, 9], [1, 1], 20), ([30, 9], [1, 1], 3000), ([200, 60], [150, 60], 100), ([2000], [1], 0)])
+def test_attention_in_place_and_strided(x, c, lens, new, prefix):
+    """out = q, q as the q part of wider rows, out as a slice of wider rows"""
+    cache = Cache(lens, 16, 2, 64, c, prefix=prefix)
+    n = sum(new)
+    wide = torch.randn(n, 10, 64, device=DEV).to(x)
+    q = wide[:, 1:5]
+    kw = dict(prefix_table=cache.prefix, prefix_len=prefix, cu_rows=_cu(new))
+    want, tol = attention64(q, cache, lens, new, 4, 0.125, x == BF16)
+    into = torch.zeros(n, 7, 64, device=DEV).to(x)
+    paged_prefix_attention(q, *cache.args(), out=into[:, 2:6], **kw)
+    check(into[:, 2:6], want, tol, 0.0)
+    assert bool((into[:, :2] == 0).all()) and bool((into[:, 6:] == 0).all())
+    beside = wide[:, 5:].clone()
+    paged_prefix_attention(q, *cache.args(), out=q, **kw)
+    check(q, want, tol, 0.0)
+    assert torch.equal(wide[:, 5:], beside)
+
+
+@pytest.mark.gpu
 def test_attention_same_bits_every_time():
     cache, q, out = _attn_case([700, 90, 1300], [1, 1, 1], 8, 2, 64, BF16, BF16, prefix=900, cu=None)
     for _ in range(5):
@@ -610,6 +660,48 @@ def test_sample_large_vocabulary(dtype):
     x, u = (torch.randn(3, 128256, generator=g) * 2.5).to(dtype), torch.rand(3, generator=g)
     for kw in (dict(), dict(top_p=f32(0.9)), dict(topk=50, top_p=f32(0.9)), dict(min_p=f32(0.01)), dict(topk=100000, top_p=f32(0.99))):
         _sample_case(x, u, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sample_crowded_rows(dtype):
+    """what the histogram, the list and its chunks cannot hold: one outlier far from a crowd, thousands of near-equal winners side by side, few distinct
+    values, a flat row, nearly everything masked"""
+    g = torch.Generator().manual_seed(2)
+    for V in (3000, 9000, 40000, 70001):
+        x = torch.randn(6, V, generator=g)
+        x[0] = x[0] * 1e-3
+        x[0, 17] = 1e4
+        x[1, V // 3:V // 3 + min(5000, V // 3)] += 8.0
+        x[2] = torch.randint(0, 3, (V,), generator=g).float()
+        x[3] = x[3] * 1e-6
+        x[4, :V - 30] = -math.inf
+        x[5] = -1e4
+        x[5, 5:80] = torch.linspace(0, 1e-3, 75)
+        x, u = x.to(dtype), torch.rand(6, generator=g)
+        for kw in (dict(top_p=f32(0.9)), dict(topk=min(V, 4000), top_p=f32(0.95)), dict(topk=64), dict(topk=65, min_p=f32(0.3)), dict(min_p=f32(0.7)), dict()):
+            _sample_case(x, u, **kw)
+
+
+@pytest.mark.gpu
+def test_sample_captured():
+    """short and long rows in one graph, replayed with new inputs"""
+    g = torch.Generator().manual_seed(6)
+    xs = [torch.randn(3, V, generator=g).to(DEV) for V in (2051, 5000, 20011)]
+    u = torch.rand(3, generator=g).to(DEV)
+    run = lambda: [sample_filtered(x, u, topk=50, top_p=0.9) for x in xs] + [sample_filtered(x, u, top_p=0.7) for x in xs]  # noqa: E731
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for seed in range(4):
+        g.manual_seed(seed)
+        for x in xs:
+            x.copy_(torch.randn(x.shape, generator=g))
+        u.copy_(torch.rand(3, generator=g))
+        graph.replay()
+        torch.randn(1000, device=DEV).sum().item()
+        assert all(torch.equal(a, b) for a, b in zip(out, run()))
 
 
 @pytest.mark.gpu
