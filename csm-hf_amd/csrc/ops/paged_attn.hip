@@ -31,7 +31,8 @@ struct AttnOpArgs {
   const int32_t* prefix;
   int64_t q_stride, out_stride;
   int n_q, rep, prefix_len;
-  uint32_t kp16, ks16, vp16, vs16;   // page and slot strides in 16-byte units: a slot's place inside the cache fits 32 bits up to 64 GB
+  uint32_t kp16, ks16, vp16, vs16;   // page and slot strides in 16-byte units (below 2^24): a slot's place inside the cache fits 32 bits up to 64 GB
+  int one_place;                     // K and V lie alike: one place serves both
   float c2;               // |scale| log2(e); the sign of scale is folded into q
   uint32_t q_flip;
   int np_tiles, nsp, no_tiles, nso, per_seq_tiles, with_prefix, tall, nsplit;   // nsplit = partial results per row
@@ -257,8 +258,9 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const Prod<XT, 
       const bool ok = pg[kt] < (uint32_t)a.c.n_pages;
       const uint32_t page = ok ? pg[kt] : 0;   // page 0 exists: callers have n_pages >= 1
       valid |= ((uint32_t)__ballot(ok) & 0xffffu) << (16 * kt);
-      ko[kt] = page * a.kp16 + sl[kt] * a.ks16;
-      vo[kt] = page * a.vp16 + sl[kt] * a.vs16;
+      ko[kt] = __umul24(page, a.kp16) + __umul24(sl[kt], a.ks16);
+      vo[kt] = ko[kt];
+      if (!a.one_place) vo[kt] = __umul24(page, a.vp16) + __umul24(sl[kt], a.vs16);
     }
     P::load(t, kb, vb, ko, vo, lane);
   };
@@ -351,11 +353,19 @@ struct Wide {
     u32x4 kr[NL], vr[NL];
     auto fetch = [&]() -> uint64_t {
       const bool ok = entry < (uint32_t)a.c.n_pages;
-      const uint32_t page = ok ? entry : 0, ko = page * a.kp16 + slot * a.ks16, vo = page * a.vp16 + slot * a.vs16;   // (page 0 exists)
+      const uint32_t page = ok ? entry : 0, ko = __umul24(page, a.kp16) + __umul24(slot, a.ks16);   // (page 0 exists)
+      uint32_t kat[NL], vat[NL];
+#pragma unroll
+      for (int i = 0; i < NL; ++i) vat[i] = kat[i] = __shfl(ko, i * KPP + key0);
+      if (!a.one_place) {
+        const uint32_t vo = __umul24(page, a.vp16) + __umul24(slot, a.vs16);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) vat[i] = __shfl(vo, i * KPP + key0);
+      }
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        kr[i] = *reinterpret_cast<const u32x4*>(kb + ((uint64_t)__shfl(ko, i * KPP + key0) << 4));
-        vr[i] = *reinterpret_cast<const u32x4*>(vb + ((uint64_t)__shfl(vo, i * KPP + key0) << 4));
+        kr[i] = *reinterpret_cast<const u32x4*>(kb + ((uint64_t)kat[i] << 4));
+        vr[i] = *reinterpret_cast<const u32x4*>(vb + ((uint64_t)vat[i] << 4));
       }
       return __ballot(ok);
     };
@@ -718,6 +728,9 @@ static int check(const csm_ops_attention_t* p) {
   const int64_t unit = c.dtype == CSM_OPS_BF16 ? 8 : 4, most_k = (c.n_pages - 1) * c.k_page_stride + (c.page_size - 1) * c.k_slot_stride,
                 most_v = (c.n_pages - 1) * c.v_page_stride + (c.page_size - 1) * c.v_slot_stride;
   if (c.n_pages && (most_k / unit > 0xffffffffll || most_v / unit > 0xffffffffll)) return ops_fail(CSM_OPS_ERR_CAPACITY, "a cache of more than 64 GB");
+  const int64_t strides[4] = {c.k_page_stride, c.k_slot_stride, c.v_page_stride, c.v_slot_stride};
+  for (int64_t x : strides)
+    if (x / unit >= 1 << 24 || c.n_pages > 1 << 24) return ops_fail(CSM_OPS_ERR_CAPACITY, "more than 2^24 pages, or pages or slots 256 MB apart");
   if (!isfinite(p->scale)) return ops_fail(CSM_OPS_ERR_ARG, "scale must be finite");
   if (!c.rows) return 0;
   if (!p->q || !p->out || (p->prefix_len && !p->prefix_table)) return ops_fail(CSM_OPS_ERR_ARG, "null pointer");
@@ -807,6 +820,7 @@ extern "C" int csm_ops_paged_prefix_attention(const csm_ops_attention_t* p, void
   const int unit = c.dtype == CSM_OPS_BF16 ? 8 : 4;
   a.kp16 = (uint32_t)(c.k_page_stride / unit); a.ks16 = (uint32_t)(c.k_slot_stride / unit);
   a.vp16 = (uint32_t)(c.v_page_stride / unit); a.vs16 = (uint32_t)(c.v_slot_stride / unit);
+  a.one_place = a.kp16 == a.vp16 && a.ks16 == a.vs16;
   a.part = reinterpret_cast<float*>(p->workspace);
   a.ml = need ? reinterpret_cast<float2*>(a.part + (size_t)c.rows * p->n_q * a.nsplit * c.head_dim) : nullptr;
   a.q_flip = p->scale < 0.f ? 0x80000000u : 0u;

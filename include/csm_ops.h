@@ -77,7 +77,8 @@ int csm_ops_paged_rope_append(const csm_ops_rope_append_t* a, void* stream);
  * reading kv head h / (n_q / n_kv).  The prefix is read once for all rows, not once per sequence.  A row that sees no key gives zeros; a
  * page number outside the cache hides its slots.  Slots that no row of the call sees may hold anything; a NaN or infinity in v of a slot that
  * some rows of a sequence see also reaches that sequence's earlier rows of the call (0 * NaN), never another sequence.  x_dtype (q and out) bf16 needs a bf16 cache: products on the bf16 matrix pipe with fp32
- * sums; x_dtype fp32 takes either cache, fp32 throughout.  head_dim 64 or 128; any n_q that is a multiple of n_kv.  `workspace`: at least
+ * sums; x_dtype fp32 takes either cache, fp32 throughout.  head_dim 64 or 128; any n_q that is a multiple of n_kv; at most 64 GB of
+ * cache and 2^24 pages.  `workspace`: at least
  * csm_ops_paged_attention_workspace bytes (16 B), contents undefined before and after; calls that may overlap in time need one each.  out may be q. */
 typedef struct {
   csm_ops_paged_t c;

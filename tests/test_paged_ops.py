@@ -156,14 +156,14 @@ class Cache:
             self.table[b, :k] = order[at:at + k]
             at += k
         self.prefix = order[:npf].to(DEV)
-        perm = {"phsd": (0, 1, 2, 3), "pshd": (0, 2, 1, 3), "hpsd": (1, 0, 2, 3)}[layout]
         shape = (n, n_kv, page, hd)
 
-        def make():
+        def make(layout):
+            perm = {"phsd": (0, 1, 2, 3), "pshd": (0, 2, 1, 3), "hpsd": (1, 0, 2, 3)}[layout]
             x = torch.randn(shape, generator=g).to(dtype)
             y = torch.empty([shape[i] for i in perm], dtype=dtype, device=DEV).permute([perm.index(i) for i in range(4)])
             return y.copy_(x)
-        self.k, self.v = make(), make()
+        self.k, self.v = (make(l) for l in (("hpsd", "pshd") if layout == "mixed" else (layout, layout)))
         self.table, self.lens = self.table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
 
     def args(self):
@@ -298,7 +298,7 @@ def test_append_types_and_heads(x, c, n_q, n_kv, hd):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("page", [1, 2, 16, 128])
-@pytest.mark.parametrize("layout", ["phsd", "pshd", "hpsd"])
+@pytest.mark.parametrize("layout", ["phsd", "pshd", "hpsd", "mixed"])
 def test_append_pages_and_layouts(page, layout):
     _append_case([40, 3, 131], [40, 2, 5], 4, 2, 64, BF16, BF16, page=page, layout=layout, wide=64, tail=3)
 
@@ -373,10 +373,12 @@ def test_attention_prefix_lengths(prefix, x, c):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("page", [1, 4, 32, 128, 1024])
-@pytest.mark.parametrize("layout", ["phsd", "pshd", "hpsd"])
+@pytest.mark.parametrize("layout", ["phsd", "pshd", "hpsd", "mixed"])
 def test_attention_pages_and_layouts(page, layout):
     _attn_case([3, 77, 200], [1, 1, 1], 4, 2, 64, BF16, BF16, page=page, prefix=50, layout=layout)
     _attn_case([30, 77], [30, 50], 4, 2, 128, F32, BF16, page=page, prefix=21, layout=layout)
+    _attn_case([30, 77], [30, 50], 4, 2, 64, BF16, BF16, page=page, prefix=21, layout=layout)
+    _attn_case([30, 77], [1, 50], 4, 2, 64, F32, F32, page=page, prefix=21, layout=layout)
 
 
 @pytest.mark.gpu
