@@ -25,6 +25,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-val
 # stamped with ITS sources.  packed-fp32-ops off: no v_pk_*_f32 in these kernels
 OPS_SRC = os.path.join(CSRC, "ops")
 OPS_LIB = os.path.join(HERE, "libcsm_ops.so")
+OPS_BINDING = os.path.join(HERE, "_ops_binding.so")   # csrc/ops/binding.cpp: the same calls for torch tensors, built against the installed torch
 OPS_UNITS = ["ops_api", "paged_append", "paged_attn", "sample_filtered"]
 OPS_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Wno-pass-failed",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
@@ -91,10 +92,10 @@ def build_library(force: bool = False, verbose: bool = False, defines=(), out: s
 
 
 def build_ops_library(force: bool = False, verbose: bool = False) -> str:
-    """libcsm_ops.so from csrc/ops (include/csm_ops.h); reused when it is newer than its sources unless `force`."""
-    deps = [os.path.join(OPS_SRC, f) for f in os.listdir(OPS_SRC) if f.endswith((".hip", ".h"))]
+    """libcsm_ops.so and _ops_binding.so from csrc/ops (include/csm_ops.h); reused when they are newer than their sources unless `force`."""
+    deps = [os.path.join(OPS_SRC, f) for f in os.listdir(OPS_SRC) if f.endswith((".hip", ".h", ".cpp"))]
     deps += [os.path.join(CSRC, "common.h"), os.path.join(os.path.dirname(HERE), "include", "csm_ops.h")]
-    if not force and os.path.exists(OPS_LIB) and os.path.getmtime(OPS_LIB) >= max(os.path.getmtime(f) for f in deps):
+    if not force and all(os.path.exists(o) and os.path.getmtime(o) >= max(os.path.getmtime(f) for f in deps) for o in (OPS_LIB, OPS_BINDING)):
         return OPS_LIB
     hipcc, obj_dir = _hipcc(), os.path.join(OPS_SRC, "build")
     os.makedirs(obj_dir, exist_ok=True)
@@ -107,13 +108,36 @@ def build_ops_library(force: bool = False, verbose: bool = False) -> str:
         if verbose:
             print(f"[build] ops/{u}.o", file=sys.stderr)
 
-    with ThreadPoolExecutor(min(len(OPS_UNITS), os.cpu_count() or 4)) as ex:
+    with ThreadPoolExecutor(min(len(OPS_UNITS) + 1, os.cpu_count() or 4)) as ex:
+        binding = ex.submit(_compile_binding, obj_dir, verbose)
         list(ex.map(compile_one, OPS_UNITS))
+        binding.result()
     cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *[os.path.join(obj_dir, u + ".o") for u in OPS_UNITS], "-o", OPS_LIB]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr[-4000:]}")
+    import torch
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["g++", "-shared", os.path.join(obj_dir, "binding.o"), "-o", OPS_BINDING, "-L" + HERE, "-l:" + os.path.basename(OPS_LIB), "-Wl,-rpath,$ORIGIN",
+           "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link of the binding failed:\n{r.stderr[-4000:]}")
     return OPS_LIB
+
+
+def _compile_binding(obj_dir: str, verbose: bool):
+    import sysconfig
+    import torch
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    dirs = [inc, os.path.join(inc, "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"], os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *["-isystem" + d for d in dirs], "-c", os.path.join(OPS_SRC, "binding.cpp"), "-o", os.path.join(obj_dir, "binding.o")]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for ops/binding.cpp:\n{r.stderr[-4000:]}")
+    if verbose:
+        print("[build] ops/binding.o", file=sys.stderr)
 
 
 if __name__ == "__main__":

@@ -50,20 +50,6 @@ def test_header_is_plain_c_and_structs_match(tmp_path):
         assert got == [n, str(C.sizeof(s))] + [str(getattr(s, f[0]).offset) for f in s._fields_]
 
 
-def test_packed_arguments_match_the_structures():
-    """the wrappers pack their arguments; every value must land in the field that the header names"""
-    def leaves(s):
-        for f in s._fields_:
-            v = getattr(s, f[0])
-            if isinstance(v, C.Structure):
-                yield from leaves(v)
-            else:
-                yield v
-    for struct_type, pack, n in ((ops.RopeAppendArgs, ops._PACK_APPEND, 30), (ops.AttentionArgs, ops._PACK_ATTENTION, 32), (ops.SampleArgs, ops._PACK_SAMPLE, 17)):
-        values = list(range(1, n + 1))
-        assert list(leaves(struct_type.from_buffer_copy(pack(*values)))) == values
-
-
 def _paged_args(p, **over):
     """a valid description of 2 sequences on made-up addresses: only ever handed to calls that must refuse it"""
     for k, v in dict(dict(k=1 << 20, v=1 << 21, dtype=1, n_pages=4, page_size=16, n_kv=2, head_dim=64, k_page_stride=2048, k_head_stride=1024, k_slot_stride=64,
@@ -89,7 +75,8 @@ def test_append_refusals(over):
 
 @pytest.mark.parametrize("over", [
     dict(dtype=0), dict(x_dtype=2), dict(head_dim=32), dict(head_dim=96), dict(n_q=3), dict(n_q=0), dict(prefix_len=-1), dict(prefix_len=33, prefix_pages=2, prefix_table=1 << 26),
-    dict(prefix_len=5, prefix_pages=1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(out=(1 << 25) + 4), dict(q_stride=100), dict(rows=1), dict(page_size=3)])
+    dict(prefix_len=5, prefix_pages=1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(out=(1 << 25) + 4), dict(q_stride=100), dict(rows=1), dict(page_size=3),
+    dict(n_pages=(1 << 24) + 1), dict(k_page_stride=1 << 30)])
 def test_attention_refusals(over):
     lib = ops.load_ops_library()
     a = ops.AttentionArgs(q=1 << 24, out=1 << 25, q_stride=256, out_stride=256, x_dtype=1, n_q=4, scale=0.125, workspace=1 << 28, workspace_bytes=1 << 27)
@@ -137,6 +124,8 @@ def test_cpu_tensors_are_refused():
         paged_rope_append(z[0], z[0], z[0], z[None], z[None], i, i[0])
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         sample_filtered(z[0], z[0, :, 0])
+    with pytest.raises(TypeError):
+        sample_filtered([[1.0]], z)
 
 
 # ---- plain implementations in 64 bits ------------------------------------------------------------------------------------
@@ -735,6 +724,23 @@ def test_python_refusals():
             paged_rope_append(qkv, tab, tab, *c.args())
     with pytest.raises(ValueError):
         paged_rope_append(torch.zeros(2, 8 * 64, device=DEV), tab, tab[:, :16], *c.args())
+
+
+@pytest.mark.gpu
+def test_numbers_and_lonely_strides():
+    """settings are whole numbers where they count something; the stride of a dimension of size one is never looked at"""
+    x, u = torch.randn(2, 9, device=DEV), torch.rand(2, device=DEV)
+    for bad, kind in ((dict(topk=2.0), TypeError), (dict(topk=1 << 70), ValueError), (dict(topk=1 << 31), ValueError), (dict(top_p="1"), TypeError), (dict(min_p=None), TypeError)):
+        with pytest.raises(kind):
+            sample_filtered(x, u, **bad)
+    c = Cache([5], 16, 1, 64, F32)
+    q = torch.randn(1, 4, 64, device=DEV)
+    odd = lambda t, *d: t.as_strided(t.shape, [7 if i in d else n for i, n in enumerate(t.stride())])  # noqa: E731
+    want = paged_prefix_attention(q, c.k, c.v, c.table, c.lens)
+    assert torch.equal(paged_prefix_attention(odd(q, 0), odd(c.k, 1), odd(c.v, 1), odd(c.table, 0), c.lens), want)
+    assert torch.equal(sample_filtered(odd(x[:1], 0), u[:1]), sample_filtered(x[:1], u[:1]))
+    qkv, tab = torch.randn(1, 6 * 64, device=DEV), torch.rand(8, 32, device=DEV)
+    assert torch.equal(paged_rope_append(odd(qkv, 0), tab, tab, odd(c.k, 1), c.v, c.table, c.lens), paged_rope_append(qkv, tab, tab, c.k, c.v, c.table, c.lens))
 
 
 # ---- the three as one serving step -----------------------------------------------------------------------------------------
