@@ -87,14 +87,20 @@ struct Prod<XT, bf16_t, HD> {
   b16x8 q[NQ][T];
   struct Tile { u32x4 k[NG][T], v[NV]; };
 
-  __device__ __forceinline__ void load_q(const XT* p, int g, uint32_t flip) {
+  struct Raw { W8<XT> w[T]; };   // q as it lies in memory
+  static __device__ __forceinline__ void load_q(Raw& raw, const XT* p, int g) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) raw.w[t].zero();
+    if (p)
+#pragma unroll
+      for (int t = 0; t < T; ++t) raw.w[t].load(p + 32 * t + 8 * g);
+  }
+  static __device__ __forceinline__ void make_q(const Raw& raw, b16x8 (&q)[NQ][T], uint32_t flip) {
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       float x[8];
-      W8<XT> w;
-      if (p) w.load(p + 32 * t + 8 * g); else w.zero();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(__float_as_uint(w.get(i)) ^ flip);
+      for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(__float_as_uint(raw.w[t].get(i)) ^ flip);
       b16x8 f[NQ];
       split8<NQ>(x, f);
 #pragma unroll
@@ -168,14 +174,19 @@ struct Prod<float, float, HD> {
   f32x4 q[U];
   struct Tile { f32x4 k[NG][U], v[NV]; };
 
-  __device__ __forceinline__ void load_q(const float* p, int g, uint32_t flip) {
+  struct Raw { f32x4 w[U]; };
+  static __device__ __forceinline__ void load_q(Raw& raw, const float* p, int g) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      f32x4 x = (f32x4)(0.f);
-      if (p) x = *reinterpret_cast<const f32x4*>(p + 16 * u + 4 * g);
+    for (int u = 0; u < U; ++u) raw.w[u] = (f32x4)(0.f);
+    if (p)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) q[u][e] = __uint_as_float(__float_as_uint(x[e]) ^ flip);
-    }
+      for (int u = 0; u < U; ++u) raw.w[u] = *reinterpret_cast<const f32x4*>(p + 16 * u + 4 * g);
+  }
+  static __device__ __forceinline__ void make_q(const Raw& raw, f32x4 (&q)[U], uint32_t flip) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[u][e] = __uint_as_float(__float_as_uint(raw.w[u][e]) ^ flip);
   }
   static __device__ __forceinline__ int k_piece(int lane) { return 4 * (lane >> 4); }
   static __device__ __forceinline__ int v_piece(int lane) { return (lane % LPK) * 4; }
@@ -228,7 +239,7 @@ struct KeyAxis {
 };
 
 template <typename XT, typename CT, int HD>
-__device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const Prod<XT, CT, HD>& pr, const KeyAxis& ax, int kvh, int k0, int k1, int first, int step,
+__device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const XT* qp, const KeyAxis& ax, int kvh, int k0, int k1, int first, int step,
                                             int lim, int lim_min, char* lds, f32x4 (&o)[HD / 16], float& m, float& l) {
   using P = Prod<XT, CT, HD>;
   constexpr int NG = P::NG, KT = 16 * NG;
@@ -269,9 +280,14 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const Prod<XT, 
   if (j >= k1) return;
   typename P::Tile t;
   uint32_t valid;
+  // a short launch is a chain of memory latencies: q is on its way while the page numbers and the first tile come
+  P pr;
+  typename P::Raw raw;
   look(j);
+  P::load_q(raw, qp, g);
   fetch(t, valid);
   look(j + hop);
+  P::make_q(raw, pr.q, a.q_flip);
   for (; j < k1; j += hop) {
     constexpr uint32_t ALL = NG == 2 ? 0xffffffffu : 0xffffu;
     f32x4 s[NG];
@@ -329,7 +345,7 @@ struct Wide {
   f32x4 o[RT][HD / 16], l4[RT];
   float m[RT];
 
-  __device__ __forceinline__ void run(const AttnOpArgs& a, const KeyAxis& ax, int kvh, int k0, int k1, const int (&lim)[RT], const int (&lim_min)[RT], int n_rt, char* lds) {
+  __device__ __forceinline__ void run(const AttnOpArgs& a, const XT* const (&qp)[RT], const KeyAxis& ax, int kvh, int k0, int k1, const int (&lim)[RT], const int (&lim_min)[RT], int n_rt, char* lds) {
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g = lane >> 4;
     const int ch = tid % CH, key0 = tid / CH;
     const char* kb = reinterpret_cast<const char*>(reinterpret_cast<const bf16_t*>(a.k) + kvh * a.c.kh + ch * 8);
@@ -369,9 +385,14 @@ struct Wide {
       }
       return __ballot(ok);
     };
+    typename Prod<XT, bf16_t, HD>::Raw raw[RT];   // (on its way while the page numbers and the first tile come)
     look(k0);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) Prod<XT, bf16_t, HD>::load_q(raw[r], qp[r], g);
     uint64_t valid = fetch();
     look(k0 + KEYS);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) Prod<XT, bf16_t, HD>::make_q(raw[r], q[r], a.q_flip);
     // LDS places of this lane: what it stages (keys KPP apart), its K operands (16-key tiles and 32-element steps apart), its V columns
     int st[NL], kp[T], vp[HD / 16];
 #pragma unroll
@@ -595,6 +616,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void paged_attn_kernel(At
       using Wd = Wide<XT, HD>;
       Wd w;
       int lim[Wd::RT], lim_min[Wd::RT], n_rt = 0;
+      const XT* qp[Wd::RT];
 #pragma unroll
       for (int r = 0; r < Wd::RT; ++r) {
         const int first = 16 * (wave + 4 * r), f = f0 + first + li;
@@ -602,21 +624,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void paged_attn_kernel(At
         lim[r] = own ? sees(f / a.rep) : a.prefix_len;
         lim_min[r] = own ? sees((f0 + first) / a.rep) : a.prefix_len;   // rows ascend: the first sees least
         const bool on = first + li < live;
-        const XT* qp = on ? reinterpret_cast<const XT*>(a.q) + (row0 + f / a.rep) * a.q_stride + (int64_t)(kvh * a.rep + f % a.rep) * HD : nullptr;
-#pragma unroll
-        for (int t = 0; t < Wd::T; ++t) {
-          float x[8];
-          W8<XT> raw;
-          if (qp) raw.load(qp + 32 * t + 8 * g); else raw.zero();
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(__float_as_uint(raw.get(i)) ^ a.q_flip);
-          b16x8 piece[Wd::NQ];
-          split8<Wd::NQ>(x, piece);
-#pragma unroll
-          for (int n = 0; n < Wd::NQ; ++n) w.q[r][n][t] = piece[n];
-        }
+        qp[r] = on ? reinterpret_cast<const XT*>(a.q) + (row0 + f / a.rep) * a.q_stride + (int64_t)(kvh * a.rep + f % a.rep) * HD : nullptr;
       }
-      w.run(a, ax, kvh, k0, k1, lim, lim_min, n_rt, lds);
+      w.run(a, qp, ax, kvh, k0, k1, lim, lim_min, n_rt, lds);
 #pragma unroll
       for (int r = 0; r < Wd::RT; ++r) {
         const int first = 16 * (wave + 4 * r), f = f0 + first + li;
@@ -634,10 +644,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void paged_attn_kernel(At
   const int f = f0 + mine + li, row = row0 + f / a.rep, head = kvh * a.rep + f % a.rep;
   const bool row_live = li < n_mine;
   if (n_mine > 0) {
-    P pr;
-    pr.load_q(row_live ? reinterpret_cast<const XT*>(a.q) + row * a.q_stride + (int64_t)head * HD : nullptr, g, a.q_flip);
+    const XT* qp = row_live ? reinterpret_cast<const XT*>(a.q) + row * a.q_stride + (int64_t)head * HD : nullptr;
     const int lim = own ? sees(f / a.rep) : a.prefix_len, lim_min = own ? sees((f0 + mine) / a.rep) : a.prefix_len;   // rows ascend: the first sees least
-    wave_attend<XT, CT, HD>(a, pr, ax, kvh, k0, k1, by_keys ? wave : 0, by_keys ? NW : 1, lim, lim_min, my_lds, o, m, l);
+    wave_attend<XT, CT, HD>(a, qp, ax, kvh, k0, k1, by_keys ? wave : 0, by_keys ? NW : 1, lim, lim_min, my_lds, o, m, l);
   }
   if (by_keys) {   // join the waves: every one rescales to the common reference and leaves its rows in LDS
     if (g == 0) { ml_s[wave][li][0] = m; ml_s[wave][li][1] = l; }
@@ -687,23 +696,32 @@ __global__ __launch_bounds__(AT) void paged_attn_join_kernel(AttnOpArgs a) {
   if (at >= (int64_t)c.rows * a.n_q) return;
   const int row = (int)(at / a.n_q), head = (int)(at - (int64_t)row * a.n_q);
   const int seq = c.cu ? ops_find_seq(c.cu, c.n_seqs, row) : row;
-  if (seq < 0 || c.lens[seq] < 0) return;
+  if (seq < 0) return;
+  const int len = c.lens[seq];
+  const float* p = a.part + at * a.nsplit * HD + d;
+  // the first partial results are on their way while the weights are made (a padded sequence's hold anything, and are not stored)
+  constexpr int AHEAD = 4;
+  vec v[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) v[i] = *reinterpret_cast<const vec*>(p + (int64_t)min(2 * i + (lane >> 5), a.nsplit - 1) * HD);
   const float2 x = lane < a.nsplit ? a.ml[at * a.nsplit + lane] : make_float2(-INFINITY, 0.f);
   const float top = wave_max(x.x);
   const float w = x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(x.x - top);   // (no key: sum 0; nothing but NaN: let it through)
   const float inv = inverse(wave_sum(w * x.y));
-  const float* p = a.part + at * a.nsplit * HD + d;
   vec o = (vec)(0.f);
-#pragma unroll 4
-  for (int s0 = 0; s0 < a.nsplit; s0 += 2) {
-    const int s = min(s0 + (lane >> 5), a.nsplit - 1);
+  auto add = [&](int s0, const vec& val) {
     const float lo = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s0));
     const float hi = s0 + 1 < a.nsplit ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s0 + 1)) : 0.f;
     const float ws = lane < 32 ? lo : hi;
-    const vec v = *reinterpret_cast<const vec*>(p + (int64_t)s * HD);
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] += ws * v[i];
-  }
+    for (int i = 0; i < N; ++i) o[i] += ws * val[i];
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (2 * i < a.nsplit) add(2 * i, v[i]);
+#pragma unroll 4
+  for (int s0 = 2 * AHEAD; s0 < a.nsplit; s0 += 2) add(s0, *reinterpret_cast<const vec*>(p + (int64_t)min(s0 + (lane >> 5), a.nsplit - 1) * HD));
+  if (len < 0) return;
   XT* y = reinterpret_cast<XT*>(a.out) + row * a.out_stride + (int64_t)head * HD + d;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -755,9 +773,11 @@ static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
   const bool narrow = c.n_seqs > 0 && flat / c.n_seqs <= 16;   // decode: items wait for memory and are cheap to cut; a tile of many rows has much to join
   const int64_t axis = p->prefix_len + own_cap;
   // few sequences and a short axis: ONE launch of tall workgroups (16 or 8 waves split the keys, the prefix among them) -- the prefix is read once per
-  // sequence, from L2, and there is nothing to join.  32 sequences, 200 + 50 slots of 64 bf16: 7.4 us against 10.7; 1 sequence, 512 + 130: 8.8
-  // against 7.8 and a launch of 3.5 us saved on the host; 1 sequence, 512 + 1000: 12.5 against 8.6, and 128 sequences, 200 + 50: 22 against 12
-  a.tall = narrow && p->prefix_len > 0 && own_tiles * c.n_kv <= 256 && axis * c.head_dim * (c.dtype == CSM_OPS_BF16 ? 2 : 4) <= 128 * 1024;
+  // sequence, from L2, and there is nothing to join.  The axis may be longer where the sequences alone give the CUs a workgroup each.  Measured (us, tall
+  // against cut, 64 bf16 or fp32): 200 + 50 slots 6.2 / 6.7 and 8.4 / 7.1 for 1 sequence, 6.8 / 8.8 and 9.2 / 10.2 for 32; 512 + 130: 8.2 / 7.1 and
+  // 13.6 / 8.0 for 1, 8.9 / 9.0 and 15.3 / 14.8 for 32; 512 + 1000: 12.5 / 11.1 and 25 / 18.5 for 16, 14.6 / 17.5 and 26.8 / 25.7 for 32; 128: 22 / 12 at 200 + 50
+  const int64_t full = own_tiles * c.n_kv;
+  a.tall = narrow && p->prefix_len > 0 && full <= 256 && axis * c.head_dim * (c.dtype == CSM_OPS_BF16 ? 2 : 4) <= 64 * 1024 + (full > 128 ? (full - 128) * 2048 : 0);
   // sequences that bring two tiles of 16 rows and more of their own read the prefix with them: nothing to share, nothing to join
   a.with_prefix = a.tall || (p->prefix_len > 0 && c.cu_rows && c.n_seqs > 0 && flat / c.n_seqs >= 32);
   const int64_t np = p->prefix_len && !a.with_prefix ? (flat + ROWS - 1) / ROWS : 0;
