@@ -279,6 +279,14 @@ struct RegRow {
   uint32_t key[E];
   uint64_t w[E];
   int per;
+  template <typename K>
+  __device__ __forceinline__ void weigh_all(const Weigh& weigh) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      w[e] = 0;
+      if (e < per && key[e]) w[e] = weigh(K::value(key[e]));
+    }
+  }
   template <bool MASS>
   __device__ __forceinline__ void stat(uint32_t c, uint32_t& cnt, uint64_t& mass) const {   // cnt: of the wave
     cnt = 0;
@@ -351,11 +359,15 @@ struct Hist {
     usable = exact || (span > 0.f && span < INFINITY && inv < INFINITY);
   }
   __device__ __forceinline__ uint32_t bin(uint32_t key) const { return exact ? key_max - key : min((uint32_t)((top - K::value(key)) * inv), (uint32_t)N - 1); }
-  template <bool MASS, int E>
-  __device__ __forceinline__ void build(const RegRow<E>& r, Block<NT>& blk) {
+  // TABLE, and a bin is a key: the weights are not there yet.  Each is computed once per key, not once per entry, and a bin's mass is count * weight --
+  // the bf16 list of a long row holds 12 000 entries of some 250 keys (64 rows of 128 256, top_p 0.9: 48.5 -> 43.3 us; whole rows seldom span few
+  // enough keys, there the second way only makes the code longer: 12.2 -> 12.7)
+  template <bool MASS, bool TABLE, int E>
+  __device__ __forceinline__ void build(RegRow<E>& r, Block<NT>& blk, const Weigh& weigh) {
+    const bool table = TABLE && exact;
     const int tid = threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { h->c[i * NT + tid] = 0; if (MASS) h->m[i * NT + tid] = 0; }
+    for (int i = 0; i < 4; ++i) { h->c[i * NT + tid] = 0; if (MASS && !table) h->m[i * NT + tid] = 0; }
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -363,7 +375,7 @@ struct Hist {
       if (r.key[e]) {
         const uint32_t b = bin(r.key[e]);
         atomicAdd(&h->c[b], 1u);
-        if (MASS) atomicAdd(reinterpret_cast<unsigned long long*>(&h->m[b]), (unsigned long long)r.w[e]);
+        if (MASS && !table) atomicAdd(reinterpret_cast<unsigned long long*>(&h->m[b]), (unsigned long long)r.w[e]);
       }
     }
     __syncthreads();
@@ -371,11 +383,20 @@ struct Hist {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       c[i] = h->c[4 * tid + i];
-      m[i] = MASS ? h->m[4 * tid + i] : 0;
+      m[i] = MASS && !table ? h->m[4 * tid + i] : 0;
+      if (table && c[i]) {
+        const uint64_t each = weigh(K::value(key_max - (4 * tid + i)));
+        h->m[4 * tid + i] = each;
+        m[i] = c[i] * each;
+      }
       cb += c[i];
       mb += m[i];
     }
-    blk.before2(cb, mb, all_c, all_m);
+    blk.before2(cb, mb, all_c, all_m);   // (its barrier is between the weights and their use)
+    if (table) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) r.w[e] = r.key[e] ? h->m[key_max - r.key[e]] : 0;
+    }
   }
   // the bin in which the running count (or mass) from the top first reaches its target, which the row does reach
   template <bool MASS>
@@ -473,7 +494,7 @@ __device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, HistLds<
   Hist<K, NT> hist(lds, key_min, key_max);
   if (n > 64) {
     if (!hist.usable) return -2;
-    hist.template build<false>(r, blk);
+    hist.template build<false, false>(r, blk, Weigh{});
     const Where w = hist.template locate<false>(k, 0.0);
     cnt = w.above + w.in;
     last = w.bin;
@@ -505,9 +526,9 @@ __device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, HistLds<
   return __ffs(in) - 1;
 }
 
-// filters and draw on entries in registers; returns the place (e, in the thread that owns it) or -1.  `base`: the mass that top_p refers to when
+// filters and draw on entries in registers, with their weights unless TABLE; returns the place (e, in the thread that owns it) or -1.  `base`: the mass that top_p refers to when
 // it is not that of these entries (< 0: it is).  `enough` comes back false when these entries cannot hold the nucleus.
-template <typename K, int E, int NT>
+template <typename K, bool TABLE, int E, int NT>
 __device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block<NT>& blk, HistLds<NT>* lds, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, double base, bool& enough) {
   enough = true;
   Cut cut{key_min, 1u, 1u};
@@ -515,8 +536,9 @@ __device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block<NT>& blk, His
   Hist<K, NT> hist(lds, key_min, key_max);
   bool binned = hist.usable && (cut_k || s.top_p < 1.f);
   uint64_t mass = 0;
+  if (TABLE && !(binned && hist.exact)) r.template weigh_all<K>(weigh);
   if (binned) {
-    hist.template build<true>(r, blk);
+    hist.template build<true, TABLE>(r, blk, weigh);
     mass = hist.all_m;
   }
   if (cut_k) {
@@ -638,7 +660,7 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
       if (i < r.per) r.w[i] = weigh(v[i]);
     }
     bool enough;
-    e = filter_and_draw<K>(r, blk, &hist, &few, weigh, s, n, key_min, key_max, -1.0, enough);
+    e = filter_and_draw<K, false>(r, blk, &hist, &few, weigh, s, n, key_min, key_max, -1.0, enough);
   }
   if (e >= 0) a.out[row] = first + e;
 }
@@ -741,7 +763,7 @@ __global__ __launch_bounds__(256) void sample_threshold_kernel(SampleOpArgs a) {
       Hist<K, NT> hist(&lds, K::key(ex.mn), K::key(ex.mx));
       Where w{0, 0, ~0u, 0};
       if (hist.usable) {
-        hist.template build<false>(r, blk);
+        hist.template build<false, false>(r, blk, Weigh{});
         w = hist.template locate<false>(rank, 0.0);
       }
       if (hist.exact) thr = hist.key_max - w.bin;
@@ -955,12 +977,9 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
     int e = -2;
     if (s.k && s.k <= 64) e = draw_small<K>(r, blk, &hist, &order, weigh, s, n, min((uint32_t)s.k, n), thr, key_max);
     if (e == -2) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        r.w[i] = 0;
-        if (i < r.per) r.w[i] = r.key[i] ? weigh(K::value(r.key[i])) : 0;
-      }
-      e = filter_and_draw<K>(r, blk, &hist, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << a.shift), enough);
+      constexpr bool TABLE = sizeof(XT) == 2;
+      if (!TABLE) r.template weigh_all<K>(weigh);
+      e = filter_and_draw<K, TABLE>(r, blk, &hist, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << a.shift), enough);
     }
     if (e >= 0) {
       const uint32_t p = tid * r.per + e;
