@@ -9,6 +9,10 @@
 //   up to 16 live rows (decode): the launch waits for memory.  The four waves split the keys, each streams its own, and they join through LDS.
 //   more rows, bf16 cache:       64-key tiles of K and V are staged once per workgroup in LDS (two buffers), every wave takes 16-row tiles.
 //   more rows, fp32 cache:       every wave streams all keys for its 16 rows.
+// Measured: 128 sequences of some 1500 own slots behind 4096 (32 / 8 heads of 64, bf16): 416 MB in 83 + 5 us, 4.8 TB/s of the 4.9 that a large copy reaches.
+// 2 sequences of 4096 new rows: 136 GFLOP in 187 us, 730 TFLOP/s of the 1330 that a large bf16 product reaches; 2162 ragged rows behind 2048 slots 485,
+// where 664 workgroups share 256 CUs.  Without its exponentials that launch (at 220 us) took 14 percent less, without the second product 15, without half of the
+// first 13, without fetching tiles 11: no single one bounds it.  One sequence behind 512 slots: 4.6 + 2.3 us, a chain of latencies.
 //
 // Per wave and 16 query rows, both products are transposed so that a lane owns one query row from score to result:
 //   S^T[key][row] = K Q^T   lane (row = lane % 16, g = lane / 16) ends with the scores of keys 4g .. 4g+3 of each 16-key group
@@ -335,7 +339,8 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const XT* qp, c
 
 // ---- many rows on a bf16 cache: 64-key tiles shared by the workgroup ---------------------------------------------------------------------------
 // bf16 queries: two 16-row tiles per wave, so that a K or V operand read from LDS feeds two products; p is ONE bf16 piece here -- a second rounding of
-// the size of the result's own (the sum l is of the same rounded p) against half again as many matrix instructions.  fp32 queries: one tile
+// the size of the result's own (the sum l is of the same rounded p) against half again as many matrix instructions: 88 -> 107 us ragged, 220 -> 271 for
+// 2 x 4096 rows, for a relative error of 0.0017 instead of 0.0022.  fp32 queries: one tile
 // per wave, q and p in three exact pieces.  l comes off the matrix pipe too, as a product with ones.
 template <typename XT, int HD>
 struct Wide {
@@ -480,7 +485,7 @@ struct Wide {
         for (int n = NP - 1; n >= 0; --n) l4[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][h][n], l4[r], 0, 0, 0);
       }
     }
-    // the wave goes first on the matrix pipe while the others are at their softmax: 2 sequences of 4096 rows 193 -> 187 us, 2153 ragged rows behind 2048 slots
+    // the wave goes first on the matrix pipe while the others are at their softmax: 2 sequences of 4096 rows 193 -> 187 us, 2162 ragged rows behind 2048 slots
     // 79 -> 77.  (Four waves per SIMD instead of three need spills: 220 and 100)
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -762,9 +767,9 @@ static int check(const csm_ops_attention_t* p) {
 }
 
 // How the work is cut.  Items should fill 256 CUs (of two to four workgroups each), but a short item is mostly start-up, and every piece costs a
-// partial result per row, written and read again.  Measured (us): 128 sequences behind 4096 slots, prefix in 2 / 4 / 8 / 16 pieces 93 / 94 / 95 / 103 and
-// alone 48 / 30 / 22 / 25; 64 sequences of 128-wide heads behind 2048 slots in 4 / 8 / 16 pieces 27 / 20 / 24; 16 fp32 sequences behind 512 slots in
-// 4 / 8 pieces 16 / 13; own slots of 128 sequences whole / halved 95 / 90; tiles of many rows whole / in 3 pieces 88 / 110.
+// partial result per row, written and read again.  Measured (us): 128 sequences behind 4096 slots, prefix in 4 / 8 / 16 pieces 86 / 88 / 96, own slots in
+// 1 / 2 / 3 / 5 pieces 92 / 88 / 90 / 92; 64 sequences of 128-wide heads behind 2048 slots, prefix in 4 / 8 / 16 pieces 25 / 18.5 / 22, own in 2 / 4 / 5
+// pieces 18.7 / 18.5 / 19.8; 16 fp32 sequences behind 512 slots, prefix in 4 / 8 / 16 pieces 14 / 11.4 / 11.9; tiles of many rows whole / in 3 pieces 88 / 110.
 static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
   const csm_ops_paged_t& c = p->c;
   a.c = ops_paged(c);

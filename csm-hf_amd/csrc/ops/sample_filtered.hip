@@ -13,6 +13,11 @@
 //   larger V:    three launches, so that few rows still use many CUs: a threshold near the 12 288th largest from 4 096 samples; per chunk of
 //                8 192 entries its maximum, its mass and the entries above the threshold; per row the cuts and the draw on those entries.
 //                Where they are not enough (a flat row whose nucleus is larger), the same search streams over the row.
+//
+// What bounds it: not the bytes.  One row of 2051 fp32: 7.0 us, the chain of steps; 512 of them, each with its own filters: 13.5 us for 4.2 MB (0.9 at the rate
+// of a large copy) -- two workgroups a CU, whose steps overlap little.  64 rows of 128 256 bf16, top_p alone: 7.4 + 19.4 + 17.1 us for 16.4 MB (3.4); the
+// chunks' 8.2 million fp64 exponentials (21 operations of 8 clocks a wave) take 11 of the 19, in the list's 17 are 4 to fetch it, 5 for the histogram, 3 for
+// the draw and the heads' sums.
 #include "ops_common.h"
 #include <math.h>
 
@@ -34,6 +39,7 @@ struct SampleOpArgs {
 constexpr int LIST = 1024 * 16;           // entries that fit the registers of a workgroup
 constexpr int SAMPLES = 4096, AIM = LIST * 3 / 4;   // the list's threshold is a sample's order statistic that aims at this many entries: at V = 131 072
                                                     // their number scatters by 613, LIST is 6.7 of that away
+// (a chunk of 8192 is 32 entries a thread: 16 chunks of a row of 128 256, so that 16 rows already fill the CUs)
 constexpr int CHUNK = 8192, CHUNK_CAP = 2048, MAX_V = 1 << 21, MAX_CHUNKS = MAX_V / CHUNK;
 struct ChunkHead { double mass; float mx; int32_t at; uint32_t count, pad; };   // mass relative to the chunk's own maximum, `at` its first place
 
@@ -1133,7 +1139,8 @@ extern "C" int csm_ops_sample_filtered(const csm_ops_sample_t* p, void* stream) 
   hipStream_t st = (hipStream_t)stream;
   const bool b = p->x_dtype == CSM_OPS_BF16;
   const dim3 grid(p->rows);
-  // few waves: each repeats the scalar part of every step, on 4 waves per SIMD it would take four times as long
+  // as few waves as hold the row at 4 or 16 entries a thread: every wave repeats the scalar part of every step, and four waves on a SIMD take turns at it.
+  // Rows of 2051 under top_p on 4 waves and on 16 (us): one 9.4 / 12.8, 512 of them 11.8 / 24.9; 512 of 1000 with 4 and with 16 entries 8.0 / 10.5
   if (p->V <= 256 * 4) {
     if (b) hipLaunchKernelGGL((sample_short_kernel<256, 4, bf16_t>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((sample_short_kernel<256, 4, float>), grid, dim3(256), 0, st, a);
