@@ -106,6 +106,10 @@ extern "C" int csm_ops_paged_rope_append(const csm_ops_rope_append_t* p, void* s
   if (!ops_aligned(p->qkv) || !ops_aligned(p->q_out) || !ops_aligned(p->cos) || !ops_aligned(p->sin) || !ops_stride16(p->qkv_stride, p->x_dtype) ||
       !ops_stride16(p->q_out_stride, p->x_dtype))
     return ops_fail(CSM_OPS_ERR_ARG, "qkv, q_out, cos and sin must start on 16 bytes and have rows of multiples of 16 bytes");
+  if (c.rows > 1 && p->q_out_stride < (int64_t)p->n_q * c.head_dim) return ops_fail(CSM_OPS_ERR_ARG, "rows of q_out overlap");
+  const int64_t size[3] = {c.n_pages, c.n_kv, c.page_size}, steps[6] = {c.k_page_stride, c.k_head_stride, c.k_slot_stride, c.v_page_stride, c.v_head_stride, c.v_slot_stride};
+  for (int i = 0; i < 6; ++i)
+    if (size[i % 3] > 1 && steps[i] < c.head_dim) return ops_fail(CSM_OPS_ERR_ARG, "slots of k_cache or v_cache overlap");
   const int64_t units = (int64_t)(p->n_q + 2 * (int64_t)c.n_kv) * (c.head_dim / 16), total = units * c.rows;
   if (total > 0x7fffff00) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
   AppendArgs a;

@@ -763,6 +763,7 @@ static int check(const csm_ops_attention_t* p) {
   if (!p->q || !p->out || (p->prefix_len && !p->prefix_table)) return ops_fail(CSM_OPS_ERR_ARG, "null pointer");
   if (!ops_aligned(p->q) || !ops_aligned(p->out) || !ops_stride16(p->q_stride, p->x_dtype) || !ops_stride16(p->out_stride, p->x_dtype))
     return ops_fail(CSM_OPS_ERR_ARG, "q and out must start on 16 bytes and have rows of multiples of 16 bytes");
+  if (c.rows > 1 && p->out_stride < (int64_t)p->n_q * c.head_dim) return ops_fail(CSM_OPS_ERR_ARG, "rows of out overlap");
   return 0;
 }
 

@@ -10,7 +10,8 @@
  *   - every pointer inside an argument struct is a DEVICE pointer of the device that is current on the calling thread; `stream` is a
  *     hipStream_t of it.  Argument structs live in host memory and are read before the call returns.
  *   - strides count ELEMENTS.  Rows, caches and tables must start on 16 bytes and their strides must keep 16-byte alignment where the
- *     struct says "16 B"; the innermost dimension is contiguous everywhere.
+ *     struct says "16 B"; the innermost dimension is contiguous everywhere.  Inputs may share memory between rows (a stride of 0); rows
+ *     of an output, and slots of a cache that is written, may not.
  *   - what only the device knows (lengths, page numbers, row offsets) is bounds-checked by the kernels: nothing outside the given tensors
  *     is ever read or written, whatever these arrays hold.
  *
@@ -75,11 +76,12 @@ int csm_ops_paged_rope_append(const csm_ops_rope_append_t* a, void* stream);
 /* ---- attention over a prefix shared by all rows and each sequence's own slots.  Row r of sequence b at slot s sees the prefix's
  * `prefix_len` slots (pages prefix_table[0 ..], same cache) and its own slots 0 .. s; out[r, h] = softmax(scale q.k) v over them, head h
  * reading kv head h / (n_q / n_kv).  The prefix is read once for all rows, not once per sequence.  A row that sees no key gives zeros; a
- * page number outside the cache hides its slots.  Slots that no row of the call sees may hold anything; a NaN or infinity in v of a slot that
- * some rows of a sequence see also reaches that sequence's earlier rows of the call (0 * NaN), never another sequence.  x_dtype (q and out) bf16 needs a bf16 cache: products on the bf16 matrix pipe with fp32
- * sums; x_dtype fp32 takes either cache, fp32 throughout.  head_dim 64 or 128; any n_q that is a multiple of n_kv; at most 64 GB of
- * cache and 2^24 pages.  `workspace`: at least
- * csm_ops_paged_attention_workspace bytes (16 B), contents undefined before and after; calls that may overlap in time need one each.  out may be q. */
+ * page number outside the cache hides its slots.  Slots that no row of the call sees may hold anything; a NaN or infinity in v of a slot
+ * that some rows of a sequence see also reaches that sequence's earlier rows of the call (0 * NaN), never another sequence.  x_dtype (q and
+ * out) bf16 needs a bf16 cache: products on the bf16 matrix pipe with fp32 sums; x_dtype fp32 takes either cache, fp32 throughout.
+ * head_dim 64 or 128; any n_q that is a multiple of n_kv; at most 64 GB of cache, 2^24 pages, pages and slots less than 256 MB apart.
+ * `workspace`: at least csm_ops_paged_attention_workspace bytes (16 B), contents undefined before and after; calls that may overlap in time
+ * need one each.  out may be q. */
 typedef struct {
   csm_ops_paged_t c;
   const void* q;                      /* 16 B; heads contiguous */

@@ -61,7 +61,7 @@ def _paged_args(p, **over):
 @pytest.mark.parametrize("over", [
     dict(dtype=2), dict(page_size=24), dict(page_size=0), dict(rows=3), dict(rows=-1), dict(n_kv=0), dict(head_dim=24), dict(head_dim=272), dict(k=(1 << 20) + 8),
     dict(v=None), dict(k_slot_stride=60), dict(v_head_stride=-64), dict(page_table=None), dict(seq_lens=None), dict(x_dtype=3), dict(qkv=None), dict(qkv=(1 << 24) + 2),
-    dict(q_out_stride=129), dict(cos=None), dict(pos_offset=-1), dict(n_q=0), dict(n_q=1 << 29), dict(table_width=1 << 28, page_size=64)])
+    dict(q_out_stride=129), dict(cos=None), dict(q_out_stride=64), dict(k_slot_stride=0), dict(v_page_stride=32), dict(k_head_stride=8), dict(pos_offset=-1), dict(n_q=0), dict(n_q=1 << 29), dict(table_width=1 << 28, page_size=64)])
 def test_append_refusals(over):
     lib = ops.load_ops_library()
     a = ops.RopeAppendArgs(qkv=1 << 24, q_out=1 << 25, qkv_stride=384, q_out_stride=128, x_dtype=1, n_q=2, cos=1 << 26, sin=1 << 27, rope_positions=64)
@@ -75,7 +75,7 @@ def test_append_refusals(over):
 
 @pytest.mark.parametrize("over", [
     dict(dtype=0), dict(x_dtype=2), dict(head_dim=32), dict(head_dim=96), dict(n_q=3), dict(n_q=0), dict(prefix_len=-1), dict(prefix_len=33, prefix_pages=2, prefix_table=1 << 26),
-    dict(prefix_len=5, prefix_pages=1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(out=(1 << 25) + 4), dict(q_stride=100), dict(rows=1), dict(page_size=3),
+    dict(prefix_len=5, prefix_pages=1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(out=(1 << 25) + 4), dict(out_stride=128), dict(out_stride=-256), dict(q_stride=100), dict(rows=1), dict(page_size=3),
     dict(n_pages=(1 << 24) + 1), dict(k_page_stride=1 << 30)])
 def test_attention_refusals(over):
     lib = ops.load_ops_library()
