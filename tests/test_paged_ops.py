@@ -505,6 +505,17 @@ def test_attention_mixed_sequences(x, prefix):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("x,c", [(BF16, BF16), (F32, BF16), (F32, F32)])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(4, 2, 64), (2, 1, 128), (3, 1, 64)])
+def test_attention_short_axes(x, c, n_q, n_kv, hd):
+    """axes that one workgroup walks alone: a text among single tokens, more sequences behind a longer axis, one key, padding"""
+    _attn_case([5, 46, 1, 30, -1, 17, 2, 44] + [3] * 20, [1, 45, 1, 1, 1, 0, 2, 1] + [1] * 20, n_q, n_kv, hd, x, c, prefix=30, seed=1)
+    _attn_case([1 + (i * 37) % 190 for i in range(180)], [1] * 180, n_q, n_kv, hd, x, c, prefix=100, seed=2)
+    _attn_case([1], [1], n_q, n_kv, hd, x, c, prefix=1, seed=3)
+    _attn_case([0, -1, 1], [1, 1, 1], n_q, n_kv, hd, x, c, prefix=33, seed=4, cu=None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x,c", [(BF16, BF16), (F32, BF16), (F32, F32)])
 @pytest.mark.parametrize("lens,new,prefix", [([30, 9], [1, 1], 20), ([30, 9], [1, 1], 3000), ([200, 60], [150, 60], 100), ([2000], [1], 0)])
 def test_attention_in_place_and_strided(x, c, lens, new, prefix):
     """out = q, q as the q part of wider rows, out as a slice of wider rows"""
