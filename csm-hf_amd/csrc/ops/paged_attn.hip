@@ -10,7 +10,7 @@
 //   more rows, bf16 cache:       64-key tiles of K and V are staged once per workgroup in LDS (two buffers), every wave takes 16-row tiles.
 //   more rows, fp32 cache:       every wave streams all keys for its 16 rows.
 // Measured: 128 sequences of some 1500 own slots behind 4096 (32 / 8 heads of 64, bf16): 416 MB in 83 + 5 us, 4.8 TB/s of the 4.9 that a large copy reaches.
-// 2 sequences of 4096 new rows: 136 GFLOP in 187 us, 730 TFLOP/s of the 1330 that a large bf16 product reaches; 2162 ragged rows behind 2048 slots 485,
+// 2 sequences of 4096 new rows: 136 GFLOP in 180 us, 755 TFLOP/s of the 1330 that a large bf16 product reaches; 2162 ragged rows behind 2048 slots 540,
 // where 664 workgroups share 256 CUs.  Without its exponentials that launch (at 220 us) took 14 percent less, without the second product 15, without half of the
 // first 13, without fetching tiles 11: no single one bounds it.  One sequence behind 512 slots: 4.6 + 2.3 us, a chain of latencies.
 //
@@ -426,16 +426,24 @@ struct Wide {
     }
   }
 
-  // one staged tile for the wave's first n_rt row tiles.  (A branch per product of the second one, not a copy without it: the copy let the scheduler hold
-  // 30 registers more, and two waves per SIMD instead of three took 10 percent longer)
+  // One staged tile for the wave's first n_rt row tiles.  (A branch per product of the second one, not a copy without it: the copy let the scheduler hold
+  // 30 registers more, and two waves per SIMD instead of three took 10 percent longer.)  The branches also keep the scheduler from moving LDS reads, so they
+  // stand ahead by hand: K one 16-key tile, V two operands.  The further a wave is in its tile, the earlier it goes: the three waves of a SIMD then sit in
+  // different phases, and one's exponentials run beside another's products.  2162 ragged rows behind 2048 slots 79 -> 70 us, 2 sequences of 4096 rows 193 -> 180;
+  // reads ahead alone 77 -> 74.5 and 185 -> 194, priority for the second product alone 77 and 187.  (Four waves per SIMD need spills: 100 and 220)
   __device__ __forceinline__ void tile(const AttnOpArgs& a, const char* ks, char* vs, const int (&kp)[T], const int (&vp)[HD / 16], uint64_t now, int j, int g, const int (&lim)[RT], const int (&lim_min)[RT], int n_rt) {
     const b16x8 ones = (b16x8)((short)0x3f80);
     f32x4 s[RT][4];
+    __builtin_amdgcn_s_setprio(1);
+    b16x8 k[2][T];
+    auto read_k = [&](int kt) {
+#pragma unroll
+      for (int x = 0; x < T; ++x) k[kt & 1][x] = *reinterpret_cast<const b16x8*>(ks + kp[x] + 16 * kt * HD * 2);
+    };
+    read_k(0);
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-      b16x8 k[T];
-#pragma unroll
-      for (int x = 0; x < T; ++x) k[x] = *reinterpret_cast<const b16x8*>(ks + kp[x] + 16 * kt * HD * 2);
+      if (kt < 3) read_k(kt + 1);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         if (r && n_rt < 2) break;
@@ -443,9 +451,10 @@ struct Wide {
 #pragma unroll
         for (int n = NQ - 1; n >= 0; --n)
 #pragma unroll
-          for (int x = 0; x < T; ++x) s[r][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[x], q[r][n][x], s[r][kt], 0, 0, 0);
+          for (int x = 0; x < T; ++x) s[r][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[kt & 1][x], q[r][n][x], s[r][kt], 0, 0, 0);
       }
     }
+    __builtin_amdgcn_s_setprio(2);
     b16x8 p[RT][2][NP];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -485,24 +494,30 @@ struct Wide {
         for (int n = NP - 1; n >= 0; --n) l4[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][h][n], l4[r], 0, 0, 0);
       }
     }
-    // the wave goes first on the matrix pipe while the others are at their softmax: 2 sequences of 4096 rows 193 -> 187 us, 2162 ragged rows behind 2048 slots
-    // 79 -> 77.  (Four waves per SIMD instead of three need spills: 220 and 100)
-    __builtin_amdgcn_s_setprio(1);
+    __builtin_amdgcn_s_setprio(3);
+    typedef __attribute__((address_space(3))) b16x4* lp;
+    constexpr int NV = HD / 8, AHEAD = 2;
+    b16x4 vx[AHEAD + 1], vy[AHEAD + 1];
+    auto read_v = [&](int i) {
+      const int h = i / (HD / 16), dt = i % (HD / 16), to = i % (AHEAD + 1);
+      vx[to] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + vp[dt] + 32 * h * HD * 2));
+      vy[to] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + vp[dt] + (32 * h + 16) * HD * 2));
+    };
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < AHEAD; ++i) read_v(i);
 #pragma unroll
-      for (int dt = 0; dt < HD / 16; ++dt) {
-        typedef __attribute__((address_space(3))) b16x4* lp;
-        const b16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + vp[dt] + 32 * h * HD * 2));
-        const b16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vs + vp[dt] + (32 * h + 16) * HD * 2));
-        const b16x8 v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    for (int i = 0; i < NV; ++i) {
+      if (i + AHEAD < NV) read_v(i + AHEAD);
+      const b16x4 x = vx[i % (AHEAD + 1)], y = vy[i % (AHEAD + 1)];
+      const b16x8 v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      const int h = i / (HD / 16), dt = i % (HD / 16);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          if (r && n_rt < 2) break;
+      for (int r = 0; r < RT; ++r) {
+        if (r && n_rt < 2) break;
 #pragma unroll
-          for (int n = NP - 1; n >= 0; --n) o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[r][h][n], o[r][dt], 0, 0, 0);
-        }
+        for (int n = NP - 1; n >= 0; --n) o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[r][h][n], o[r][dt], 0, 0, 0);
       }
+    }
     __builtin_amdgcn_s_setprio(0);
   }
 };
