@@ -7,8 +7,8 @@
 //   own item    : rows of one sequence, range inside its own slots (its prefix too, where every sequence brings rows enough of its own);
 // and leaves (max, sum, unnormalised output) per row, which a second small launch joins.
 //   up to 16 live rows (decode): the launch waits for memory.  The four waves split the keys, each streams its own, and they join through LDS.
-//   more rows, bf16 cache:       64-key tiles of K and V are staged once per workgroup in LDS (two buffers), every wave takes 16-row tiles.
-//   more rows, fp32 cache:       every wave streams all keys for its 16 rows.
+//   more rows: 64-key tiles (32 fp32) of K and V are staged once per workgroup in LDS (two buffers), every wave takes 16-row tiles.
+//   more rows in a tall workgroup (below; a text among single tokens): every wave streams all keys for its 16 rows.
 // Measured: 128 sequences of some 1500 own slots behind 4096 (32 / 8 heads of 64, bf16): 416 MB in 83 + 5 us, 4.8 TB/s of the 4.9 that a large copy reaches.
 // 2 sequences of 4096 new rows: 136 GFLOP in 180 us, 755 TFLOP/s of the 1330 that a large bf16 product reaches; 2162 ragged rows behind 2048 slots 540,
 // where 664 workgroups share 256 CUs.  Without its exponentials that launch (at 220 us) took 14 percent less, without the second product 15, without half of the
@@ -337,13 +337,15 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const XT* qp, c
   l = xor32_sum(xor16_sum(l));
 }
 
-// ---- many rows on a bf16 cache: 64-key tiles shared by the workgroup ---------------------------------------------------------------------------
+// ---- many rows: tiles shared by the workgroup; bf16 cache: 64 keys ---------------------------------------------------------------------------
 // bf16 queries: two 16-row tiles per wave, so that a K or V operand read from LDS feeds two products; p is ONE bf16 piece here -- a second rounding of
 // the size of the result's own (the sum l is of the same rounded p) against half again as many matrix instructions: 88 -> 107 us ragged, 220 -> 271 for
 // 2 x 4096 rows, for a relative error of 0.0017 instead of 0.0022.  fp32 queries: one tile
 // per wave, q and p in three exact pieces.  l comes off the matrix pipe too, as a product with ones.
+template <typename XT, typename CT, int HD>
+struct Wide;
 template <typename XT, int HD>
-struct Wide {
+struct Wide<XT, bf16_t, HD> {
   static constexpr int RT = sizeof(XT) == 2 ? 2 : 1, NQ = sizeof(XT) == 2 ? 1 : 3, NP = NQ, T = HD / 32, KEYS = 64, CH = HD / 8, KPP = AT / CH, NL = KEYS / KPP;
   static constexpr int TILE = KEYS * HD * 2, LDS_BYTES = 4 * TILE;   // K, V, two buffers
   b16x8 q[RT][NQ][T];
@@ -522,6 +524,130 @@ struct Wide {
   }
 };
 
+// The same on an fp32 cache: 32-key tiles, 16 rows a wave, fp32 products.  Without the sharing each wave fetches every key for itself, and a workgroup of 64
+// rows waits for four times the bytes: 2162 ragged rows behind 2048 slots 489 -> 410 us (92 TFLOP/s of the 154 that a large fp32 product reaches).  LDS rows are 4 floats longer than a key: the 16 keys of a K operand then
+// cover all banks, and so do the 4 of a V operand.
+template <int HD>
+struct Wide<float, float, HD> {
+  using P = Prod<float, float, HD>;
+  static constexpr int RT = 1, KEYS = 32, CH = HD / 4, KPP = AT / CH, NL = KEYS / KPP, LD = P::LD, U = P::U;
+  static constexpr int TILE = KEYS * LD * 4, LDS_BYTES = 4 * TILE;   // K, V, two buffers
+  f32x4 q[U], o[RT][HD / 16], l4[RT];
+  float m[RT];
+
+  __device__ __forceinline__ void run(const AttnOpArgs& a, const float* const (&qp)[RT], const KeyAxis& ax, int kvh, int k0, int k1, const int (&lim)[RT], const int (&lim_min)[RT], int n_rt, char* lds) {
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, g = lane >> 4;
+    const int ch = tid % CH, key0 = tid / CH;
+    const char* kb = reinterpret_cast<const char*>(reinterpret_cast<const float*>(a.k) + kvh * a.c.kh + ch * 4);
+    const char* vb = reinterpret_cast<const char*>(reinterpret_cast<const float*>(a.v) + kvh * a.c.vh + ch * 4);
+    m[0] = -INFINITY;
+    l4[0] = (f32x4)(0.f);
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) o[0][i] = (f32x4)(0.f);
+    if (k0 >= k1) return;
+    uint32_t entry = 0, slot = 0;   // of key lane % 32
+    auto look = [&](int j0) {
+      const int j = j0 + (lane & 31);
+      entry = ~0u;
+      slot = 0;
+      if (j < k1) entry = ax.entry(j, a.c, slot);
+    };
+    f32x4 kr[NL], vr[NL];
+    auto fetch = [&]() -> uint32_t {
+      const bool ok = entry < (uint32_t)a.c.n_pages;
+      const uint32_t page = ok ? entry : 0, ko = __umul24(page, a.kp16) + __umul24(slot, a.ks16);   // (page 0 exists)
+      uint32_t kat[NL], vat[NL];
+#pragma unroll
+      for (int i = 0; i < NL; ++i) vat[i] = kat[i] = __shfl(ko, i * KPP + key0);
+      if (!a.one_place) {
+        const uint32_t vo = __umul24(page, a.vp16) + __umul24(slot, a.vs16);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) vat[i] = __shfl(vo, i * KPP + key0);
+      }
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        kr[i] = *reinterpret_cast<const f32x4*>(kb + ((uint64_t)kat[i] << 4));
+        vr[i] = *reinterpret_cast<const f32x4*>(vb + ((uint64_t)vat[i] << 4));
+      }
+      return (uint32_t)__ballot(ok);
+    };
+    typename P::Raw raw;
+    look(k0);
+    P::load_q(raw, qp[0], g);
+    uint32_t valid = fetch();
+    look(k0 + KEYS);
+    P::make_q(raw, q, a.q_flip);
+    const int st = (key0 * LD + ch * 4) * 4, kp = (li * LD + 4 * g) * 4;
+    int buf = 0;
+    for (int j = k0; j < k1; j += KEYS, buf ^= 1) {
+      char* const ks = lds + buf * 2 * TILE;
+      char* const vs = ks + TILE;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        if (valid != ~0u && !((valid >> (i * KPP + key0)) & 1)) vr[i] = (f32x4)(0.f);   // 0 * (what an unused slot holds) must be 0
+        *reinterpret_cast<f32x4*>(ks + st + i * KPP * LD * 4) = kr[i];
+        *reinterpret_cast<f32x4*>(vs + st + i * KPP * LD * 4) = vr[i];
+      }
+      __syncthreads();   // (one per tile: a buffer is written again only two tiles later)
+      const uint32_t now = valid;
+      if (j + KEYS < k1) {
+        valid = fetch();
+        look(j + 2 * KEYS);
+      }
+      if (n_rt) tile(a, ks, vs, kp, now, j, g, lane, lim[0], lim_min[0]);
+    }
+    l4[0] = (f32x4)(xor32_sum(xor16_sum(l4[0][0])));
+  }
+
+  __device__ __forceinline__ void tile(const AttnOpArgs& a, const char* ks, char* vs, int kp, uint32_t now, int j, int g, int lane, int lim, int lim_min) {
+    f32x4 s[2];
+    s[0] = s[1] = (f32x4)(0.f);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      f32x4 k[2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) k[kt] = *reinterpret_cast<const f32x4*>(ks + kp + (16 * kt * LD + 16 * u) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[kt][e], q[u][e], s[kt], 0, 0, 0);
+    }
+    if (now != ~0u || j + KEYS > lim_min) {
+      const uint32_t seen = now >> (4 * g);
+      const int left = lim - j - 4 * g;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[kt][e] = ((seen >> (16 * kt + e)) & 1) && 16 * kt + e < left ? s[kt][e] : -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kt][e]);
+    top *= a.c2;
+    if (__any(top > m[0] + SLACK)) {
+      top = xor32_max(xor16_max(top));
+      const float m_new = fmaxf(m[0], top), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[0] - m_new);
+      l4[0][0] *= alpha;
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) o[0][i] *= alpha;
+      m[0] = m_new;
+    }
+    const float ref = m[0] == -INFINITY ? 0.f : m[0];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      f32x4 p[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[0][e] = __builtin_amdgcn_exp2f(__fmaf_rn(s[kt][e], a.c2, -ref));
+        l4[0][0] += p[0][e];
+      }
+      P::accumulate(p, vs, P::v_place(lane) + 16 * kt * LD, o[0], lane);
+    }
+  }
+};
+
 // ---- results ------------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
 __device__ __forceinline__ void store4(bf16_t* p, const f32x4& v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])); }
@@ -580,10 +706,10 @@ __device__ __forceinline__ void put(const AttnOpArgs& a, int row, int head, int 
 template <typename XT, typename CT, int HD, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void paged_attn_kernel(AttnOpArgs a) {
   using P = Prod<XT, CT, HD>;
-  constexpr bool WIDE = sizeof(CT) == 2 && NW == 4;
+  constexpr bool WIDE = NW == 4;
   constexpr int ROWS = tile_rows(sizeof(XT) == 2 ? CSM_OPS_BF16 : CSM_OPS_F32);
   constexpr int WAVE_LDS = P::LDS_BYTES > 16 * (HD + 4) * 4 ? P::LDS_BYTES : 16 * (HD + 4) * 4;   // V tile; at the end 16 rows of fp32 results
-  constexpr int LDS = WIDE && Wide<XT, HD>::LDS_BYTES > NW * WAVE_LDS ? Wide<XT, HD>::LDS_BYTES : NW * WAVE_LDS;
+  constexpr int LDS = WIDE && Wide<XT, CT, HD>::LDS_BYTES > NW * WAVE_LDS ? Wide<XT, CT, HD>::LDS_BYTES : NW * WAVE_LDS;
   __shared__ __attribute__((aligned(16))) char lds[LDS];
   __shared__ float ml_s[NW][16][2];
   const Paged& c = a.c;
@@ -637,7 +763,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void paged_attn_kernel(At
   const bool by_keys = live <= 16;
   if constexpr (WIDE) {
     if (!by_keys) {   // 16-row tiles wave, wave + 4
-      using Wd = Wide<XT, HD>;
+      using Wd = Wide<XT, CT, HD>;
       Wd w;
       int lim[Wd::RT], lim_min[Wd::RT], n_rt = 0;
       const XT* qp[Wd::RT];
