@@ -15,9 +15,9 @@
 //                Where they are not enough (a flat row whose nucleus is larger), the same search streams over the row.
 //
 // What bounds it: not the bytes.  One row of 2051 fp32: 7.0 us, the chain of steps; 512 of them, each with its own filters: 13.5 us for 4.2 MB (0.9 at the rate
-// of a large copy) -- two workgroups a CU, whose steps overlap little.  64 rows of 128 256 bf16, top_p alone: 7.4 + 19.4 + 17.1 us for 16.4 MB (3.4); the
-// chunks' 8.2 million fp64 exponentials (21 operations of 8 clocks a wave) take 11 of the 19, in the list's 17 are 4 to fetch it, 5 for the histogram, 3 for
-// the draw and the heads' sums.
+// of a large copy) -- two workgroups a CU, whose steps overlap little.  64 rows of 128 256 bf16, top_p alone: 7.4 + 17 + 17.1 us for 16.4 MB (3.4); the
+// chunks' 8.2 million fp64 exponentials (13 operations of 8 clocks a wave) take some 8 of the 17, in the list's 17 are 4 to fetch it, 5 for the histogram, 3
+// for the draw and the heads' sums.
 #include "ops_common.h"
 #include <math.h>
 
@@ -82,6 +82,32 @@ struct Weigh {
     p = __fma_rn(p, f, 9.6181291076284772e-03); p = __fma_rn(p, f, 5.5504108664821580e-02); p = __fma_rn(p, f, 2.4022650695910071e-01);
     p = __fma_rn(p, f, 6.9314718055994531e-01); p = __fma_rn(p, f, 1.0);
     return (uint64_t)__double_as_longlong(ldexp(p, (int)n + shift) + 4503599627370496.0) & 0xfffffffffffffull;
+  }
+};
+
+// The same where millions of them bound the launch: 2^t = 2^(n / 32) 2^f with |f| <= 1/64, the root from a table in LDS (no two of its entries share a bank),
+// f to the 5th power (below 2^-48).  Adding 1.5 * 2^47 leaves n in the low mantissa; 13 fp64 operations instead of 20, 43.8 -> 41.4 us for 64 rows of
+// 128 256 bf16 logits.  Where an exponential is one link of a chain of steps, the shorter way without a table to wait for is Weigh's.
+__device__ const double roots[32] = {  // 2^(i / 32)
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+struct WeighMany {
+  float mx;
+  double k2;
+  int shift;
+  const double* table;   // in LDS
+  __device__ __forceinline__ uint64_t operator()(float x) const {
+    if (mx == INFINITY) return x == INFINITY ? 1ull << shift : 0ull;
+    const double t = fmax(((double)x - (double)mx) * k2, -1000.0), whole = t + 211106232532992.0, f = t - (whole - 211106232532992.0);
+    const int n = (int)(uint32_t)__double_as_longlong(whole);
+    const double root = table[n & 31];
+    double p = 0.0013333558146428441;   // ln(2)^i / i!, i = 5 .. 0
+    p = __fma_rn(p, f, 0.009618129107628477); p = __fma_rn(p, f, 0.055504108664821576); p = __fma_rn(p, f, 0.2402265069591007);
+    p = __fma_rn(p, f, 0.6931471805599453); p = __fma_rn(p, f, 1.0);
+    const double scale = __hiloint2double(__double2hiint(root) + (((n >> 5) + shift) << 20), __double2loint(root));
+    return (uint64_t)__double_as_longlong(__fma_rn(p, scale, 4503599627370496.0)) & 0xfffffffffffffull;
   }
 };
 
@@ -789,6 +815,7 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
   __shared__ double mass_s[4];
   __shared__ uint32_t cnt_s[4];
   __shared__ int at_s;
+  __shared__ double roots_s[32];
   const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const XT* x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
   const Setting s = setting(a, row);
@@ -808,6 +835,7 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
     v[e] = y != y ? -INFINITY : y;
   }
   if (tid == 0) at_s = a.V;
+  if (tid < 32) roots_s[tid] = roots[tid];
   float mx = -INFINITY;
 #pragma unroll
   for (int e = 0; e < PER; ++e) mx = fmaxf(mx, v[e]);
@@ -830,7 +858,7 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
   // the chunk's mass where it counts: no top-k, and a nucleus or nothing at all to cut
   double mass = 0.0;
   if (!s.k && (s.top_p < 1.f || s.min_p == 0.f) && mx > -INFINITY) {
-    const Weigh weigh{mx, 1.4426950408889634074 / (double)s.T, 51};
+    const WeighMany weigh{mx, 1.4426950408889634074 / (double)s.T, 51, roots_s};
     uint64_t m = 0;
 #pragma unroll
     for (int e = 0; e < PER; ++e) m += weigh(v[e]);
