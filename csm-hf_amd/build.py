@@ -1,5 +1,6 @@
 """Build libcsm_hip.so (gfx950) in-tree with hipcc.  No torch involvement: the library is a plain C-ABI
-shared object (include/csm_hip.h).  `python -m csm_hf_amd.build` or `build_library()`."""
+shared object (include/csm_hip.h).  `python -m csm_hf_amd.build` or `build_library()`, which also build the stand-alone
+operators: libcsm_ops.so (include/csm_ops.h, plain C too) and its binding for torch tensors, _ops_binding.so."""
 from __future__ import annotations
 
 import os

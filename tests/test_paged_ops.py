@@ -441,6 +441,40 @@ def test_attention_never_reads_what_is_not_seen(x, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n_q,n_kv,hd", [(4, 2, 64), (2, 1, 128)])
+@pytest.mark.parametrize("new", [[1, 1], [21, 20], [200, 3]])
+def test_attention_exact_mode_never_reads_what_is_not_seen(new, n_q, n_kv, hd):
+    """the same on an fp32 cache: what lies past the lengths and on other pages may be anything"""
+    lens, prefix = [new[0] + 4, new[1] + 13], 45
+    cache = Cache(lens, 16, n_kv, hd, F32, prefix=prefix, seed=5)
+    seen = torch.zeros(cache.k.shape[0], 16, dtype=torch.bool, device=DEV)
+    for b, n in enumerate(lens):
+        for t in range(n):
+            seen[cache.table[b, t // 16], t % 16] = True
+    for t in range(prefix):
+        seen[cache.prefix[t // 16], t % 16] = True
+    q = torch.randn(sum(new), n_q, hd, device=DEV)
+    want, tol = attention64(q, cache, lens, new, n_q, hd ** -0.5, False)
+    hidden = (~seen)[:, None, :, None].expand_as(cache.k)
+    for junk in (math.nan, math.inf, -math.inf, 3e38):
+        cache.k[hidden], cache.v[hidden] = junk, junk
+        check(paged_prefix_attention(q, *cache.args(), prefix_table=cache.prefix, prefix_len=prefix, cu_rows=_cu(new)), want, tol, 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_kv,hd", [(2, 64), (1, 128)])
+def test_attention_exact_mode_nonsense_row_offsets_end_in_bounds(n_kv, hd):
+    cache = Cache([40, 40, 40, 40], 16, n_kv, hd, F32, prefix=20)
+    q = torch.randn(90, 4, hd, device=DEV)
+    for cu in ([0, 9, -4, 2 ** 31 - 1, 40], [50, 60, 70, 80, 90], [4, 3, 2, 1, 0], [0, 90, 90, 90, 90]):
+        paged_prefix_attention(q, *cache.args(), prefix_table=cache.prefix, prefix_len=20, cu_rows=torch.tensor(cu, dtype=torch.int32, device=DEV))
+        torch.cuda.synchronize()
+    cache.lens.fill_(2 ** 31 - 1)
+    paged_prefix_attention(q, *cache.args(), prefix_table=cache.prefix, prefix_len=20, cu_rows=_cu([60, 10, 10, 10]))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 def test_attention_nonsense_row_offsets_end_in_bounds():
     cache = Cache([40, 40, 40, 40], 16, 2, 64, BF16, prefix=20)
     q = torch.randn(40, 4, 64, device=DEV).bfloat16()
