@@ -424,7 +424,8 @@ struct Hist {
       cb += c[i];
       mb += m[i];
     }
-    blk.before2(cb, mb, all_c, all_m);   // (its barrier is between the weights and their use)
+    if (MASS) blk.before2(cb, mb, all_c, all_m);   // (its barrier is between the weights and their use)
+    else cb = blk.before(cb, all_c);
     if (table) {
 #pragma unroll
       for (int e = 0; e < E; ++e) r.w[e] = r.key[e] ? h->m[key_max - r.key[e]] : 0;
