@@ -14,7 +14,7 @@
 //                8 192 entries its maximum, its mass and the entries above the threshold; per row the cuts and the draw on those entries.
 //                Where they are not enough (a flat row whose nucleus is larger), the same search streams over the row.
 //
-// What bounds it: not the bytes.  One row of 2051 fp32: 7.0 us, the chain of steps; 512 of them, each with its own filters: 13.5 us for 4.2 MB (0.9 at the rate
+// What bounds it: not the bytes.  One row of 2051 fp32: 6.5 us, the chain of steps; 512 of them, each with its own filters: 13 us for 4.2 MB (0.9 at the rate
 // of a large copy) -- two workgroups a CU, whose steps overlap little.  64 rows of 128 256 bf16, top_p alone: 7.4 + 17 + 17.1 us for 16.4 MB (3.4); the
 // chunks' 8.2 million fp64 exponentials (13 operations of 8 clocks a wave) take some 8 of the 17, in the list's 17 are 4 to fetch it, 5 for the histogram, 3
 // for the draw and the heads' sums.
@@ -306,9 +306,11 @@ __device__ __forceinline__ Cut find_cut(Src& src, Block<NT>& blk, Few* few, cons
 }
 
 // a row (or list) in registers: thread t holds entries t * per .. t * per + per - 1; key 0, w 0 = not (or no longer) an entry
-template <int E>
+// BINS: the entries' bins of the histogram built last are kept too (a row of 2051 under a small top-k 7.7 -> 7.1 us); not where 1024 threads hold a whole row
+// with its values, whose registers that would spill (19.1 -> 19.8)
+template <int E, bool BINS = true>
 struct RegRow {
-  uint32_t key[E];
+  uint32_t key[E], bin[BINS ? E : 1];
   uint64_t w[E];
   int per;
   template <typename K>
@@ -352,8 +354,8 @@ struct RegRow {
 };
 
 // of the entries equal to a cut, drop those that it does not keep (entries below it are left: they lie under every later probe)
-template <int E, int NT>
-__device__ __forceinline__ void drop_ties(RegRow<E>& r, Block<NT>& blk, const Cut& c) {
+template <int E, bool BINS, int NT>
+__device__ __forceinline__ void drop_ties(RegRow<E, BINS>& r, Block<NT>& blk, const Cut& c) {
   if (c.ties >= c.same) return;
   uint32_t mine = 0, total;
 #pragma unroll
@@ -391,11 +393,13 @@ struct Hist {
     usable = exact || (span > 0.f && span < INFINITY && inv < INFINITY);
   }
   __device__ __forceinline__ uint32_t bin(uint32_t key) const { return exact ? key_max - key : min((uint32_t)((top - K::value(key)) * inv), (uint32_t)N - 1); }
+  template <int E, bool BINS>
+  __device__ __forceinline__ uint32_t bin_of(const RegRow<E, BINS>& r, int e) const { return BINS ? r.bin[e] : bin(r.key[e]); }
   // TABLE, and a bin is a key: the weights are not there yet.  Each is computed once per key, not once per entry, and a bin's mass is count * weight --
   // the bf16 list of a long row holds 12 000 entries of some 250 keys (64 rows of 128 256, top_p 0.9: 48.5 -> 43.3 us; whole rows seldom span few
   // enough keys, there the second way only makes the code longer: 12.2 -> 12.7)
-  template <bool MASS, bool TABLE, int E>
-  __device__ __forceinline__ void build(RegRow<E>& r, Block<NT>& blk, const Weigh& weigh) {
+  template <bool MASS, bool TABLE, int E, bool BINS>
+  __device__ __forceinline__ void build(RegRow<E, BINS>& r, Block<NT>& blk, const Weigh& weigh) {
     const bool table = TABLE && exact;
     const int tid = threadIdx.x;
 #pragma unroll
@@ -406,6 +410,7 @@ struct Hist {
       if (E > 4 && e % 4 == 0 && e >= r.per) break;
       if (r.key[e]) {
         const uint32_t b = bin(r.key[e]);
+        if (BINS) r.bin[e] = b;
         atomicAdd(&h->c[b], 1u);
         if (MASS && !table) atomicAdd(reinterpret_cast<unsigned long long*>(&h->m[b]), (unsigned long long)r.w[e]);
       }
@@ -449,8 +454,8 @@ struct Hist {
     return {h->bin[t], h->above[t], h->in[t], h->mass[t]};
   }
   // the exact cut in that bin; false: more than 64 entries of several keys crowd there
-  template <bool MASS, int E>
-  __device__ __forceinline__ bool resolve(const RegRow<E>& r, const Where& w, Few* few, const Weigh& weigh, uint32_t want_n, double want_m, Cut& cut, uint64_t& kept) {
+  template <bool MASS, int E, bool BINS>
+  __device__ __forceinline__ bool resolve(const RegRow<E, BINS>& r, const Where& w, Few* few, const Weigh& weigh, uint32_t want_n, double want_m, Cut& cut, uint64_t& kept) {
     if (exact) {
       cut.key = key_max - w.bin;
       cut.same = w.in;
@@ -466,7 +471,7 @@ struct Hist {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       if (E > 4 && e % 4 == 0 && e >= r.per) break;
-      if (r.key[e] && bin(r.key[e]) == w.bin) {
+      if (r.key[e] && bin_of(r, e) == w.bin) {
         const int at = atomicAdd(&few->n, 1);
         if (at < 64) few->key[at] = r.key[e];
       }
@@ -521,8 +526,8 @@ __device__ __forceinline__ int draw_few(uint32_t key, uint32_t k, const Weigh& w
 // The short way for a small top-k: the top bins that hold k entries and no more than 64 go in index order to one wave.  -2: too many crowd in the last
 // of these bins.  Otherwise the place (e, in the thread that owns it) or -1.  Needs keys only.
 struct FewOrder { uint32_t key[64]; int hit; };
-template <typename K, int E, int NT>
-__device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, HistLds<NT>* lds, FewOrder* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t k, uint32_t key_min, uint32_t key_max) {
+template <typename K, int E, bool BINS, int NT>
+__device__ __forceinline__ int draw_small(RegRow<E, BINS>& r, Block<NT>& blk, HistLds<NT>* lds, FewOrder* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t k, uint32_t key_min, uint32_t key_max) {
   uint32_t cnt = n, last = ~0u;   // the listed bins end with `last`
   Hist<K, NT> hist(lds, key_min, key_max);
   if (n > 64) {
@@ -537,7 +542,7 @@ __device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, HistLds<
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (E > 4 && e % 4 == 0 && e >= r.per) break;
-    if (r.key[e] && (last == ~0u || hist.bin(r.key[e]) <= last)) in |= 1u << e;
+    if (r.key[e] && (last == ~0u || hist.bin_of(r, e) <= last)) in |= 1u << e;
   }
   const uint32_t mine = __popc(in), first = blk.before(mine, total);
   if (mine) {
@@ -561,8 +566,8 @@ __device__ __forceinline__ int draw_small(RegRow<E>& r, Block<NT>& blk, HistLds<
 
 // filters and draw on entries in registers, with their weights unless TABLE; returns the place (e, in the thread that owns it) or -1.  `base`: the mass that top_p refers to when
 // it is not that of these entries (< 0: it is).  `enough` comes back false when these entries cannot hold the nucleus.
-template <typename K, bool TABLE, int E, int NT>
-__device__ __forceinline__ int filter_and_draw(RegRow<E>& r, Block<NT>& blk, HistLds<NT>* lds, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, double base, bool& enough) {
+template <typename K, bool TABLE, int E, bool BINS, int NT>
+__device__ __forceinline__ int filter_and_draw(RegRow<E, BINS>& r, Block<NT>& blk, HistLds<NT>* lds, Few* few, const Weigh& weigh, const Setting& s, uint32_t n, uint32_t key_min, uint32_t key_max, double base, bool& enough) {
   enough = true;
   Cut cut{key_min, 1u, 1u};
   const bool cut_k = s.k && (uint32_t)s.k < n;
@@ -654,7 +659,7 @@ __global__ __launch_bounds__(NT) void sample_short_kernel(SampleOpArgs a) {
   const XT* x = reinterpret_cast<const XT*>(a.logits) + row * a.stride;
   const Setting s = setting(a, row);
   Block<NT> blk{&red};
-  RegRow<E> r;
+  RegRow<E, NT == 256> r;
   r.per = (a.V + NT - 1) / NT;
   const int first = tid * r.per, mine = min(r.per, a.V - first);   // (mine <= 0 behind the row's end)
   float v[E];
