@@ -39,7 +39,7 @@ struct AttnOpArgs {
   int one_place;                     // K and V lie alike: one place serves both
   float c2;               // |scale| log2(e); the sign of scale is folded into q
   uint32_t q_flip;
-  int np_tiles, nsp, no_tiles, nso, per_seq_tiles, with_prefix, tall, nsplit;   // nsplit = partial results per row
+  int np_tiles, nsp, no_tiles, nso, per_seq_tiles, with_prefix, tall, narrow, nsplit;   // nsplit = partial results per row
   float* part;            // [rows * n_q][nsplit][hd]
   float2* ml;             // [rows * n_q][nsplit] (reference in log2 units, sum)
 };
@@ -338,15 +338,18 @@ __device__ __forceinline__ void wave_attend(const AttnOpArgs& a, const XT* qp, c
 }
 
 // ---- many rows: tiles shared by the workgroup; bf16 cache: 64 keys ---------------------------------------------------------------------------
-// bf16 queries: two 16-row tiles per wave, so that a K or V operand read from LDS feeds two products; p is ONE bf16 piece here -- a second rounding of
-// the size of the result's own (the sum l is of the same rounded p) against half again as many matrix instructions: 88 -> 107 us ragged, 220 -> 271 for
-// 2 x 4096 rows, for a relative error of 0.0017 instead of 0.0022.  fp32 queries: one tile
-// per wave, q and p in three exact pieces.  l comes off the matrix pipe too, as a product with ones.
-template <typename XT, typename CT, int HD>
+// bf16 queries: two 16-row tiles per wave, so that a K or V operand read from LDS feeds two products.  FINE: p in two bf16 pieces (16 bits), so that
+// rounding p adds nothing to the one rounding of the result; otherwise in ONE piece, a second rounding of the size of the result's own (the sum l is of
+// the same rounded p) against a third of the matrix instructions.  Two pieces / one (us; relative error 0.0017 / 0.0021-0.0023 throughout): prefix items of
+// decode launches, which wait for memory beside the sequences' own items, 88.3 / 87.8 for 128 sequences of some 1500 slots behind 4096, 25.0 / 24.1 behind 2048,
+// 14.8 / 13.7 for 32; many rows of their own, bound by issue slots, 89.7 / 70.1 for 2162 ragged rows, 252 / 187 for 2 x 4096.  So the decode launches
+// (AttnOpArgs::narrow) take two and the others one.  fp32 queries: one tile per wave, q and p in three exact pieces.  l comes off the matrix pipe too, as
+// a product with ones.
+template <typename XT, typename CT, int HD, bool FINE>
 struct Wide;
-template <typename XT, int HD>
-struct Wide<XT, bf16_t, HD> {
-  static constexpr int RT = sizeof(XT) == 2 ? 2 : 1, NQ = sizeof(XT) == 2 ? 1 : 3, NP = NQ, T = HD / 32, KEYS = 64, CH = HD / 8, KPP = AT / CH, NL = KEYS / KPP;
+template <typename XT, int HD, bool FINE>
+struct Wide<XT, bf16_t, HD, FINE> {
+  static constexpr int RT = sizeof(XT) == 2 ? 2 : 1, NQ = sizeof(XT) == 2 ? 1 : 3, NP = sizeof(XT) == 2 && FINE ? 2 : NQ, T = HD / 32, KEYS = 64, CH = HD / 8, KPP = AT / CH, NL = KEYS / KPP;
   static constexpr int TILE = KEYS * HD * 2, LDS_BYTES = 4 * TILE;   // K, V, two buffers
   b16x8 q[RT][NQ][T];
   f32x4 o[RT][HD / 16], l4[RT];
@@ -527,8 +530,8 @@ struct Wide<XT, bf16_t, HD> {
 // The same on an fp32 cache: 32-key tiles, 16 rows a wave, fp32 products.  Without the sharing each wave fetches every key for itself, and a workgroup of 64
 // rows waits for four times the bytes: 2162 ragged rows behind 2048 slots 489 -> 410 us (92 TFLOP/s of the 154 that a large fp32 product reaches).  LDS rows are 4 floats longer than a key: the 16 keys of a K operand then
 // cover all banks, and so do the 4 of a V operand.
-template <int HD>
-struct Wide<float, float, HD> {
+template <int HD, bool FINE>
+struct Wide<float, float, HD, FINE> {
   using P = Prod<float, float, HD>;
   static constexpr int RT = 1, KEYS = 32, CH = HD / 4, KPP = AT / CH, NL = KEYS / KPP, LD = P::LD, U = P::U;
   static constexpr int TILE = KEYS * LD * 4, LDS_BYTES = 4 * TILE;   // K, V, two buffers
@@ -703,13 +706,13 @@ __device__ __forceinline__ void put(const AttnOpArgs& a, int row, int head, int 
   }
 }
 
-template <typename XT, typename CT, int HD, int NW>
+template <typename XT, typename CT, int HD, int NW, bool FINE>
 __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void paged_attn_kernel(AttnOpArgs a) {
   using P = Prod<XT, CT, HD>;
   constexpr bool WIDE = NW == 4;
   constexpr int ROWS = tile_rows(sizeof(XT) == 2 ? CSM_OPS_BF16 : CSM_OPS_F32);
   constexpr int WAVE_LDS = P::LDS_BYTES > 16 * (HD + 4) * 4 ? P::LDS_BYTES : 16 * (HD + 4) * 4;   // V tile; at the end 16 rows of fp32 results
-  constexpr int LDS = WIDE && Wide<XT, CT, HD>::LDS_BYTES > NW * WAVE_LDS ? Wide<XT, CT, HD>::LDS_BYTES : NW * WAVE_LDS;
+  constexpr int LDS = WIDE && Wide<XT, CT, HD, FINE>::LDS_BYTES > NW * WAVE_LDS ? Wide<XT, CT, HD, FINE>::LDS_BYTES : NW * WAVE_LDS;
   __shared__ __attribute__((aligned(16))) char lds[LDS];
   __shared__ float ml_s[NW][16][2];
   const Paged& c = a.c;
@@ -763,7 +766,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void paged_attn_kernel(At
   const bool by_keys = live <= 16;
   if constexpr (WIDE) {
     if (!by_keys) {   // 16-row tiles wave, wave + 4
-      using Wd = Wide<XT, CT, HD>;
+      using Wd = Wide<XT, CT, HD, FINE>;
       Wd w;
       int lim[Wd::RT], lim_min[Wd::RT], n_rt = 0;
       const XT* qp[Wd::RT];
@@ -921,14 +924,14 @@ static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
   a.per_seq_tiles = (a.rep + ROWS - 1) / ROWS;
   const int64_t own_tiles = c.cu_rows ? flat / ROWS + c.n_seqs : (int64_t)c.n_seqs * a.per_seq_tiles;
   const int64_t own_cap = (int64_t)c.table_width * c.page_size;
-  const bool narrow = c.n_seqs > 0 && flat / c.n_seqs <= 16;   // decode: items wait for memory and are cheap to cut; a tile of many rows has much to join
+  a.narrow = c.n_seqs > 0 && flat / c.n_seqs <= 16;   // decode: items wait for memory and are cheap to cut; a tile of many rows has much to join
   const int64_t axis = p->prefix_len + own_cap;
   // few sequences and a short axis: ONE launch of tall workgroups (16 or 8 waves split the keys, the prefix among them) -- the prefix is read once per
   // sequence, from L2, and there is nothing to join.  The axis may be longer where the sequences alone give the CUs a workgroup each.  Measured (us, tall
   // against cut, 64 bf16 or fp32): 200 + 50 slots 6.2 / 6.7 and 8.4 / 7.1 for 1 sequence, 6.8 / 8.8 and 9.2 / 10.2 for 32; 512 + 130: 8.2 / 7.1 and
   // 13.6 / 8.0 for 1, 8.9 / 9.0 and 15.3 / 14.8 for 32; 512 + 1000: 12.5 / 11.1 and 25 / 18.5 for 16, 14.6 / 17.5 and 26.8 / 25.7 for 32; 128: 22 / 12 at 200 + 50
   const int64_t full = own_tiles * c.n_kv;
-  a.tall = narrow && p->prefix_len > 0 && full <= 256 && axis * c.head_dim * (c.dtype == CSM_OPS_BF16 ? 2 : 4) <= 64 * 1024 + (full > 128 ? (full - 128) * 2048 : 0);
+  a.tall = a.narrow && p->prefix_len > 0 && full <= 256 && axis * c.head_dim * (c.dtype == CSM_OPS_BF16 ? 2 : 4) <= 64 * 1024 + (full > 128 ? (full - 128) * 2048 : 0);
   // sequences that bring two tiles of 16 rows and more of their own read the prefix with them: nothing to share, nothing to join
   a.with_prefix = a.tall || (p->prefix_len > 0 && c.cu_rows && c.n_seqs > 0 && flat / c.n_seqs >= 32);
   const int64_t np = p->prefix_len && !a.with_prefix ? (flat + ROWS - 1) / ROWS : 0;
@@ -942,7 +945,7 @@ static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
     return (int)(n < 1 ? 1 : n > MAX_SPLIT / 2 ? MAX_SPLIT / 2 : n);
   };
   a.nsp = np ? splits(np * c.n_kv, p->prefix_len, 64, 64, 256) : 0;
-  a.nso = a.tall ? 1 : splits(own_tiles * c.n_kv, own_keys, 512, 128, narrow ? 2048 : 0);
+  a.nso = a.tall ? 1 : splits(own_tiles * c.n_kv, own_keys, 512, 128, a.narrow ? 2048 : 0);
   a.np_tiles = (int)np; a.no_tiles = (int)own_tiles; a.nsplit = a.nsp + a.nso;
   if (((int64_t)a.np_tiles * a.nsp + (int64_t)a.no_tiles * a.nso) * c.n_kv > 0x7fffffff) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
   return 0;
@@ -967,8 +970,10 @@ template <typename XT, typename CT, int HD>
 static int launch(const AttnOpArgs& a, hipStream_t st) {
   const unsigned items = (unsigned)(((int64_t)a.np_tiles * a.nsp + (int64_t)a.no_tiles * a.nso) * a.c.n_kv);
   constexpr int TALL = HD == 64 ? 16 : 8;   // as many waves as their registers allow
-  if (a.tall) hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD, TALL>), dim3(items), dim3(64 * TALL), 0, st, a);
-  else hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD, 4>), dim3(items), dim3(AT), 0, st, a);
+  constexpr bool EXACT = sizeof(XT) == 4;   // fp32 queries: p is exact either way, one body
+  if (a.tall) hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD, TALL, true>), dim3(items), dim3(64 * TALL), 0, st, a);
+  else if (a.narrow || EXACT) hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD, 4, true>), dim3(items), dim3(AT), 0, st, a);
+  else hipLaunchKernelGGL((paged_attn_kernel<XT, CT, HD, 4, EXACT>), dim3(items), dim3(AT), 0, st, a);
   OPS_HIP(hipGetLastError());
   if (a.nsplit > 1) {
     const unsigned n = (unsigned)(((int64_t)a.c.rows * a.n_q + 3) / 4);

@@ -119,7 +119,8 @@ def paged_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     has already appended the rows' own keys.  A row at slot s sees the `prefix_len` slots on the pages `prefix_table` (int32) and own slots 0 .. s.
     The prefix is read once for the batch, not once per sequence; `prefix_len = 0` is plain paged attention.  `scale` defaults to
     `head_dim ** -0.5`.  head_dim is 64 or 128, n_q any multiple of n_kv.  With float32 q everything is float32; with bfloat16 q the products
-    run on the bf16 matrix pipe with float32 sums, the softmax weights of the second one rounded to bfloat16 where more than 16 rows share a tile.
+    run on the bf16 matrix pipe with float32 sums, the softmax weights of the second one held in 16 bits (two bfloat16 pieces), or rounded to bfloat16
+    where the sequences bring more than 16 query rows (`rows * n_q / n_kv`) each on average.
 
     A row that sees no key gives zeros.  Rows of padding (`seq_lens < 0`) and rows behind `cu_rows[-1]` keep what `out` held (`out` may be `q`).
     Slots on pages outside the cache are not seen.  Slots that no row of the call sees may hold anything; a NaN or infinity in v of a slot that
