@@ -1,8 +1,10 @@
 // Sampling with temperature, top-k, top-p and min-p from one given uniform per row (include/csm_ops.h).
 //   w_i = exp((x_i - max) / T);  rows ordered by (x descending, index ascending);  every filter keeps a PREFIX of that order, so the kept set
 //   is "key > cut, and the first `ties` entries with key == cut";  the token is where the running sum of kept w (index order) passes u * total.
-// Sums are uint64 fixed point (w scaled by 2^min(62 - ceil log2 V, 51)) of weights computed in fp64: exact integer additions, so neither the
-// split over threads nor any order of arrival changes a result, and what is rounded away per weight is below 2^-45 of the largest.
+// Sums are uint64 fixed point of weights computed in fp64: exact integer additions, so neither the split over threads nor any order of arrival
+// changes a result.  The scale of a weight is 2^min(62 - ceil log2 n, 51) where at most n entries are summed (a row in registers, a list, a chunk: n <= 16 384),
+// and 2^min(61 - floor log2 mass, 51) where a long row is streamed, `mass` its total in units of the largest weight: what is rounded away per weight is
+// below 2^-49 of the largest, or 2^-61 of the total.
 //
 // No sort of the row: a histogram over its values (counts and masses, a few bins per thread, LDS atomics on integers) is summed from the top, the bin in
 // which a cut falls is gathered (at most 64 entries) and ranked exactly by one wave.  Rows whose values crowd in one bin go the long way:
@@ -24,7 +26,7 @@
 struct SampleOpArgs {
   const void* logits;
   int64_t stride;
-  int V, shift;   // shift: binary point of the fixed-point weights
+  int V, shift;   // shift: binary point of the weights where the whole row may be summed, whatever it holds
   const float *uniform, *temperatures, *top_ps, *min_ps;
   const int32_t* topks;
   float temperature, top_p, min_p;
@@ -37,6 +39,7 @@ struct SampleOpArgs {
   uint2* lists;            // [rows][chunks][CHUNK_CAP] (key, index)
 };
 constexpr int LIST = 1024 * 16;           // entries that fit the registers of a workgroup
+constexpr int LIST_SHIFT = 48;            // binary point of their weights: 2^14 of them stay within 2^62
 constexpr int SAMPLES = 4096, AIM = LIST * 3 / 4;   // the list's threshold is a sample's order statistic that aims at this many entries: at V = 131 072
                                                     // their number scatters by 613, LIST is 6.7 of that away
 // (a chunk of 8192 is 32 entries a thread: 16 chunks of a row of 128 256, so that 16 rows already fill the CUs)
@@ -927,7 +930,7 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
     return;
   }
   const double k2 = 1.4426950408889634074 / (double)s.T;
-  const Weigh weigh{mx, k2, a.shift};
+  Weigh weigh{mx, k2, LIST_SHIFT};
   // masses of the chunks in one scale, summed by one wave in a fixed order: the same bits every time
   if (tid < a.chunks) cum_s[tid] = h.mx == mx ? h.mass : h.mx == -INFINITY || mx == INFINITY ? 0.0 : h.mass * exp2(fmax(((double)h.mx - (double)mx) * k2, -1200.0));
   uint64_t n_list;
@@ -945,7 +948,7 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
       if (4 * lane + i < a.chunks) cum_s[4 * lane + i] = before + c[i];
   }
   __syncthreads();
-  const double all = cum_s[a.chunks - 1];
+  double all = cum_s[a.chunks - 1];
   const uint32_t key_max = K::key(mx);
 
   LongRow<XT, ALIGNED> src;
@@ -960,7 +963,7 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
     const double want = (double)s.u * all;
     int c = 0;
     while (c < a.chunks - 1 && !(cum_s[c] > want)) ++c;
-    const double rest = (want - (c ? cum_s[c - 1] : 0.0)) * (double)(1ull << a.shift);
+    const double rest = (want - (c ? cum_s[c - 1] : 0.0)) * (double)(1ull << LIST_SHIFT);
     constexpr int PER = CHUNK / NT;
     const int i0 = c * CHUNK + tid * PER;
     uint64_t w[PER], mine = 0, total;
@@ -996,7 +999,7 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
 
   bool ok = !crowded && n_list > 0 && n_list <= LIST;
   if (ok && s.k) ok = n_list >= (uint64_t)s.k || thr <= K::NONE + 1;
-  if (ok && !s.k && s.top_p >= 1.f) ok = thr <= K::NONE + 1 || (double)weigh(K::value(thr)) < (double)s.min_p * (double)(1ull << a.shift);   // min-p alone: all it keeps is listed
+  if (ok && !s.k && s.top_p >= 1.f) ok = thr <= K::NONE + 1 || (double)weigh(K::value(thr)) < (double)s.min_p * (double)(1ull << LIST_SHIFT);   // min-p alone: all it keeps is listed
   if (ok) {
     const uint2* lists = a.lists + (int64_t)row * a.chunks * CHUNK_CAP;
     for (int c = wave; c < a.chunks; c += 16) {
@@ -1019,7 +1022,7 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
     if (e == -2) {
       constexpr bool TABLE = sizeof(XT) == 2;
       if (!TABLE) r.template weigh_all<K>(weigh);
-      e = filter_and_draw<K, TABLE>(r, blk, &hist, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << a.shift), enough);
+      e = filter_and_draw<K, TABLE>(r, blk, &hist, &few, weigh, s, n, thr, key_max, s.k ? -1.0 : all * (double)(1ull << LIST_SHIFT), enough);
     }
     if (e >= 0) {
       const uint32_t p = tid * r.per + e;
@@ -1034,9 +1037,17 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   Cut cut{0u, 0u, 0u};
   {
     uint32_t n;
-    uint64_t none = 0;
-    src.template stat<false>(K::NONE + 1, n, none);
-    n = blk.count(n);
+    uint64_t sum = 0;
+    if (!s.k && s.top_p < 1.f) {
+      src.template stat<false>(K::NONE + 1, n, sum);
+      n = blk.count(n);
+    } else {   // the chunks' masses are not there: the total in the coarsest scale (2^21 weights within 2^-21 of it) finds the finest that holds it
+      weigh.shift = a.shift;
+      src.template stat<true>(K::NONE + 1, n, sum);
+      blk.template sum<true>(n, sum);
+      all = ldexp((double)sum, -a.shift);
+    }
+    weigh.shift = min(61 - ilogb(all), 51);
     if (s.k && (uint32_t)s.k < n) cut = find_cut<K, false>(src, blk, &few, weigh, K::NONE + 1, n, 0, key_max + 1, (uint32_t)s.k, 0.0);
   }
   if (s.top_p < 1.f) {

@@ -104,7 +104,8 @@ int csm_ops_paged_prefix_attention(const csm_ops_attention_t* a, void* stream);
  * [0, 1) is clamped to it.  topk <= 0 or >= V, top_p >= 1, min_p <= 0 switch that filter off; the first entry is always kept.  The pointers
  * give one value per row and win over the scalars; NULL = the scalar for all rows.  Per-row values the kernel cannot use are read as the
  * nearest that it can (temperature < 0 or NaN: 0; top_p < 0 or NaN: 0; min_p > 1: 1, NaN: 0).  V up to 2^21.  Weights are
- * computed in fp64 and summed in 64-bit fixed point, chunks of a long row in fp64 in their order: the same input gives the same token. */
+ * computed in fp64 and summed in 64-bit fixed point, chunks of a long row in fp64 in their order: the same input gives the same token.  A weight is
+ * held to 2^-49 of the row's largest, or to 2^-61 of their sum where that is more; smaller ones count as 0. */
 typedef struct {
   const void* logits;                 /* [rows][V] at logits_stride, any alignment */
   int64_t logits_stride;

@@ -1,11 +1,12 @@
 """The stand-alone operators of include/csm_ops.h where they are used otherwise than in test_paged_ops.py: roundings of single steps, settings and
 sizes at the end of their ranges, calls that have to be refused.  Tolerances count roundings (half a step: fp32 2^-24, bf16 2^-8)."""
+import math
 
 import pytest
 import torch
 
-from csm_hf_amd import paged_prefix_attention
-from test_paged_ops import BF16, Cache, DEV, HALF, attention64, check
+from csm_hf_amd import paged_prefix_attention, sample_filtered
+from test_paged_ops import BF16, Cache, DEV, F32, HALF, attention64, check
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------
@@ -27,3 +28,29 @@ def _abs_v(cache):
     other = object.__new__(Cache)
     other.__dict__.update(cache.__dict__, v=cache.v.abs())
     return other
+
+
+# ---- sampling ------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("how", ["all", "top_p", "topk", "min_p"])
+@pytest.mark.parametrize("V,low,first,u", [(2 ** 21, -29.75, True, 1 - 2.0 ** -24), (2 ** 21, -31.0, False, 2.0 ** -27), (2 ** 18 + 1, -30.0, False, 2.0 ** -27), (2 ** 17, -30.0, False, 2.0 ** -28)])
+def test_sample_flat_tail_of_the_longest_rows(V, low, first, u, how, dtype):
+    """One dominant value and a flat tail of V - 1 others that holds 2^-27 to 2^-22 of the mass, with a target inside it.  A weight is off by 2^-52 of the
+    largest at most (2^-49 where the row's chunks are drawn from): with x = (u (1 + n w) - 1) / w, or u (1 + n w) / w, and the tail's mass above 1 - u (or u),
+    V of these roundings move x by at most V 2^-52 / w places, a nucleus that cuts the tail by as much again."""
+    if how == "top_p" and V < 2 ** 21:
+        pytest.skip("the tail is smaller than what the largest top_p below 1 leaves out")
+    x = torch.full((1, V), low)
+    x[0, 0 if first else V - 1] = 0.0
+    w, n = math.exp(low), V - 1
+    kw = {"all": dict(), "top_p": dict(top_p=1 - 2.0 ** -24), "topk": dict(topk=V - V // 8), "min_p": dict(min_p=w / 2)}[how]
+    if how == "topk":
+        n = kw["topk"] - 1
+    if how == "top_p":
+        n = min(n, max(0, math.ceil((kw["top_p"] * (1 + n * w) - 1) / w)))
+    want = u * (1 + n * w)
+    place = (want - 1) / w + 1 if first else want / w        # tail entries in front of the token
+    got = int(sample_filtered(x.to(dtype).to(DEV), torch.tensor([u], device=DEV), **kw))
+    assert 0 < place < n
+    assert abs(got - place) <= 2 * (V * 2.0 ** -52 + (8192 * 2.0 ** -49 if how == "all" else 0)) / w + 1
