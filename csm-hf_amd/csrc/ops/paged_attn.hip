@@ -21,6 +21,7 @@
 // ds_read_b64_tr_b16, which hands out the columns.  The running reference m moves only when a score exceeds it by 2^8 (p <= 256 is harmless in
 // fp32 sums), so no cross-lane maximum and no rescaling happen in most tiles.
 #include "ops_common.h"
+#include <float.h>
 #include <math.h>
 
 typedef __attribute__((ext_vector_type(8))) short b16x8;
@@ -45,6 +46,7 @@ struct AttnOpArgs {
 };
 
 constexpr int AT = 256, MAX_SPLIT = 64;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr int tile_rows(int x_dtype) { return x_dtype == CSM_OPS_BF16 ? 128 : 64; }
 constexpr float SLACK = 8.f;
 
@@ -902,7 +904,7 @@ static int check(const csm_ops_attention_t* p) {
   const int64_t strides[4] = {c.k_page_stride, c.k_slot_stride, c.v_page_stride, c.v_slot_stride};
   for (int64_t x : strides)
     if (x / unit >= 1 << 24 || c.n_pages > 1 << 24) return ops_fail(CSM_OPS_ERR_CAPACITY, "more than 2^24 pages, or pages or slots 256 MB apart");
-  if (!isfinite(p->scale)) return ops_fail(CSM_OPS_ERR_ARG, "scale must be finite");
+  if (!isfinite(p->scale * LOG2E)) return ops_fail(CSM_OPS_ERR_ARG, "scale must be finite, and so must scale * log2(e)");
   if (!c.rows) return 0;
   if (!p->q || !p->out || (p->prefix_len && !p->prefix_table)) return ops_fail(CSM_OPS_ERR_ARG, "null pointer");
   if (!ops_aligned(p->q) || !ops_aligned(p->out) || !ops_stride16(p->q_stride, p->x_dtype) || !ops_stride16(p->out_stride, p->x_dtype))
@@ -1000,8 +1002,8 @@ extern "C" int csm_ops_paged_prefix_attention(const csm_ops_attention_t* p, void
   a.part = reinterpret_cast<float*>(p->workspace);
   a.ml = need ? reinterpret_cast<float2*>(a.part + (size_t)c.rows * p->n_q * a.nsplit * c.head_dim) : nullptr;
   a.q_flip = p->scale < 0.f ? 0x80000000u : 0u;
-  // a scale of 0 becomes one that no finite score can raise above 0: -inf times it is still -inf
-  a.c2 = fmaxf(fabsf(p->scale) * 1.4426950408889634f, 1e-37f);
+  // a scale of 0 becomes the smallest there is: -inf times it is still -inf, and the largest finite score is 5e-7
+  a.c2 = fmaxf(fabsf(p->scale) * LOG2E, FLT_TRUE_MIN);
   hipStream_t st = (hipStream_t)stream;
   const bool xb = p->x_dtype == CSM_OPS_BF16, cb = c.dtype == CSM_OPS_BF16;
   if (c.head_dim == 64) return xb ? launch<bf16_t, bf16_t, 64>(a, st) : cb ? launch<float, bf16_t, 64>(a, st) : launch<float, float, 64>(a, st);

@@ -5,8 +5,8 @@ import math
 import pytest
 import torch
 
-from csm_hf_amd import paged_prefix_attention, sample_filtered
-from test_paged_ops import BF16, Cache, DEV, F32, HALF, attention64, check
+from csm_hf_amd import ops, paged_prefix_attention, sample_filtered
+from test_paged_ops import BF16, Cache, DEV, F32, HALF, _cu, _paged_args, attention64, check
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------
@@ -28,6 +28,30 @@ def _abs_v(cache):
     other = object.__new__(Cache)
     other.__dict__.update(cache.__dict__, v=cache.v.abs())
     return other
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("x,c", [(BF16, BF16), (F32, BF16), (F32, F32)])
+@pytest.mark.parametrize("new", [[1, 1], [1, 40]])
+@pytest.mark.parametrize("scale", [0.0, 5e-38, -5e-38, 1e-44])
+def test_attention_smallest_scales(scale, new, x, c):
+    """scores near 1e37 under scales below 1e-37: a plain mean for a scale of 0, the softmax of the scaled scores for the others"""
+    lens, prefix = [90, 300], 70
+    cache = Cache(lens, 16, 2, 64, c, prefix=prefix, seed=3)
+    cache.k *= 1e18
+    q = (torch.randn(sum(new), 4, 64, generator=torch.Generator().manual_seed(3)) * 1e18).to(x).to(DEV)
+    got = paged_prefix_attention(q, *cache.args(), prefix_table=cache.prefix, prefix_len=prefix, cu_rows=_cu(new), scale=scale)
+    s = float(torch.tensor(scale, dtype=F32))
+    want, tol = attention64(q, cache, lens, new, 4, s, x == BF16)
+    # scale * log2(e) is a denormal number of steps of 2^-149, off by one of them: 2^-149 times scores of at most 64 * 5e18 * 5e18 is 2^-18
+    check(got, want, tol + 2 * 2.0 ** -18, 0.0)
+
+
+def test_scales_that_are_not_finite_in_powers_of_two_are_refused():
+    lib = ops.load_ops_library()
+    a = ops.AttentionArgs(q=1 << 24, out=1 << 25, q_stride=256, out_stride=256, x_dtype=1, n_q=4, scale=3e38, workspace=1 << 28, workspace_bytes=1 << 27)
+    _paged_args(a.c)
+    assert lib.csm_ops_paged_prefix_attention(bytes(a), None) == -1
 
 
 # ---- sampling ------------------------------------------------------------------------------------------------------------
