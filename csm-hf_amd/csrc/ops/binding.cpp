@@ -5,6 +5,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <cmath>
 #include <limits>
@@ -19,7 +20,7 @@ struct Refused { PyObject* type; std::string text; };   // type nullptr: the Pyt
 [[noreturn]] void refuse(const std::string& text) { throw Refused{PyExc_ValueError, text}; }
 void need(bool ok, const char* text) { if (!ok) refuse(text); }
 
-// The tensors of one call: all on one GPU, none that asks for a gradient.
+// The tensors of one call: all on one GPU, with values in their memory, none that asks for a derivative.
 struct Call {
   int device = -1;
   c10::OptionalDeviceGuard guard;   // the tensors' device is current from the first of them on, until the call returns
@@ -38,6 +39,11 @@ struct Call {
     if (t.get_device() != device) refuse(std::string(name) + " is on cuda:" + std::to_string(t.get_device()) + ", expected cuda:" + std::to_string(device));
     if (t.requires_grad() && at::GradMode::is_enabled())
       throw Refused{PyExc_RuntimeError, std::string(name) + " requires a gradient: this operator has no backward pass (call it under torch.no_grad())"};
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+      throw Refused{PyExc_RuntimeError, std::string(name) + " has a forward-mode tangent: this operator has no derivative"};
+    // wrappers of function transforms (vmap, jvp) have no memory of their own; a lazily negated view holds other values than it stands for
+    if (!t.has_storage()) throw Refused{PyExc_RuntimeError, std::string(name) + " is a tensor inside a function transform: this operator cannot be transformed"};
+    if (t.is_neg()) refuse(std::string(name) + " is a negated view: pass its resolve_neg()");
     return t;
   }
   const at::Tensor* maybe(const char* name, PyObject* o) { return o == Py_None ? nullptr : &take(name, o); }

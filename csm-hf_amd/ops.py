@@ -7,7 +7,8 @@
 The reference has no paged cache; the arithmetic is that of its decode step (rotary embedding, grouped-query attention and `sample_topk`,
 modeling_csm.py:170-189, 345-354), and the tables are `csm_hf_amd.engine.rope_tables`.  All three launch on the CURRENT torch stream of the
 tensors' device, do not synchronise, keep nothing between calls and can be captured into a graph.  Inference only: a tensor that asks for a
-gradient is refused while gradients are enabled.  There is no CPU fallback."""
+gradient is refused while gradients are enabled, and so are tensors with a forward-mode tangent and tensors inside a function transform
+(`torch.func.vmap`, `jvp`).  There is no CPU fallback."""
 from __future__ import annotations
 
 import ctypes as C

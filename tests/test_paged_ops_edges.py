@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from csm_hf_amd import ops, paged_prefix_attention, sample_filtered
+from csm_hf_amd import ops, paged_prefix_attention, paged_rope_append, sample_filtered
 from test_paged_ops import BF16, Cache, DEV, F32, HALF, _cu, _paged_args, attention64, check
 
 
@@ -78,3 +78,35 @@ def test_sample_flat_tail_of_the_longest_rows(V, low, first, u, how, dtype):
     got = int(sample_filtered(x.to(dtype).to(DEV), torch.tensor([u], device=DEV), **kw))
     assert 0 < place < n
     assert abs(got - place) <= 2 * (V * 2.0 ** -52 + (8192 * 2.0 ** -49 if how == "all" else 0)) / w + 1
+
+
+# ---- refusals --------------------------------------------------------------------------------------------------------------
+def _calls():
+    """each operator as a function of one of its tensors, that tensor, and the words its name has in a refusal"""
+    c = Cache([5, 5], 16, 2, 64, F32, prefix=16)
+    q, qkv, tab = torch.randn(2, 4, 64, device=DEV), torch.randn(2, 8 * 64, device=DEV), torch.rand(32, 32, device=DEV)
+    x, u = torch.randn(2, 99, device=DEV), torch.rand(2, device=DEV)
+    return [(lambda t: paged_prefix_attention(t, *c.args()), q), (lambda t: paged_prefix_attention(q, t, c.v, c.table, c.lens), c.k),
+            (lambda t: paged_rope_append(t, tab, tab, *c.args()), qkv), (lambda t: paged_rope_append(qkv, tab, t, *c.args()), tab),
+            (lambda t: sample_filtered(t, u), x), (lambda t: sample_filtered(x, u, temperature=t), u)]
+
+
+@pytest.mark.gpu
+def test_tangents_transforms_and_negated_views_are_refused():
+    import torch.autograd.forward_ad as fwd
+    for f, t in _calls():
+        f(t)
+        with fwd.dual_level():
+            dual = fwd.make_dual(t, torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="tangent"):
+                f(dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                f(dual)
+            f(fwd.unpack_dual(dual).primal)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (t,), (torch.ones_like(t),))
+        with pytest.raises(RuntimeError, match="function transform"):
+            torch.func.vmap(f)(t[None])
+        with pytest.raises(ValueError, match="negated"):
+            f(torch._neg_view(t))
+        f(t)
