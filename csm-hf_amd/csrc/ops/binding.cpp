@@ -74,6 +74,9 @@ const int32_t* ints(const char* name, const at::Tensor& t, int64_t n) {
   return (const int32_t*)t.data_ptr();
 }
 
+// what a call wrote: autograd notices when it has saved the tensor for a backward pass (inference tensors have no version to raise)
+void written(const at::Tensor& t) { if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
+
 void paged(Call& call, csm_ops_paged_t& c, PyObject* k_obj, PyObject* v_obj, PyObject* table_obj, PyObject* lens_obj, PyObject* cu_obj, int64_t rows) {
   const at::Tensor &k = call.take("k_cache", k_obj), &v = call.take("v_cache", v_obj), &table = call.take("page_table", table_obj), &lens = call.take("seq_lens", lens_obj);
   need(k.dim() == 4 && dtype_of(k) >= 0 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(),
@@ -147,6 +150,7 @@ PyObject* rope_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
     a.cos = (const float*)cos.data_ptr(); a.sin = (const float*)sin.data_ptr();
     a.rope_positions = i32("positions", cos.size(0)); a.pos_offset = py_i32("pos_offset", o[8]);
     done(csm_ops_paged_rope_append(&a, call.stream()));
+    written(THPVariable_Unpack(o[3])); written(THPVariable_Unpack(o[4])); written(q);
     return result(o[9], q);
   });
 }
@@ -180,6 +184,7 @@ PyObject* prefix_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
       a.workspace = scratch.data_ptr();
     }
     done(csm_ops_paged_prefix_attention(&a, call.stream()));
+    written(out);
     return result(o[9], out);
   });
 }

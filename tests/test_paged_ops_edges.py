@@ -110,3 +110,27 @@ def test_tangents_transforms_and_negated_views_are_refused():
         with pytest.raises(ValueError, match="negated"):
             f(torch._neg_view(t))
         f(t)
+
+
+@pytest.mark.gpu
+def test_writes_into_tensors_saved_for_a_backward_pass_are_noticed():
+    """autograd raises instead of using a cache or an output that a call has changed since"""
+    c = Cache([5, 5], 16, 2, 64, F32)
+    qkv, tab = torch.randn(2, 8 * 64, device=DEV), torch.rand(32, 32, device=DEV)
+    q_out, out = torch.zeros(2, 4, 64, device=DEV), torch.zeros(2, 4, 64, device=DEV)
+    append = lambda: paged_rope_append(qkv, tab, tab, *c.args(), q_out=q_out)  # noqa: E731
+    attend = lambda: paged_prefix_attention(q_out, *c.args(), out=out)  # noqa: E731
+    for saved, call in ((c.k, append), (c.v, append), (q_out, append), (out, attend)):
+        w = torch.ones_like(saved, requires_grad=True)
+        y = (w * saved).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    w = torch.ones_like(q_out, requires_grad=True)
+    y = (w * q_out).sum()
+    attend()                                              # reads q and the cache
+    y.backward()
+    assert torch.equal(w.grad, q_out)
+    with torch.inference_mode():
+        k = c.k.clone()
+    paged_rope_append(qkv, tab, tab, k, c.v, c.table, c.lens)
