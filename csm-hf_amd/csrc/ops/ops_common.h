@@ -9,6 +9,8 @@ int ops_check_paged(const csm_ops_paged_t& c);          // 0 or a recorded failu
 inline bool ops_aligned(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 inline size_t ops_size(int dtype) { return dtype == CSM_OPS_BF16 ? 2 : 4; }
 inline bool ops_stride16(int64_t s, int dtype) { return (s * (int64_t)ops_size(dtype)) % 16 == 0; }
+// a launch has fewer than 2^32 threads in all: checked before the first launch of a call
+inline bool ops_launchable(int64_t workgroups, int threads) { return workgroups * threads <= 0xffffffffll; }
 #define OPS_HIP(call)                                                                             \
   do {                                                                                            \
     const hipError_t e_ = (call);                                                                 \

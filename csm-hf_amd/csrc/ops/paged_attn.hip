@@ -949,7 +949,9 @@ static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {
   a.nsp = np ? splits(np * c.n_kv, p->prefix_len, 64, 64, 256) : 0;
   a.nso = a.tall ? 1 : splits(own_tiles * c.n_kv, own_keys, 512, 128, a.narrow ? 2048 : 0);
   a.np_tiles = (int)np; a.no_tiles = (int)own_tiles; a.nsplit = a.nsp + a.nso;
-  if (((int64_t)a.np_tiles * a.nsp + (int64_t)a.no_tiles * a.nso) * c.n_kv > 0x7fffffff) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
+  if (!ops_launchable(((int64_t)a.np_tiles * a.nsp + (int64_t)a.no_tiles * a.nso) * c.n_kv, a.tall ? 1024 : AT) ||
+      (a.nsplit > 1 && !ops_launchable(((int64_t)c.rows * p->n_q + 3) / 4, AT)))
+    return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
   return 0;
 }
 static size_t workspace(const csm_ops_attention_t* p, const AttnOpArgs& a) {

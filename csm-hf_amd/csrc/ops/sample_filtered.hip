@@ -39,6 +39,7 @@ struct SampleOpArgs {
   uint2* lists;            // [rows][chunks][CHUNK_CAP] (key, index)
 };
 constexpr int LIST = 1024 * 16;           // entries that fit the registers of a workgroup
+constexpr int SHORT = 256 * 16;           // entries that fit those of a small one
 constexpr int LIST_SHIFT = 48;            // binary point of their weights: 2^14 of them stay within 2^62
 constexpr int SAMPLES = 4096, AIM = LIST * 3 / 4;   // the list's threshold is a sample's order statistic that aims at this many entries: at V = 131 072
                                                     // their number scatters by 613, LIST is 6.7 of that away
@@ -1130,7 +1131,8 @@ static int check(const csm_ops_sample_t* p) {
   if (p->x_dtype != CSM_OPS_F32 && p->x_dtype != CSM_OPS_BF16) return ops_fail(CSM_OPS_ERR_ARG, "unknown dtype %d", p->x_dtype);
   if (p->rows < 0 || p->V < 1) return ops_fail(CSM_OPS_ERR_ARG, "rows must not be negative and V must be positive");
   if (p->V > MAX_V) return ops_fail(CSM_OPS_ERR_CAPACITY, "V = %d: at most 2^21", p->V);
-  if ((int64_t)p->rows * ((p->V + CHUNK - 1) / CHUNK) > 0x7fffffff) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
+  const bool lists = p->V > LIST;
+  if (!ops_launchable(p->rows, p->V > SHORT ? 1024 : 256) || (lists && !ops_launchable((int64_t)p->rows * ((p->V + CHUNK - 1) / CHUNK), 256))) return ops_fail(CSM_OPS_ERR_CAPACITY, "too many rows for one launch");
   if (!p->temperatures && !(p->temperature >= 0.f && p->temperature < INFINITY)) return ops_fail(CSM_OPS_ERR_ARG, "temperature must be finite and not negative");
   if (!p->topks && (p->topk < 0 || p->topk > p->V)) return ops_fail(CSM_OPS_ERR_ARG, "selected index k out of range");
   if (!p->top_ps && !(p->top_p > 0.f && p->top_p <= 1.f)) return ops_fail(CSM_OPS_ERR_ARG, "top_p must lie in (0, 1]");
@@ -1189,7 +1191,7 @@ extern "C" int csm_ops_sample_filtered(const csm_ops_sample_t* p, void* stream) 
   if (p->V <= 256 * 4) {
     if (b) hipLaunchKernelGGL((sample_short_kernel<256, 4, bf16_t>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((sample_short_kernel<256, 4, float>), grid, dim3(256), 0, st, a);
-  } else if (p->V <= 256 * 16) {
+  } else if (p->V <= SHORT) {
     if (b) hipLaunchKernelGGL((sample_short_kernel<256, 16, bf16_t>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((sample_short_kernel<256, 16, float>), grid, dim3(256), 0, st, a);
   } else if (p->V <= LIST) {

@@ -1,5 +1,6 @@
 """The stand-alone operators of include/csm_ops.h where they are used otherwise than in test_paged_ops.py: roundings of single steps, settings and
 sizes at the end of their ranges, calls that have to be refused.  Tolerances count roundings (half a step: fp32 2^-24, bf16 2^-8)."""
+import ctypes as C
 import math
 
 import pytest
@@ -134,3 +135,31 @@ def test_writes_into_tensors_saved_for_a_backward_pass_are_noticed():
     with torch.inference_mode():
         k = c.k.clone()
     paged_rope_append(qkv, tab, tab, k, c.v, c.table, c.lens)
+
+
+@pytest.mark.parametrize("refused,over", [
+    (True, dict(rows=1 << 24, n_seqs=1 << 24)), (False, dict(rows=1 << 22, n_seqs=1 << 22)),
+    # many short sequences of 31 query rows a kv-head: the partial results' launch is the largest
+    (True, dict(rows=2200000, n_seqs=2200000, n_q=31, n_kv=1, prefix_table=1 << 26, prefix_pages=2, prefix_len=32)),
+    (False, dict(rows=2100000, n_seqs=2100000, n_q=31, n_kv=1, prefix_table=1 << 26, prefix_pages=2, prefix_len=32))])
+def test_attention_launches_of_2_32_threads_are_refused(refused, over):
+    """before anything is launched: sizes that fit are only asked for their workspace"""
+    lib, need = ops.load_ops_library(), C.c_size_t()
+    a = ops.AttentionArgs(q=1 << 24, out=1 << 25, q_stride=31 * 64 + 64, out_stride=31 * 64 + 64, x_dtype=0, n_q=4, scale=0.125, workspace=1 << 28, workspace_bytes=1 << 60)
+    _paged_args(a.c, **over)
+    for k, v in over.items():
+        if not hasattr(a.c, k):
+            setattr(a, k, v)
+    assert lib.csm_ops_paged_attention_workspace(bytes(a), C.byref(need)) == (-3 if refused else 0)
+    if refused:
+        assert lib.csm_ops_paged_prefix_attention(bytes(a), None) == -3 and b"one launch" in lib.csm_ops_last_error()
+
+
+@pytest.mark.parametrize("V,rows", [(1000, 1 << 24), (4096, 1 << 24), (4097, 1 << 22), (16384, 1 << 22), (16385, 1 << 22), (131072, 1 << 20), (1 << 21, 1 << 16)])
+def test_sample_launches_of_2_32_threads_are_refused(V, rows):
+    lib, need = ops.load_ops_library(), C.c_size_t()
+    a = ops.SampleArgs(logits=1 << 20, logits_stride=0, x_dtype=0, rows=rows, V=V, uniform=1 << 21, temperature=1.0, top_p=0.5, out=1 << 22, workspace=1 << 30, workspace_bytes=1 << 60)
+    assert lib.csm_ops_sample_workspace(bytes(a), C.byref(need)) == -3
+    assert lib.csm_ops_sample_filtered(bytes(a), None) == -3 and b"one launch" in lib.csm_ops_last_error()
+    a.rows -= 1
+    assert lib.csm_ops_sample_workspace(bytes(a), C.byref(need)) == 0
