@@ -107,7 +107,7 @@ def paged_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k
 
     A sequence with `seq_lens < 0` is padding.  Its rows, rows behind `cu_rows[-1]` and rows whose slot, page or rotary position lies outside the
     table, the cache or the tables are skipped: nothing is written for them, in q_out either.  Two rows that share a cache slot (a page that
-    two sequences write to) leave either row's values there.  q, k and v must not overlap in memory with the cache."""
+    two sequences write to) leave either row's values there.  q, k and v must not overlap in memory with the cache, nor k_cache with v_cache."""
     return (_binding or _load_binding()).rope_append(qkv, cos, sin, k_cache, v_cache, page_table, seq_lens, cu_rows, pos_offset, q_out)
 
 

@@ -11,7 +11,8 @@
  *     hipStream_t of it.  Argument structs live in host memory and are read before the call returns.
  *   - strides count ELEMENTS.  Rows, caches and tables must start on 16 bytes and their strides must keep 16-byte alignment where the
  *     struct says "16 B"; the innermost dimension is contiguous everywhere.  Inputs may share memory between rows (a stride of 0); rows
- *     of an output, and slots of a cache that is written, may not.
+ *     of an output, and slots of a cache that is written, may not: its strides must nest (each at least what the smaller ones span), and K and V
+ *     must lie apart.
  *   - what only the device knows (lengths, page numbers, row offsets) is bounds-checked by the kernels: nothing outside the given tensors
  *     is ever read or written, whatever these arrays hold.
  *

@@ -163,3 +163,43 @@ def test_sample_launches_of_2_32_threads_are_refused(V, rows):
     assert lib.csm_ops_sample_filtered(bytes(a), None) == -3 and b"one launch" in lib.csm_ops_last_error()
     a.rows -= 1
     assert lib.csm_ops_sample_workspace(bytes(a), C.byref(need)) == 0
+
+
+def _append_args(**over):
+    a = ops.RopeAppendArgs(qkv=1 << 24, q_out=1 << 25, qkv_stride=384, q_out_stride=128, x_dtype=1, n_q=2, cos=1 << 26, sin=1 << 27, rope_positions=64)
+    _paged_args(a.c, **over)
+    return a
+
+
+# (4 pages of 2 heads of 16 slots of 64 bf16 values)
+@pytest.mark.parametrize("over", [
+    dict(k_page_stride=64), dict(k_page_stride=1024), dict(v_head_stride=512), dict(v_page_stride=1984), dict(k_page_stride=1024, k_head_stride=1024), dict(k_slot_stride=128),
+    dict(v=1 << 20), dict(v=(1 << 20) + 2048), dict(v=(1 << 20) + 2 * 2 * 2048, n_pages=3), dict(k=(1 << 21) + 64), dict(v=1 << 20, v_page_stride=4096)])
+def test_append_refuses_caches_whose_slots_overlap(over):
+    assert ops.load_ops_library().csm_ops_paged_rope_append(bytes(_append_args(**over)), None) == -1 and b"overlap" in ops.load_ops_library().csm_ops_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("make", [
+    lambda n: torch.zeros(n, 2, 2, 16, 64, device=DEV).unbind(1), lambda n: torch.zeros(2, n, 2, 16, 64, device=DEV).unbind(0), lambda n: torch.zeros(n, 2, 16, 2, 64, device=DEV).unbind(3),
+    lambda n: torch.zeros(n, 16, 2, 2, 64, device=DEV).permute(3, 0, 2, 1, 4).unbind(0), lambda n: torch.zeros(n, 2, 16, 128, device=DEV).split(64, 3), lambda n: torch.zeros(2 * n, 2, 16, 64, device=DEV).unflatten(0, (n, 2)).unbind(1)[::-1],
+    lambda n: torch.zeros(2, n, 16, 128, device=DEV).permute(1, 0, 2, 3).split(64, 3), lambda n: (torch.zeros(n, 2, 16, 64, device=DEV), torch.zeros(n, 16, 2, 64, device=DEV).transpose(1, 2))])
+def test_append_into_one_buffer_for_k_and_v(make):
+    """every order of pages, heads, slots, and of K beside V, that keeps the slots apart"""
+    c = Cache([9, 33, 1], 16, 2, 64, F32, seed=2)
+    k, v = make(c.k.shape[0])
+    qkv, tab = torch.randn(43, 8 * 64, device=DEV), torch.rand(33, 32, device=DEV)
+    for t in (c.k, c.v):
+        t.zero_()
+    cu = _cu([9, 33, 1])
+    assert torch.equal(paged_rope_append(qkv, tab, tab, k, v, c.table, c.lens, cu_rows=cu), paged_rope_append(qkv, tab, tab, *c.args(), cu_rows=cu))
+    assert torch.equal(k, c.k) and torch.equal(v, c.v)
+
+
+@pytest.mark.gpu
+def test_append_refuses_one_tensor_for_both_caches():
+    c = Cache([5], 16, 2, 64, F32)
+    qkv, tab = torch.randn(1, 8 * 64, device=DEV), torch.rand(32, 32, device=DEV)
+    for k, v in ((c.k, c.k), (c.k[:-1], c.k[1:]), (c.k[:1].expand(3, 2, 16, 64), c.v[:3])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            paged_rope_append(qkv, tab, tab, k, v, c.table, c.lens)
