@@ -36,15 +36,20 @@ struct SampleOpArgs {
   int chunks;
   uint32_t* thr;           // [rows]
   struct ChunkHead* heads; // [rows][chunks]
-  uint2* lists;            // [rows][chunks][CHUNK_CAP] (key, index)
+  uint2* lists;            // [rows][chunks][CHUNK] (key, index)
 };
 constexpr int LIST = 1024 * 16;           // entries that fit the registers of a workgroup
 constexpr int SHORT = 256 * 16;           // entries that fit those of a small one
 constexpr int LIST_SHIFT = 48;            // binary point of their weights: 2^14 of them stay within 2^62
 constexpr int SAMPLES = 4096, AIM = LIST * 3 / 4;   // the list's threshold is a sample's order statistic that aims at this many entries: at V = 131 072
                                                     // their number scatters by 613, LIST is 6.7 of that away
-// (a chunk of 8192 is 32 entries a thread: 16 chunks of a row of 128 256, so that 16 rows already fill the CUs)
-constexpr int CHUNK = 8192, CHUNK_CAP = 2048, MAX_V = 1 << 21, MAX_CHUNKS = MAX_V / CHUNK;
+// (a chunk of 8192 is 32 entries a thread: 16 chunks of a row of 128 256, so that 16 rows already fill the CUs).  Any chunk may list all it has, so the
+// list fails by its total alone, wherever in the row the large values stand.  The rows that stream for it: a nucleus (or what min-p keeps) larger than the list;
+// more equal values at the threshold than fit; a sample far off -- the total scatters by sqrt(3 (V - 12 288)), so LIST is 4.7 of that away at V = 2^18, but
+// 2.3 at 2^20 and 1.6 at 2^21 (one row in a hundred, in twenty).  Chunk lists of 2048 overflowed in every row below V = 49 152, and where one chunk held 2.6 times
+// its share: 64 rows under top_p 0.9 (us, then / now) 177 / 48 at V = 16 385, 217 / 36 at 32 000, 432 / 42 at 50 257, 773 / 44 at 128 256 with the
+// largest values in the first chunk.
+constexpr int CHUNK = 8192, MAX_V = 1 << 21, MAX_CHUNKS = MAX_V / CHUNK;
 struct ChunkHead { double mass; float mx; int32_t at; uint32_t count, pad; };   // mass relative to the chunk's own maximum, `at` its first place
 
 // Order keys: larger value = larger key, one key per value of the type (a search that must end on a single key needs 16 fewer steps where
@@ -887,10 +892,10 @@ __global__ __launch_bounds__(256) void sample_chunk_kernel(SampleOpArgs a) {
   }
   if (mine) {
     uint32_t p = before + upto - mine;
-    uint2* list = a.lists + ((int64_t)row * a.chunks + chunk) * CHUNK_CAP;
+    uint2* list = a.lists + ((int64_t)row * a.chunks + chunk) * CHUNK;
 #pragma unroll
     for (int e = 0; e < PER; ++e)
-      if (v[e] >= thr) { if (p < CHUNK_CAP) list[p] = make_uint2(K::key(v[e]), (uint32_t)(i0 + e)); ++p; }
+      if (v[e] >= thr) list[p++] = make_uint2(K::key(v[e]), (uint32_t)(i0 + e));
   }
 }
 
@@ -937,7 +942,6 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
   uint64_t n_list;
   const uint64_t start = blk.before((uint64_t)(tid < a.chunks ? h.count : 0), n_list);
   if (tid < a.chunks) start_s[tid] = (uint32_t)start;
-  const uint32_t crowded = blk.count(__popcll(__ballot(h.count > CHUNK_CAP)));
   __syncthreads();
   if (tid < 64) {   // 4 consecutive chunks a lane
     double c[4], run = 0.0;
@@ -998,15 +1002,15 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
     return;
   }
 
-  bool ok = !crowded && n_list > 0 && n_list <= LIST;
+  bool ok = n_list > 0 && n_list <= LIST;
   if (ok && s.k) ok = n_list >= (uint64_t)s.k || thr <= K::NONE + 1;
   if (ok && !s.k && s.top_p >= 1.f) ok = thr <= K::NONE + 1 || (double)weigh(K::value(thr)) < (double)s.min_p * (double)(1ull << LIST_SHIFT);   // min-p alone: all it keeps is listed
   if (ok) {
-    const uint2* lists = a.lists + (int64_t)row * a.chunks * CHUNK_CAP;
+    const uint2* lists = a.lists + (int64_t)row * a.chunks * CHUNK;
     for (int c = wave; c < a.chunks; c += 16) {
       const uint32_t at = start_s[c], cnt = (c + 1 < a.chunks ? start_s[c + 1] : (uint32_t)n_list) - at;
 #pragma unroll 8
-      for (uint32_t i = lane; i < cnt; i += 64) keys[at + i] = lists[(int64_t)c * CHUNK_CAP + i].x;
+      for (uint32_t i = lane; i < cnt; i += 64) keys[at + i] = lists[(int64_t)c * CHUNK + i].x;
     }
     __syncthreads();
     RegRow<E> r;
@@ -1029,7 +1033,7 @@ __global__ __launch_bounds__(1024) void sample_list_kernel(SampleOpArgs a) {
       const uint32_t p = tid * r.per + e;
       int c = 0;
       while (c + 1 < a.chunks && start_s[c + 1] <= p) ++c;
-      a.out[row] = (int)lists[(int64_t)c * CHUNK_CAP + (p - start_s[c])].y;
+      a.out[row] = (int)lists[(int64_t)c * CHUNK + (p - start_s[c])].y;
     }
     if (enough) return;
   }
@@ -1146,8 +1150,8 @@ static size_t workspace(const csm_ops_sample_t* p, SampleOpArgs& a) {   // heads
   char* base = reinterpret_cast<char*>(p->workspace);
   a.heads = reinterpret_cast<ChunkHead*>(base);
   a.lists = reinterpret_cast<uint2*>(base + n * sizeof(ChunkHead));
-  a.thr = reinterpret_cast<uint32_t*>(base + n * (sizeof(ChunkHead) + CHUNK_CAP * sizeof(uint2)));
-  return n * (sizeof(ChunkHead) + CHUNK_CAP * sizeof(uint2)) + (size_t)p->rows * 4;
+  a.thr = reinterpret_cast<uint32_t*>(base + n * (sizeof(ChunkHead) + CHUNK * sizeof(uint2)));
+  return n * (sizeof(ChunkHead) + CHUNK * sizeof(uint2)) + (size_t)p->rows * 4;
 }
 
 extern "C" int csm_ops_sample_workspace(const csm_ops_sample_t* p, size_t* bytes) {

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from csm_hf_amd import ops, paged_prefix_attention, paged_rope_append, sample_filtered
-from test_paged_ops import BF16, Cache, DEV, F32, HALF, _cu, _paged_args, attention64, check
+from test_paged_ops import BF16, Cache, DEV, F32, HALF, _cu, _paged_args, _sample_case, attention64, check, f32
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------
@@ -79,6 +79,48 @@ def test_sample_flat_tail_of_the_longest_rows(V, low, first, u, how, dtype):
     got = int(sample_filtered(x.to(dtype).to(DEV), torch.tensor([u], device=DEV), **kw))
     assert 0 < place < n
     assert abs(got - place) <= 2 * (V * 2.0 ** -52 + (8192 * 2.0 ** -49 if how == "all" else 0)) / w + 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,skew", [(16385, 0), (20000, 0), (32000, 0), (50257, 0), (65000, 0), (128256, 2.0), (128256, 8.0)])
+def test_sample_long_rows_of_every_length(V, skew, dtype):
+    """lengths at which a chunk lists a large part of its entries, and rows whose large values all stand in one chunk"""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(3, V, generator=g) * 2.5
+    x[:, 8192:16384] += skew
+    u = torch.rand(3, generator=g)
+    for kw in (dict(top_p=f32(0.9)), dict(min_p=f32(0.05)), dict(topk=4000, top_p=f32(0.95))):
+        _sample_case(x.to(dtype), u, **kw)
+
+
+def _us(f):
+    """least time of a call among others, in microseconds"""
+    f()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(10):
+            f()
+    a, b, best = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True), math.inf
+    for _ in range(8):
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) * 100)
+    return best
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,skew", [(16385, 0), (20000, 0), (32000, 0), (50257, 0), (128256, 3.0)])
+def test_sample_long_rows_do_not_stream(V, skew):
+    """64 rows whose nucleus fits the list take about the time of 64 rows of 128 256 spread evenly (20 percent more at most; a search that streams over the
+    row takes four times as much and more)"""
+    g = torch.Generator().manual_seed(0)
+    make = lambda n: (torch.randn(64, n, generator=g) * 2.5).to(BF16).to(DEV)  # noqa: E731
+    even, x, u = make(128256), make(V), torch.rand(64, generator=g).to(DEV)
+    x[:, :8192] += skew
+    assert _us(lambda: sample_filtered(x, u, temperature=0.9, top_p=0.9)) < 2.5 * _us(lambda: sample_filtered(even, u, temperature=0.9, top_p=0.9))
 
 
 # ---- refusals --------------------------------------------------------------------------------------------------------------
