@@ -1,6 +1,7 @@
-"""Build libcsm_hip.so (gfx950) in-tree with hipcc.  No torch involvement: the library is a plain C-ABI
-shared object (include/csm_hip.h).  `python -m csm_hf_amd.build` or `build_library()`, which also build the stand-alone
-operators: libcsm_ops.so (include/csm_ops.h, plain C too) and its binding for torch tensors, _ops_binding.so."""
+"""Build libcsm_hip.so (include/csm_hip.h) and libcsm_ops.so (include/csm_ops.h) for gfx950 in-tree with hipcc: plain C-ABI shared objects, no
+torch involvement -- `python csm-hf_amd/build.py` makes them on a host without torch.  `python -m csm_hf_amd.build` or `build_library()`.
+Behind them comes _ops_binding.so, the operators' binding for torch tensors (g++, torch and Python headers): where it cannot be built the
+libraries stand all the same, and the torch entry points of csm_hf_amd.ops raise."""
 from __future__ import annotations
 
 import os
@@ -30,6 +31,7 @@ OPS_BINDING = os.path.join(HERE, "_ops_binding.so")   # csrc/ops/binding.cpp: th
 OPS_UNITS = ["ops_api", "paged_append", "paged_attn", "sample_filtered"]
 OPS_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Wno-pass-failed",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+BINDING_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__"]
 OPS_UNIT_FLAGS = {"paged_attn": ["-mllvm", "--amdgpu-mfma-vgpr-form"]}   # accumulators in VGPRs: the softmax reads every score at once
 
 
@@ -64,11 +66,20 @@ def sources_sha256() -> str:
 
 def build_library(force: bool = False, verbose: bool = False, defines=(), out: str = None) -> str:
     """`defines` / `out`: A/B variants of the same ABI (e.g. ("CSM_NO_PROBE",) -> libcsm_hip_noprobe.so), selected at
-    run time with the CSM_HIP_LIB environment variable."""
-    global OBJ
-    lib_out = out or LIB
+    run time with the CSM_HIP_LIB environment variable.  Without them the operators' library and its binding are built too."""
+    path = _build_engine(force, verbose, defines, out)
     if not defines and out is None:
         build_ops_library(force, verbose)
+        try:
+            build_ops_binding(force, verbose)
+        except Exception as e:
+            print(f"[build] no {os.path.basename(OPS_BINDING)} (csm_hf_amd.ops will raise): {e}", file=sys.stderr)
+    return path
+
+
+def _build_engine(force, verbose, defines, out) -> str:
+    global OBJ
+    lib_out = out or LIB
     if not force and not defines and os.path.exists(LIB) and os.path.getmtime(LIB) >= _sources_mtime():
         return LIB
     hipcc = _hipcc()
@@ -92,11 +103,15 @@ def build_library(force: bool = False, verbose: bool = False, defines=(), out: s
     return lib_out
 
 
+def _newer(path: str, deps) -> bool:
+    return os.path.exists(path) and os.path.getmtime(path) >= max(os.path.getmtime(f) for f in deps)
+
+
 def build_ops_library(force: bool = False, verbose: bool = False) -> str:
-    """libcsm_ops.so and _ops_binding.so from csrc/ops (include/csm_ops.h); reused when they are newer than their sources unless `force`."""
-    deps = [os.path.join(OPS_SRC, f) for f in os.listdir(OPS_SRC) if f.endswith((".hip", ".h", ".cpp"))]
+    """libcsm_ops.so from csrc/ops (include/csm_ops.h); reused when it is newer than its sources unless `force`."""
+    deps = [os.path.join(OPS_SRC, f) for f in os.listdir(OPS_SRC) if f.endswith((".hip", ".h"))]
     deps += [os.path.join(CSRC, "common.h"), os.path.join(os.path.dirname(HERE), "include", "csm_ops.h")]
-    if not force and all(os.path.exists(o) and os.path.getmtime(o) >= max(os.path.getmtime(f) for f in deps) for o in (OPS_LIB, OPS_BINDING)):
+    if not force and _newer(OPS_LIB, deps):
         return OPS_LIB
     hipcc, obj_dir = _hipcc(), os.path.join(OPS_SRC, "build")
     os.makedirs(obj_dir, exist_ok=True)
@@ -109,39 +124,55 @@ def build_ops_library(force: bool = False, verbose: bool = False) -> str:
         if verbose:
             print(f"[build] ops/{u}.o", file=sys.stderr)
 
-    with ThreadPoolExecutor(min(len(OPS_UNITS) + 1, os.cpu_count() or 4)) as ex:
-        binding = ex.submit(_compile_binding, obj_dir, verbose)
+    with ThreadPoolExecutor(min(len(OPS_UNITS), os.cpu_count() or 4)) as ex:
         list(ex.map(compile_one, OPS_UNITS))
-        binding.result()
     cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *[os.path.join(obj_dir, u + ".o") for u in OPS_UNITS], "-o", OPS_LIB]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr[-4000:]}")
-    import torch
-    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = ["g++", "-shared", os.path.join(obj_dir, "binding.o"), "-o", OPS_BINDING, "-L" + HERE, "-l:" + os.path.basename(OPS_LIB), "-Wl,-rpath,$ORIGIN",
-           "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link of the binding failed:\n{r.stderr[-4000:]}")
     return OPS_LIB
 
 
-def _compile_binding(obj_dir: str, verbose: bool):
+def binding_stamp() -> str:
+    """What _ops_binding.so has to have been built for: the installed torch (its inlined layouts are compiled in), this Python, the flags."""
     import sysconfig
     import torch
-    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    return (f"csm_ops binding for torch {torch.__version__} ({torch.version.git_version}), C++11 ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, "
+            f"{sysconfig.get_config_var('SOABI')}, {' '.join(BINDING_FLAGS)}")
+
+
+def build_ops_binding(force: bool = False, verbose: bool = False) -> str:
+    """_ops_binding.so from csrc/ops/binding.cpp; reused when it is newer than its sources and carries `binding_stamp()` unless `force`."""
+    import sysconfig
+    import torch
+    stamp, obj_dir = binding_stamp(), os.path.join(OPS_SRC, "build")
+    deps = [os.path.join(OPS_SRC, "binding.cpp"), os.path.join(os.path.dirname(HERE), "include", "csm_ops.h")]
+    if not force and _newer(OPS_BINDING, deps):
+        with open(OPS_BINDING, "rb") as f:
+            if stamp.encode() in f.read():
+                return OPS_BINDING
+    os.makedirs(obj_dir, exist_ok=True)
+    base = os.path.dirname(torch.__file__)
+    inc, lib = os.path.join(base, "include"), os.path.join(base, "lib")
     dirs = [inc, os.path.join(inc, "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"], os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *["-isystem" + d for d in dirs], "-c", os.path.join(OPS_SRC, "binding.cpp"), "-o", os.path.join(obj_dir, "binding.o")]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for ops/binding.cpp:\n{r.stderr[-4000:]}")
+    obj = os.path.join(obj_dir, "binding.o")
+    for what, cmd in (("g++ failed for ops/binding.cpp", ["g++", *BINDING_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DCSM_BINDING_STAMP="{stamp}"',
+                                                          *["-isystem" + d for d in dirs], "-c", deps[0], "-o", obj]),
+                      ("link of the binding failed", ["g++", "-shared", obj, "-o", OPS_BINDING, "-L" + HERE, "-l:" + os.path.basename(OPS_LIB), "-Wl,-rpath,$ORIGIN",
+                                                      "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"])):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"{what}:\n{r.stderr[-4000:]}")
     if verbose:
         print("[build] ops/binding.o", file=sys.stderr)
+    return OPS_BINDING
 
 
 if __name__ == "__main__":
     defs = tuple(a[2:] for a in sys.argv[1:] if a.startswith("-D"))
     outs = [a[6:] for a in sys.argv[1:] if a.startswith("--out=")]
     print(build_library(force="--force" in sys.argv or bool(defs), verbose=True, defines=defs, out=outs[0] if outs else None))
+    if not defs and not outs:
+        import importlib.util
+        if importlib.util.find_spec("torch"):   # with torch there is something to bind to: a binding that could not be built is an error
+            build_ops_binding()

@@ -237,4 +237,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops_binding", nullptr, -1, method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__ops_binding(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__ops_binding(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", CSM_BINDING_STAMP) < 0) Py_CLEAR(m);   // compared with what is installed when it is loaded
+  return m;
+}
