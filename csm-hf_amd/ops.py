@@ -24,7 +24,7 @@ OPS_EXPORTS = ["csm_ops_paged_rope_append", "csm_ops_paged_attention_workspace",
                "csm_ops_sample_filtered", "csm_ops_last_error", "csm_ops_abi_version"]
 
 
-# the argument structures of include/csm_ops.h, for callers of the C entries without torch
+# the argument structures of include/csm_ops.h, for callers of the C entries: load_ops_library().csm_ops_sample_filtered(ctypes.byref(args), stream)
 class PagedArgs(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
                 ("n_kv", C.c_int32), ("head_dim", C.c_int32),
@@ -68,9 +68,9 @@ def load_ops_library():
             fn = getattr(lib, name)
             fn.restype = C.c_int
             if name.endswith("_workspace"):
-                fn.argtypes = [C.c_char_p, C.POINTER(C.c_size_t)]
+                fn.argtypes = [C.c_void_p, C.POINTER(C.c_size_t)]
             elif name not in ("csm_ops_last_error", "csm_ops_abi_version"):
-                fn.argtypes = [C.c_char_p, C.c_void_p]
+                fn.argtypes = [C.c_void_p, C.c_void_p]
         lib.csm_ops_last_error.restype = C.c_char_p
         if lib.csm_ops_abi_version() != OPS_ABI_VERSION:
             raise RuntimeError(f"libcsm_ops.so ABI {lib.csm_ops_abi_version()} != binding {OPS_ABI_VERSION}")

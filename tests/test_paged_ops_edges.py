@@ -245,3 +245,23 @@ def test_append_refuses_one_tensor_for_both_caches():
     for k, v in ((c.k, c.k), (c.k[:-1], c.k[1:]), (c.k[:1].expand(3, 2, 16, 64), c.v[:3])):
         with pytest.raises(RuntimeError, match="overlap"):
             paged_rope_append(qkv, tab, tab, k, v, c.table, c.lens)
+
+
+def test_c_entries_take_structures_by_reference():
+    lib, need = ops.load_ops_library(), C.c_size_t()
+    s = ops.SampleArgs(logits=1 << 20, logits_stride=20000, rows=2, V=20000, uniform=1 << 21, temperature=1.0, top_p=0.5, out=1 << 22)
+    assert lib.csm_ops_sample_workspace(C.byref(s), C.byref(need)) == 0 and need.value > 0
+    assert lib.csm_ops_sample_filtered(C.byref(s), None) == -3                 # no workspace
+    assert lib.csm_ops_paged_rope_append(C.byref(_append_args(k_slot_stride=60)), None) == -1
+    a = ops.AttentionArgs(q=1 << 24, out=1 << 25, q_stride=256, out_stride=256, x_dtype=1, n_q=4, scale=0.125)
+    _paged_args(a.c)
+    assert lib.csm_ops_paged_attention_workspace(C.byref(a), C.byref(need)) == 0
+
+
+@pytest.mark.gpu
+def test_c_entry_on_a_structure():
+    lib = ops.load_ops_library()
+    x, u, out = torch.randn(3, 500, device=DEV), torch.rand(3, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    s = ops.SampleArgs(logits=x.data_ptr(), logits_stride=500, x_dtype=0, rows=3, V=500, uniform=u.data_ptr(), temperature=0.8, top_p=0.9, topk=50, out=out.data_ptr())
+    assert lib.csm_ops_sample_filtered(C.byref(s), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, sample_filtered(x, u, temperature=0.8, top_p=0.9, topk=50)[:, 0])
