@@ -3,8 +3,8 @@
 // Bound by memory: every input element is read once, every output written once, 1.5 flops per byte.  A thread owns 16 elements of one head:
 // 8 of the lower half and the 8 they rotate with (q, k), or 16 consecutive ones (v), so that both partners are in its registers and all
 // traffic is 16-byte vectors; consecutive threads take consecutive 8-element pieces of a row.
-// Measured: 98.6 MB (16 sequences of some 500 fp32 rows of 32 + 2 x 8 heads of 64) in 18.2 us, 5.4 TB/s, where a large copy reaches 4.9 with memory alone;
-// 26.9 MB of bf16 rows in 7.3 us; 96 rows in 3.3 and one in 2.3, which are a launch and four dependent reads (length, page, row).
+// Measured: 98.6 MB (4 sequences of some 2000 fp32 rows of 8 + 2 x 2 heads of 128) in 18.0 us, 5.5 TB/s, where a large copy reaches 4.9 with memory alone;
+// 26.9 MB of bf16 rows (2162 of 32 + 2 x 8 heads of 64) in 6.6 us; 96 rows in 3.5 and one in 2.4, which are a launch and four dependent reads (length, page, row).
 #include "ops_common.h"
 #include <algorithm>
 

@@ -9,10 +9,10 @@
 //   up to 16 live rows (decode): the launch waits for memory.  The four waves split the keys, each streams its own, and they join through LDS.
 //   more rows: 64-key tiles (32 fp32) of K and V are staged once per workgroup in LDS (two buffers), every wave takes 16-row tiles.
 //   more rows in a tall workgroup (below; a text among single tokens): every wave streams all keys for its 16 rows.
-// Measured: 128 sequences of some 1500 own slots behind 4096 (32 / 8 heads of 64, bf16): 416 MB in 83 + 5 us, 4.8 TB/s of the 4.9 that a large copy reaches.
-// 2 sequences of 4096 new rows: 136 GFLOP in 180 us, 755 TFLOP/s of the 1330 that a large bf16 product reaches; 2162 ragged rows behind 2048 slots 540,
+// Measured: 128 sequences of some 1500 own slots behind 4096 (32 / 8 heads of 64, bf16): 416 MB in 83 + 5 us, 4.7 TB/s of the 4.9 that a large copy reaches.
+// 2 sequences of 4096 new rows: 136 GFLOP in 184 us, 740 TFLOP/s of the 1330 that a large bf16 product reaches; 2162 ragged rows behind 2048 slots 540,
 // where 664 workgroups share 256 CUs.  Without its exponentials that launch (at 220 us) took 14 percent less, without the second product 15, without half of the
-// first 13, without fetching tiles 11: no single one bounds it.  One sequence behind 512 slots: 4.6 + 2.3 us, a chain of latencies.
+// first 13, without fetching tiles 11: no single one bounds it.  One sequence behind 512 slots: two launches in 6.9 us, a chain of latencies.
 //
 // Per wave and 16 query rows, both products are transposed so that a lane owns one query row from score to result:
 //   S^T[key][row] = K Q^T   lane (row = lane % 16, g = lane / 16) ends with the scores of keys 4g .. 4g+3 of each 16-key group
@@ -914,7 +914,7 @@ static int check(const csm_ops_attention_t* p) {
 }
 
 // How the work is cut.  Items should fill 256 CUs (of two to four workgroups each), but a short item is mostly start-up, and every piece costs a
-// partial result per row, written and read again.  Measured (us): 128 sequences behind 4096 slots, prefix in 4 / 8 / 16 pieces 86 / 88 / 96, own slots in
+// partial result per row, written and read again.  Measured (us): 128 sequences behind 4096 slots, prefix in 4 / 8 / 16 pieces 86 / 88 / 96 (one rule for all of these takes 8), own slots in
 // 1 / 2 / 3 / 5 pieces 92 / 88 / 90 / 92; 64 sequences of 128-wide heads behind 2048 slots, prefix in 4 / 8 / 16 pieces 25 / 18.5 / 22, own in 2 / 4 / 5
 // pieces 18.7 / 18.5 / 19.8; 16 fp32 sequences behind 512 slots, prefix in 4 / 8 / 16 pieces 14 / 11.4 / 11.9; tiles of many rows whole / in 3 pieces 88 / 110.
 static int plan(const csm_ops_attention_t* p, AttnOpArgs& a) {

@@ -121,7 +121,9 @@ def paged_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
     q `[rows, n_q, head_dim]` (rotated, unscaled; float32, or bfloat16 over a bfloat16 cache), rows and cache as in `paged_rope_append`, which
     has already appended the rows' own keys.  A row at slot s sees the `prefix_len` slots on the pages `prefix_table` (int32) and own slots 0 .. s.
-    The prefix is read once for the batch, not once per sequence; `prefix_len = 0` is plain paged attention.  `scale` defaults to
+    The prefix is stored once for the batch, and read once for all rows of a decode batch (sequences with 32 query rows each, and few on a short axis,
+    read it with their own slots);
+    `prefix_len = 0` is plain paged attention.  `scale` defaults to
     `head_dim ** -0.5`.  head_dim is 64 or 128, n_q any multiple of n_kv.  With float32 q everything is float32; with bfloat16 q the products
     run on the bf16 matrix pipe with float32 sums, the softmax weights of the second one held in 16 bits (two bfloat16 pieces), or rounded to bfloat16
     where the sequences bring more than 16 query rows (`rows * n_q / n_kv`) each on average.
@@ -138,7 +140,8 @@ def sample_filtered(logits: torch.Tensor, uniform: torch.Tensor, *, temperature:
     """Tokens drawn from `softmax(logits / temperature)` cut by top-k, then top-p, then min-p, with ONE given uniform per row; int32 `[..., 1]`.
 
     logits `[..., V]` (float32 or bfloat16), uniform `[...]` float32 in [0, 1).  Each setting is a number, or a tensor `[...]` with one value per
-    row (float32; int32 for topk).  Entries are ordered by value, equal ones by index; the kept ones are the first `topk` (0 = all), of these
+    row (float32; int32 for topk).  Numbers are checked: `0 <= temperature < inf`, `0 <= topk <= V`, `0 < top_p <= 1`, `0 <= min_p <= 1`; of a tensor's
+    values any is taken, topk <= 0 or >= V, top_p >= 1 and min_p <= 0 as off, others as the nearest that can be used.  Entries are ordered by value, equal ones by index; the kept ones are the first `topk` (0 = all), of these
     the fewest that reach `top_p` of their mass, of these the ones with at least `min_p` times the largest probability; the token is the first
     index at which the running sum of kept probability passes `uniform` times its total.  `temperature = 0` is the arg-max, the lowest index
     of equals, like `sample_topk`; exactly `topk` entries stay, so `topk = 1` is the arg-max too (`sample_topk` keeps every entry that ties with

@@ -76,7 +76,9 @@ int csm_ops_paged_rope_append(const csm_ops_rope_append_t* a, void* stream);
 
 /* ---- attention over a prefix shared by all rows and each sequence's own slots.  Row r of sequence b at slot s sees the prefix's
  * `prefix_len` slots (pages prefix_table[0 ..], same cache) and its own slots 0 .. s; out[r, h] = softmax(scale q.k) v over them, head h
- * reading kv head h / (n_q / n_kv).  The prefix is read once for all rows, not once per sequence.  A row that sees no key gives zeros; a
+ * reading kv head h / (n_q / n_kv).  The prefix is stored once for all sequences.  It is also read once
+ * for every 128 query rows of a kv-head (64 with fp32 q), whichever sequences they are of, except where that would not pay: sequences that bring 32
+ * query rows (rows * n_q / n_kv) each and more on average, and few sequences on a short axis, read it with their own slots.  A row that sees no key gives zeros; a
  * page number outside the cache hides its slots.  Slots that no row of the call sees may hold anything; a NaN or infinity in v of a slot
  * that some rows of a sequence see also reaches that sequence's earlier rows of the call (0 * NaN), never another sequence.  x_dtype (q and
  * out) bf16 needs a bf16 cache: products on the bf16 matrix pipe with fp32 sums; x_dtype fp32 takes either cache, fp32 throughout.
@@ -102,9 +104,10 @@ int csm_ops_paged_prefix_attention(const csm_ops_attention_t* a, void* stream);
  * min(n_k, n_p, n_m) entries: n_k = topk, n_p = the fewest whose w reach top_p of the w of the first n_k, n_m = those with w >= min_p; the
  * token is the first index (in index order) at which the running sum of kept w exceeds u times their total.  temperature 0 = arg-max, the
  * lowest index of equals.  NaN logits count as -inf; several +inf share the row equally; a row of nothing but -inf gives -1.  u outside
- * [0, 1) is clamped to it.  topk <= 0 or >= V, top_p >= 1, min_p <= 0 switch that filter off; the first entry is always kept.  The pointers
- * give one value per row and win over the scalars; NULL = the scalar for all rows.  Per-row values the kernel cannot use are read as the
- * nearest that it can (temperature < 0 or NaN: 0; top_p < 0 or NaN: 0; min_p > 1: 1, NaN: 0).  V up to 2^21.  Weights are
+ * [0, 1) is clamped to it.  The first entry is always kept.
+ * The scalars hold for all rows and are checked: 0 <= temperature < inf, 0 <= topk <= V (0 or V: off), 0 < top_p <= 1 (1: off), 0 <= min_p <= 1 (0: off).
+ * A pointer gives one value per row instead; the host does not see these, so any is taken: topk <= 0 or >= V, top_p >= 1, min_p <= 0 switch that
+ * filter off, and others are read as the nearest that can be used (temperature < 0 or NaN: 0; top_p < 0 or NaN: 0; min_p > 1: 1, NaN: 0).  V up to 2^21.  Weights are
  * computed in fp64 and summed in 64-bit fixed point, chunks of a long row in fp64 in their order: the same input gives the same token.  A weight is
  * held to 2^-49 of the row's largest, or to 2^-61 of their sum where that is more; smaller ones count as 0. */
 typedef struct {
