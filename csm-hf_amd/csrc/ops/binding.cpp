@@ -41,6 +41,7 @@ struct Call {
       throw Refused{PyExc_RuntimeError, std::string(name) + " requires a gradient: this operator has no backward pass (call it under torch.no_grad())"};
     if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
       throw Refused{PyExc_RuntimeError, std::string(name) + " has a forward-mode tangent: this operator has no derivative"};
+    if (t.layout() != at::kStrided) refuse(std::string(name) + " must be a dense tensor");
     // wrappers of function transforms (vmap, jvp) have no memory of their own; a lazily negated view holds other values than it stands for
     if (!t.has_storage()) throw Refused{PyExc_RuntimeError, std::string(name) + " is a tensor inside a function transform: this operator cannot be transformed"};
     if (t.is_neg()) refuse(std::string(name) + " is a negated view: pass its resolve_neg()");

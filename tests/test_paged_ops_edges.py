@@ -135,7 +135,7 @@ def _calls():
 
 
 @pytest.mark.gpu
-def test_tangents_transforms_and_negated_views_are_refused():
+def test_tangents_transforms_sparse_tensors_and_negated_views_are_refused():
     import torch.autograd.forward_ad as fwd
     for f, t in _calls():
         f(t)
@@ -150,6 +150,8 @@ def test_tangents_transforms_and_negated_views_are_refused():
             torch.func.jvp(f, (t,), (torch.ones_like(t),))
         with pytest.raises(RuntimeError, match="function transform"):
             torch.func.vmap(f)(t[None])
+        with pytest.raises(ValueError, match="dense"):
+            f(t.to_sparse())
         with pytest.raises(ValueError, match="negated"):
             f(torch._neg_view(t))
         f(t)
