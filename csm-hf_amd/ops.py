@@ -88,8 +88,9 @@ def _load_binding():
         except ImportError as e:
             raise RuntimeError(f"csm_hf_amd/_ops_binding.so is missing or was built against another torch ({e}): build it with `python -m csm_hf_amd.build`") from e
         from .build import binding_stamp
-        if _ops_binding.built_for != binding_stamp():
-            raise RuntimeError(f"csm_hf_amd/_ops_binding.so was built for another torch or Python ({_ops_binding.built_for!r}, here: {binding_stamp()!r}): build it with `python -m csm_hf_amd.build`")
+        built_for = getattr(_ops_binding, "built_for", None)   # (None: older than the stamp)
+        if built_for != binding_stamp():
+            raise RuntimeError(f"csm_hf_amd/_ops_binding.so was built for another torch or Python ({built_for!r}, here: {binding_stamp()!r}): build it with `python -m csm_hf_amd.build`")
         _binding = _ops_binding
     return _binding
 

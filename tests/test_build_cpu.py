@@ -94,3 +94,12 @@ def test_binding_for_another_torch_is_refused_when_loaded(monkeypatch):
     monkeypatch.setattr(torch, "__version__", "0.0.1")
     with pytest.raises(RuntimeError, match="built for another torch.*csm_hf_amd.build"):
         ops._load_binding()
+
+
+def test_binding_without_a_stamp_is_refused_when_loaded(monkeypatch):
+    monkeypatch.setattr(ops, "_binding", None)
+    ops._load_binding()
+    monkeypatch.setattr(ops, "_binding", None)
+    monkeypatch.setattr(importlib.import_module(ops.__package__), "_ops_binding", object())
+    with pytest.raises(RuntimeError, match="built for another torch.*csm_hf_amd.build"):
+        ops._load_binding()
